@@ -414,6 +414,40 @@ int llmq_adamw_update_f32(float* params, const float* grads, float* m, float* v,
                           float beta1, float beta2, int t, float eps, float weight_decay, const float* grad_scale,
                           float* abs_max_or_null, unsigned int seed, void* stream);
 
+/*
+ * Causal attention on the fused QKV tensor [B, T, Nq + 2*Nkv, head_dim] (bf16, what llmq_rope_forward_bf16 writes): query
+ * head h attends to key/value head h / (Nq / Nkv).  Query t of row b looks at the keys max(0, first_key[b, t]) <= k <= t;
+ * first_key_or_null (int32 [B, T], NULL = 0 everywhere) is the document's first token for packed documents, t - w + 1 for a
+ * sliding window of w keys, and any value above t for a row that may look at nothing (padding).
+ *     s = softmax_scale * q_t . k_k;   lse[b, h, t] = ln sum_k exp(s);   out[b, t, h] = sum_k exp(s - lse) v_k
+ * A row without keys: out = 0, lse = -inf.  Scores and sums in fp32; the probabilities are rounded to bf16 for the product
+ * with the values.  What lies in places the mask excludes never reaches a result, NaN and infinities included; where a value in
+ * an allowed place is not finite, the outputs it enters are not finite either (NaN, also where the formula gives an infinity).
+ * abs_max_or_null: reset, then max |out|, bit-identical to llmq_abs_max_bf16(out).  head_dim: a multiple of 8 up to 128;
+ * softmax_scale > 0.  out must not be qkv.
+ * Replaces: attention_forward_cudnn(nv_bfloat16* out, float* stats, const nv_bfloat16* inp, ...)  (cuDNN-frontend graphs,
+ *           src/kernels/cudnn_att.cpp) and the reference's own kernel, src/kernels/attention.cu:20 (head_dim 64 / 128).
+ */
+int llmq_attention_forward_bf16(uint16_t* out, float* lse, const uint16_t* qkv, const int* first_key_or_null,
+                                float* abs_max_or_null, float softmax_scale, int B, int T, int Nq, int Nkv, int head_dim,
+                                void* stream);
+
+/*
+ * Backward pass of the above: dqkv [B, T, Nq + 2*Nkv, head_dim] (what llmq_rope_backward_bf16 takes) from dout and the
+ * forward's out, lse, qkv and first_key.  The probabilities are recomputed from lse; with D = sum_d dout * out,
+ *     p = exp(s - lse);  ds = p (dout . v - D);  dq = scale sum_k ds k;  dk = scale sum_{h, t} ds q;  dv = sum_{h, t} p dout
+ * (sums of dk, dv over the query heads of the group).  p and ds are rounded to bf16 for their products, sums are fp32 in a
+ * fixed order (deterministic), every element of dqkv is written.  Masked places as in the forward pass.
+ * scratch: at least llmq_attention_backward_scratch_bytes(B, T, Nq, Nkv, head_dim) bytes, 16-byte aligned, overwritten by every
+ * call; calls that share it must be stream ordered.  dqkv must be a tensor of its own.
+ * Replaces: attention_backward_cudnn(nv_bfloat16* dqkvr, const float* stats, const nv_bfloat16* out, const nv_bfloat16* dout,
+ *           const nv_bfloat16* qkvr, ...)  (src/kernels/cudnn_att.cpp) and src/kernels/attention.cu:152.
+ */
+int64_t llmq_attention_backward_scratch_bytes(int B, int T, int Nq, int Nkv, int head_dim);
+int llmq_attention_backward_bf16(uint16_t* dqkv, const uint16_t* dout, const uint16_t* out, const float* lse,
+                                 const uint16_t* qkv, const int* first_key_or_null, void* scratch, size_t scratch_bytes,
+                                 float softmax_scale, int B, int T, int Nq, int Nkv, int head_dim, void* stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

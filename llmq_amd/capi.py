@@ -28,6 +28,7 @@ EXPORTS = [
     "llmq_swiglu_forward_f32", "llmq_swiglu_backward_f32", "llmq_rope_forward_f32", "llmq_rope_backward_f32",
     "llmq_precompute_freqs_cis_f32", "llmq_rmsnorm_forward_f32", "llmq_fused_residual_rmsnorm_forward_f32",
     "llmq_rmsnorm_backward_f32", "llmq_adamw_update_f32",
+    "llmq_attention_forward_bf16", "llmq_attention_backward_bf16", "llmq_attention_backward_scratch_bytes",
 ]
 
 if not os.path.exists(LIB_PATH):
@@ -79,10 +80,15 @@ for _name in ("swiglu_forward", "swiglu_backward", "rope_forward", "rope_backwar
 lib.llmq_precompute_freqs_cis_f32.argtypes = lib.llmq_precompute_freqs_cis_f16.argtypes
 lib.llmq_adamw_update_f32.argtypes = [_vp, _vp, _vp, _vp, _i64, C.c_float, C.c_float, C.c_float, _int, C.c_float, C.c_float, _vp,
                                       _vp, C.c_uint, _vp]
+lib.llmq_attention_forward_bf16.argtypes = [_vp, _vp, _vp, _vp, _vp, C.c_float, _int, _int, _int, _int, _int, _vp]
+lib.llmq_attention_backward_bf16.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _vp, C.c_size_t, C.c_float, _int, _int, _int, _int,
+                                             _int, _vp]
+lib.llmq_attention_backward_scratch_bytes.argtypes = [_int, _int, _int, _int, _int]
 for _name in EXPORTS[3:]:
     getattr(lib, _name).restype = _int
 lib.llmq_backward_bias_scratch_bytes.restype = _i64
 lib.llmq_rmsnorm_backward_scratch_bytes.restype = _i64
+lib.llmq_attention_backward_scratch_bytes.restype = _i64
 
 LLMQ_OK, LLMQ_ERR_INVALID_ARGUMENT, LLMQ_ERR_RUNTIME = 0, 1, 2
 

@@ -22,6 +22,9 @@ Names, argument order and in-place "out first" convention are the reference's:
     precompute_freqs_cis(dim, end, theta)
     adamw_update(params, grads, m, v, learning_rate, beta1, beta2, t, eps, weight_decay, grad_scale, m_scales=None,
                  abs_max=None, seed=0, stream=0)
+    attention_forward(out, lse, qkv, abs_max, Nq, Nkv, first_key=None, softmax_scale=None, stream=0)
+    attention_backward(dqkv, dout, out, lse, qkv, scratch, Nq, Nkv, first_key=None, softmax_scale=None, stream=0)
+    get_attention_backward_scratch_size(B, T, Nq, Nkv, HD)
 `stream` is a raw hipStream_t handle (0 = torch's current stream).
 """
 import torch
@@ -392,3 +395,74 @@ def adamw_update(params, grads, m, v, learning_rate, beta1, beta2, t, eps, weigh
     capi.check(capi.lib.llmq_adamw_update_bf16(p, g, pm, int(m.dtype == torch.bfloat16), pv, int(v.dtype == torch.bfloat16), n,
                                                float(learning_rate), float(beta1), float(beta2), int(t), float(eps),
                                                float(weight_decay), gs, a, int(seed) & 0xFFFFFFFF, _stream(stream)))
+
+
+def _launch_context(stream, *tensors):
+    """(context, stream handle) for a call on `tensors`, which must share a device: the call runs on that device, on
+    `stream` or the device's current stream, whatever the current device is."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if dev is not None and t.device != dev:
+            raise ValueError("all tensors must be on one device (got %s and %s)" % (dev, t.device))
+        dev = t.device
+    return torch.cuda.device(dev), stream if stream else torch.cuda.current_stream(dev).cuda_stream
+
+
+def _attention_dims(qkv, per_query, Nq, Nkv, first_key, softmax_scale):
+    """(B, T, head_dim, scale) of qkv [B, T, (Nq + 2 Nkv) HD]; per_query: name -> tensor [B, T, Nq HD]."""
+    if qkv.dim() != 3:
+        raise ValueError("qkv must be [B, T, (Nq + 2 Nkv) * head_dim]")
+    if Nq <= 0 or Nkv <= 0 or Nq % Nkv or qkv.shape[2] % (Nq + 2 * Nkv):
+        raise ValueError("qkv must be [B, T, (Nq + 2 Nkv) * head_dim] with Nq a multiple of Nkv")
+    B, T, HD = int(qkv.shape[0]), int(qkv.shape[1]), int(qkv.shape[2]) // (Nq + 2 * Nkv)
+    for name, t in per_query.items():
+        if tuple(t.shape) != (B, T, Nq * HD):
+            raise ValueError("%s must be [B, T, Nq * head_dim]" % name)
+    if first_key is not None and tuple(first_key.shape) != (B, T):
+        raise ValueError("first_key must be [B, T]")
+    return B, T, HD, float(softmax_scale) if softmax_scale is not None else max(HD, 1) ** -0.5
+
+
+def attention_forward(out, lse, qkv, abs_max, Nq, Nkv, first_key=None, softmax_scale=None, stream=0):
+    """Causal attention on the fused QKV tensor [B, T, (Nq + 2 Nkv) * HD] (bf16, what rope_forward writes): out [B, T, Nq * HD]
+    bf16 and lse [B, Nq, T] fp32; abs_max (fp32 device scalar or None) receives max |out|.  Query t of row b looks at the keys
+    max(0, first_key[b, t]) .. t (first_key: int32 [B, T] or None for 0): the document's first token for packed documents,
+    t - w + 1 for a sliding window, any value above t for a row that looks at nothing (out 0, lse -inf).
+    softmax_scale: 1 / sqrt(HD) unless given.  HD: a multiple of 8 up to 128."""
+    B, T, HD, scale = _attention_dims(qkv, {"out": out}, Nq, Nkv, first_key, softmax_scale)
+    if tuple(lse.shape) != (B, Nq, T):
+        raise ValueError("lse must be [B, Nq, T]")
+    bf, f32 = (torch.bfloat16,), (torch.float32,)
+    o, l, x = _dev(out, "out", bf), _dev(lse, "lse", f32), _dev(qkv, "qkv", bf)
+    f = _dev(first_key, "first_key", (torch.int32,), optional=True)
+    a = _dev(abs_max, "abs_max", f32, optional=True)
+    ctx, st = _launch_context(stream, qkv, out, lse, first_key, abs_max)
+    with ctx:
+        capi.check(capi.lib.llmq_attention_forward_bf16(o, l, x, f, a, scale, B, T, int(Nq), int(Nkv), HD, st))
+
+
+def get_attention_backward_scratch_size(B, T, Nq, Nkv, HD):
+    """Bytes of scratch attention_backward needs for these sizes."""
+    return int(capi.lib.llmq_attention_backward_scratch_bytes(int(B), int(T), int(Nq), int(Nkv), int(HD)))
+
+
+def attention_backward(dqkv, dout, out, lse, qkv, scratch, Nq, Nkv, first_key=None, softmax_scale=None, stream=0):
+    """Gradient of attention_forward: dqkv (shape of qkv, every element written) from dout and the forward's out, lse, qkv,
+    first_key and softmax_scale.  scratch: a device tensor of at least get_attention_backward_scratch_size(B, T, Nq, Nkv, HD)
+    bytes; calls that share it must be stream ordered.  Deterministic."""
+    B, T, HD, scale = _attention_dims(qkv, {"out": out, "dout": dout}, Nq, Nkv, first_key, softmax_scale)
+    if dqkv.shape != qkv.shape:
+        raise ValueError("dqkv must have the shape of qkv")
+    if tuple(lse.shape) != (B, Nq, T):
+        raise ValueError("lse must be [B, Nq, T]")
+    bf, f32 = (torch.bfloat16,), (torch.float32,)
+    d, g, o, x = _dev(dqkv, "dqkv", bf), _dev(dout, "dout", bf), _dev(out, "out", bf), _dev(qkv, "qkv", bf)
+    l = _dev(lse, "lse", f32)
+    f = _dev(first_key, "first_key", (torch.int32,), optional=True)
+    s = _dev(scratch, "scratch")
+    ctx, st = _launch_context(stream, qkv, dqkv, dout, out, lse, first_key, scratch)
+    with ctx:
+        capi.check(capi.lib.llmq_attention_backward_bf16(d, g, o, l, x, f, s, scratch.numel() * scratch.element_size(), scale, B, T,
+                                                         int(Nq), int(Nkv), HD, st))

@@ -22,6 +22,9 @@ order, defaults and mutation declarations on top of the gfx950 C ABI, so code wr
     adamw_update(params, grads, m, v, learning_rate, beta1, beta2, t, eps, weight_decay, grad_scale, m_scales=None,
                  abs_max=None, seed=0, stream=0)
     rope_forward(out, inp, freqs_cis, absmax=None, Nq, Nkv, stream=0);  rope_backward(dinp, dout, freqs_cis, absmax=None, Nq, Nkv, stream=0)
+    attention_forward(out, lse, inp, absmax=None, Nq, Nkv, first_key=None, softmax_scale=0, stream=0)
+    attention_backward(dinp, dout, out, lse, inp, scratch, Nq, Nkv, first_key=None, softmax_scale=0, stream=0)
+    get_attention_backward_scratch_size(B, T, Nq, Nkv, HD)
 
 matmul is in the torch sense (c = op(a) @ op(b), mode: TT=0, TN=1, NT=2, NN=3).  FP8 operands are served in
 mode NT (c[M,N] = a[M,K] @ b[N,K]^T, both K-contiguous: every shape with K % 16 == 0) and, for bf16 output on
@@ -142,6 +145,23 @@ def adamw_update(params: torch.Tensor, grads: torch.Tensor, m: torch.Tensor, v: 
                  stream: int = 0) -> None:
     _k.adamw_update(params, grads, m, v, learning_rate, beta1, beta2, t, eps, weight_decay, grad_scale, m_scales, abs_max,
                     seed, stream)
+
+
+@torch.library.custom_op("llmq::attention_forward", mutates_args=("out", "lse", "absmax"))
+def attention_forward(out: torch.Tensor, lse: torch.Tensor, inp: torch.Tensor, absmax: torch.Tensor | None = None, Nq: int = 0,
+                      Nkv: int = 0, first_key: torch.Tensor | None = None, softmax_scale: float = 0.0, stream: int = 0) -> None:
+    _k.attention_forward(out, lse, inp, absmax, Nq, Nkv, first_key, softmax_scale or None, stream)
+
+
+@torch.library.custom_op("llmq::attention_backward", mutates_args=("dinp", "scratch"))
+def attention_backward(dinp: torch.Tensor, dout: torch.Tensor, out: torch.Tensor, lse: torch.Tensor, inp: torch.Tensor,
+                       scratch: torch.Tensor, Nq: int, Nkv: int, first_key: torch.Tensor | None = None,
+                       softmax_scale: float = 0.0, stream: int = 0) -> None:
+    _k.attention_backward(dinp, dout, out, lse, inp, scratch, Nq, Nkv, first_key, softmax_scale or None, stream)
+
+
+def get_attention_backward_scratch_size(B: int, T: int, Nq: int, Nkv: int, HD: int):
+    return _k.get_attention_backward_scratch_size(B, T, Nq, Nkv, HD)
 
 
 def get_rmsnorm_backward_scratch_size(C: int):
