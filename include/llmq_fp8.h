@@ -448,6 +448,45 @@ int llmq_attention_backward_bf16(uint16_t* dqkv, const uint16_t* dout, const uin
                                  const uint16_t* qkv, const int* first_key_or_null, void* scratch, size_t scratch_bytes,
                                  float softmax_scale, int B, int T, int Nq, int Nkv, int head_dim, void* stream);
 
+/*
+ * Log probabilities of given tokens.  logits: N rows of V values, P >= V elements apart (padded vocabulary: columns V .. P-1
+ * are not looked at); targets: int32 [N].  Per row:
+ *     lse = ln sum_v exp(x_v);  logp = x_t - lse (0 where t is not in [0, V): an ignored row);
+ *     entropy_or_null = lse - sum_v p_v x_v;
+ *     top_logp / top_ids [N, k]: the k largest x_v - lse in falling order and their columns, equal values by column; k = 0: not
+ *     wanted (pointers may be NULL), k <= 32.  With V < k, or NaN among the logits, the places left over hold -1 and -inf
+ *     (NaN where lse is NaN).
+ * -inf logits (banned tokens) have probability 0 and add nothing; a row of nothing else has lse and logp -inf and entropy 0.  A
+ * row that holds NaN or +inf has NaN for lse, logp and entropy.  All sums fp32 in a fixed order (deterministic).
+ * scratch: at least llmq_token_logprobs_scratch_bytes(N, V, k) bytes (0 for many rows: may be NULL), 16-byte aligned,
+ * overwritten by every call; calls that share it must be stream ordered.  logits 16-byte aligned, any P.
+ * Counterpart in the reference: the loss half of fused_classifier, src/kernels/fused_classifier.cu:92,246 (one target a row).
+ */
+int64_t llmq_token_logprobs_scratch_bytes(int64_t N, int V, int k);
+int llmq_token_logprobs_bf16(float* logp, float* entropy_or_null, float* lse, float* top_logp, int* top_ids,
+                             const uint16_t* logits, const int* targets, void* scratch, size_t scratch_bytes, int64_t N, int V,
+                             int64_t P, int k, void* stream);
+int llmq_token_logprobs_f32(float* logp, float* entropy_or_null, float* lse, float* top_logp, int* top_ids,
+                            const float* logits, const int* targets, void* scratch, size_t scratch_bytes, int64_t N, int V,
+                            int64_t P, int k, void* stream);
+
+/*
+ * Gradient of logp and entropy with respect to the logits, in their type:
+ *     dlogits[v] = dlogp (1[v = t] - p_v) - dentropy p_v (x_v - lse + entropy),   p_v = exp(x_v - lse)
+ * rounded once; columns V .. P-1 are written as zeros.  lse (and, with dentropy, entropy) are the forward's.  dlogp counts as 0
+ * for an ignored row; a row whose two gradients are 0 is written as zeros whatever its logits hold (padding), and so is a row
+ * whose lse is -inf.
+ * dlogits may be logits (in place).  abs_max_or_null: reset, then max |dlogits| over all columns, bit-identical to llmq_abs_max
+ * of the tensor.  The loss -mean logp has dlogp = -1 / N.
+ * Counterpart in the reference: the gradient half of fused_classifier, src/kernels/fused_classifier.cu:92.
+ */
+int llmq_token_logprobs_backward_bf16(uint16_t* dlogits, const float* dlogp, const float* dentropy_or_null,
+                                      const uint16_t* logits, const int* targets, const float* lse, const float* entropy_or_null,
+                                      float* abs_max_or_null, int64_t N, int V, int64_t P, void* stream);
+int llmq_token_logprobs_backward_f32(float* dlogits, const float* dlogp, const float* dentropy_or_null, const float* logits,
+                                     const int* targets, const float* lse, const float* entropy_or_null, float* abs_max_or_null,
+                                     int64_t N, int V, int64_t P, void* stream);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

@@ -29,6 +29,8 @@ EXPORTS = [
     "llmq_precompute_freqs_cis_f32", "llmq_rmsnorm_forward_f32", "llmq_fused_residual_rmsnorm_forward_f32",
     "llmq_rmsnorm_backward_f32", "llmq_adamw_update_f32",
     "llmq_attention_forward_bf16", "llmq_attention_backward_bf16", "llmq_attention_backward_scratch_bytes",
+    "llmq_token_logprobs_bf16", "llmq_token_logprobs_f32", "llmq_token_logprobs_scratch_bytes",
+    "llmq_token_logprobs_backward_bf16", "llmq_token_logprobs_backward_f32",
 ]
 
 if not os.path.exists(LIB_PATH):
@@ -84,11 +86,17 @@ lib.llmq_attention_forward_bf16.argtypes = [_vp, _vp, _vp, _vp, _vp, C.c_float, 
 lib.llmq_attention_backward_bf16.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _vp, C.c_size_t, C.c_float, _int, _int, _int, _int,
                                              _int, _vp]
 lib.llmq_attention_backward_scratch_bytes.argtypes = [_int, _int, _int, _int, _int]
+lib.llmq_token_logprobs_bf16.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, C.c_size_t, _i64, _int, _i64, _int, _vp]
+lib.llmq_token_logprobs_f32.argtypes = lib.llmq_token_logprobs_bf16.argtypes
+lib.llmq_token_logprobs_scratch_bytes.argtypes = [_i64, _int, _int]
+lib.llmq_token_logprobs_backward_bf16.argtypes = [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _int, _i64, _vp]
+lib.llmq_token_logprobs_backward_f32.argtypes = lib.llmq_token_logprobs_backward_bf16.argtypes
 for _name in EXPORTS[3:]:
     getattr(lib, _name).restype = _int
 lib.llmq_backward_bias_scratch_bytes.restype = _i64
 lib.llmq_rmsnorm_backward_scratch_bytes.restype = _i64
 lib.llmq_attention_backward_scratch_bytes.restype = _i64
+lib.llmq_token_logprobs_scratch_bytes.restype = _i64
 
 LLMQ_OK, LLMQ_ERR_INVALID_ARGUMENT, LLMQ_ERR_RUNTIME = 0, 1, 2
 

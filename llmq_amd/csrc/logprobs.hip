@@ -1,0 +1,571 @@
+// Log probabilities of given tokens with entropy and the k most likely tokens, and their gradient, for gfx950.
+//
+// Per row of logits x[0 .. V) (bf16 or fp32; rows are P >= V elements apart) and its token t:
+//     lse = ln sum_v exp(x_v);  logp = x_t - lse;  entropy = lse - sum_v p_v x_v,  p_v = exp(x_v - lse)
+//     dx_v = dlogp (1[v = t] - p_v) - dentropy p_v (x_v - lse + entropy)
+// (The reference's counterpart is its fused classifier, src/kernels/fused_classifier.cu:92,246,307: loss and gradient of one
+// target per row; entropy and alternatives have none.)
+//
+// HBM bound: the forward reads the logits once (2 or 4 bytes each), the gradient reads and writes them once.
+//
+// Forward: one pass with a running reference r and sums in base 2.  With d = (x - r) log2 e,
+//     s = sum 2^d,   w = sum d 2^d,   lse = r + log2(s) ln 2,   entropy = (log2 s - w / s) ln 2.
+// A lane's reference only follows a logit that has outgrown it by 11 (a factor of 6e4), so the sums are rarely rescaled; fp32
+// sums lose nothing by a common factor.  x - r is formed first: exact for neighbours, and no logit overflows, the type's lowest
+// value (a common mask) included.
+//
+// The k most likely tokens need no second pass over the row: each lane keeps the largest logit of its granules of 16 bytes and
+// the first granule that holds it.  The k-th best of the lanes' (value, granule) pairs bounds the k-th best logit from below, and
+// only the k lanes that reach it can hold one of the k: their granules alone are read again, from the caches.
+#include "common.hpp"
+#include "absmax_reduce.hpp"
+
+namespace llmq {
+
+typedef float f32x2_lp __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_lp __attribute__((ext_vector_type(2)));
+
+constexpr int kLpThreads = 256, kTopMax = 32, kCandidates = 1024, kSplitMax = 64;
+constexpr float kLog2eLp = 1.44269504088896340736f, kLn2Lp = 0.69314718055994530942f;
+
+struct LogprobArgs {
+    const void* logits;
+    const int* targets;
+    float *logp, *entropy, *lse;       // entropy may be NULL
+    float* top_logp;                   // [N, k]
+    int* top_ids;
+    void* scratch;                     // splits > 1: per (row, split) r, s, w, then per (row, split) k keys
+    int64_t P;
+    int N, V, k, splits;
+};
+
+struct LogprobGradArgs {
+    void* dlogits;
+    const void* logits;
+    const float *dlogp, *dentropy;     // dentropy (and entropy) may be NULL
+    const int* targets;
+    const float *lse, *entropy;
+    unsigned* abs_max;
+    int64_t P, items;
+    int N, V, chunks;
+};
+
+// 16 bytes of logits as floats, and back.
+template <typename E> struct Granule;
+template <> struct Granule<uint16_t> {
+    static constexpr int kN = 8;
+    static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[8]) {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[2 * i] = bf16_lo(w[i]), x[2 * i + 1] = bf16_hi(w[i]);
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&x)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x2_lp p = {x[2 * i], x[2 * i + 1]};
+            w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(p, bf16x2_lp));
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    static __device__ __forceinline__ float one(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+    static __device__ __forceinline__ uint16_t round(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
+};
+template <> struct Granule<float> {
+    static constexpr int kN = 4;
+    static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[4]) {
+        x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&x)[4]) {
+        return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+    }
+    static __device__ __forceinline__ float one(float v) { return v; }
+    static __device__ __forceinline__ float round(float x) { return x; }
+};
+
+// The granules of a row: 16-byte aligned pieces, the first and the last of which may be partly outside [0, n).  Where rows
+// are not multiples of 16 bytes apart, they begin inside a granule.
+template <typename E>
+struct Row {
+    const E* p;
+    int lead, n, granules;   // elements of granule 0 before the row, elements of the row
+
+    __device__ __forceinline__ Row(const void* base, int64_t at, int n_) : p(static_cast<const E*>(base) + at), n(n_) {
+        lead = (int)((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(E));
+        granules = (lead + n + Granule<E>::kN - 1) / Granule<E>::kN;
+    }
+    __device__ __forceinline__ int first(int g) const { return g * Granule<E>::kN - lead; }
+    __device__ __forceinline__ bool whole(int g) const { return first(g) >= 0 && first(g) + Granule<E>::kN <= n; }
+    __device__ __forceinline__ uint4 load(int g) const { return *reinterpret_cast<const uint4*>(p + first(g)); }
+    // the granule's values, -inf outside the row
+    __device__ __forceinline__ void values(int g, float (&x)[Granule<E>::kN]) const {
+        if (whole(g)) {
+            Granule<E>::unpack(load(g), x);
+        } else {
+#pragma unroll
+            for (int j = 0; j < Granule<E>::kN; ++j) {
+                const int e = first(g) + j;
+                x[j] = e >= 0 && e < n ? Granule<E>::one(p[e]) : -__builtin_huge_valf();
+            }
+        }
+    }
+};
+
+// Order-preserving integer of a float, 0 for NaN (which is never among the k); -0 counts as +0.
+__device__ __forceinline__ uint32_t order_of(float x) {
+    if (x != x) return 0;
+    const uint32_t b = __float_as_uint(x + 0.f);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o); }
+// larger: a larger value, or the same at a lower place; 0: nothing
+__device__ __forceinline__ uint64_t key_of(uint32_t order, uint32_t place) { return order ? (uint64_t)order << 32 | (uint32_t)~place : 0; }
+
+struct Sums {
+    float r, s, w;   // reference (-inf: nothing yet), sum, weighted sum
+};
+__device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
+    Sums c;
+    c.r = __builtin_fmaxf(a.r, b.r);
+    const float ref = c.r == -__builtin_huge_valf() ? 0.f : c.r;
+    const float da = __builtin_fmaxf((a.r - ref) * kLog2eLp, -1e4f), db = __builtin_fmaxf((b.r - ref) * kLog2eLp, -1e4f);
+    const float fa = __builtin_amdgcn_exp2f(da), fb = __builtin_amdgcn_exp2f(db);
+    c.s = a.s * fa + b.s * fb;
+    c.w = (a.w + da * a.s) * fa + (b.w + db * b.s) * fb;
+    return c;
+}
+
+__device__ __forceinline__ float lse_of(const Sums& t) { return t.s == 0.f ? -__builtin_huge_valf() : t.r + __builtin_amdgcn_logf(t.s) * kLn2Lp; }
+
+// What one thread writes for a row.
+__device__ __forceinline__ float write_row(const LogprobArgs& a, int row, const Sums& t, float target, bool given) {
+    const float lse = lse_of(t);
+    a.lse[row] = lse;
+    a.logp[row] = !given ? 0.f : lse == -__builtin_huge_valf() ? lse : target - lse;
+    if (a.entropy) a.entropy[row] = t.s == 0.f ? 0.f : (__builtin_amdgcn_logf(t.s) - t.w / t.s) * kLn2Lp;
+    return lse;
+}
+
+// One row (splits == 1) or one share of its granules per workgroup.
+template <typename E, bool ENTROPY, bool TOP>
+__global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs a) {
+    constexpr int kN = Granule<E>::kN, kWaves = kLpThreads / kWave;
+    __shared__ Sums wave_sums[kWaves];
+    __shared__ float shared_lse;
+    const int tid = threadIdx.x, row = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
+    const Row<E> x(a.logits, row * a.P, a.V);
+    const int g0 = (int)((int64_t)x.granules * split / a.splits), g1 = (int)((int64_t)x.granules * (split + 1) / a.splits);
+
+    Sums t = {-__builtin_huge_valf(), 0.f, 0.f};
+    float ref = 0.f, best = __builtin_nanf("");
+    int best_g = 0;
+    auto take = [&](const float (&v)[kN], int g) {
+        float top = v[0];
+#pragma unroll
+        for (int j = 1; j < kN; ++j) top = __builtin_fmaxf(top, v[j]);
+        if constexpr (TOP) {
+            if (top > best || best != best) best = top, best_g = g;   // NaN: nothing yet
+        }
+        if (__any(top > t.r + 11.f)) {
+            const float next = __builtin_fmaxf(t.r, top);
+            if (next > -__builtin_huge_valf()) {
+                const float d = __builtin_fmaxf((t.r - next) * kLog2eLp, -1e4f), f = __builtin_amdgcn_exp2f(d);
+                t.w = (t.w + d * t.s) * f;
+                t.s *= f;
+                t.r = ref = next;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kN; ++j) {
+            const float d = (v[j] - ref) * kLog2eLp, e = __builtin_amdgcn_exp2f(d);
+            t.s += e;
+            if constexpr (ENTROPY) t.w = __builtin_fmaf(__builtin_fmaxf(d, -1e4f), e, t.w);   // 0 times -inf is nothing
+        }
+    };
+    // whole granules w0 .. w1 - 1, four loads in flight per lane; a lane walks its granules in rising order
+    const int w0 = g0 + (g0 < g1 && !x.whole(g0) ? 1 : 0), w1 = g1 - (w0 < g1 && !x.whole(g1 - 1) ? 1 : 0);
+    if (w0 > g0 && tid == 0) {
+        float v[kN];
+        x.values(g0, v);
+        take(v, g0);
+    }
+    int g = w0 + tid;
+    for (; g + 3 * kLpThreads < w1; g += 4 * kLpThreads) {
+        uint4 q[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) q[u] = x.load(g + u * kLpThreads);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            float v[kN];
+            Granule<E>::unpack(q[u], v);
+            take(v, g + u * kLpThreads);
+        }
+    }
+    for (; g < w1; g += kLpThreads) {
+        float v[kN];
+        Granule<E>::unpack(x.load(g), v);
+        take(v, g);
+    }
+    if (w1 < g1 && (g1 - 1 - w0) % kLpThreads == tid) {
+        float v[kN];
+        x.values(g1 - 1, v);
+        take(v, g1 - 1);
+    }
+
+    Sums all = t;
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) {
+        const Sums o = {__shfl_xor(all.r, off, kWave), __shfl_xor(all.s, off, kWave), __shfl_xor(all.w, off, kWave)};
+        // the lower lane's first: both lanes of a pair get the same sum
+        all = (tid & off) ? join(o, all) : join(all, o);
+    }
+    if (tid % kWave == 0) wave_sums[tid / kWave] = all;
+    __syncthreads();
+    if (tid == 0) {
+        all = wave_sums[0];
+        for (int w = 1; w < kWaves; ++w) all = join(all, wave_sums[w]);
+        if (a.splits == 1) {
+            const int target = a.targets[row];
+            const bool given = target >= 0 && target < a.V;
+            shared_lse = write_row(a, row, all, given ? Granule<E>::one(x.p[target]) : 0.f, given);
+        } else {
+            static_cast<Sums*>(a.scratch)[blockIdx.x] = all;
+        }
+    }
+
+    if constexpr (TOP) {
+        __shared__ uint64_t keys[kLpThreads];
+        __shared__ uint64_t list[kCandidates];
+        __shared__ int chosen[kTopMax];
+        __shared__ int count, lanes;
+        __shared__ uint64_t floor_key;
+        const uint64_t mine = key_of(order_of(best), (uint32_t)best_g);
+        keys[tid] = mine;
+        if (tid == 0) count = 0, lanes = 0, floor_key = 1;
+        __syncthreads();
+        int rank = 0;
+        for (int i = 0; i < kLpThreads; ++i) rank += keys[i] > mine;
+        if (mine && rank < a.k) {
+            chosen[rank] = tid;
+            atomicAdd(&lanes, 1);
+            if (rank == a.k - 1) floor_key = mine;
+        }
+        __syncthreads();
+        const uint64_t bound = floor_key;
+        const int turns = (w1 - w0 + kLpThreads - 1) / kLpThreads + 2;   // and the two cut granules
+        for (int i = tid; i < lanes * turns; i += kLpThreads) {
+            const int lane = chosen[i / turns], turn = i % turns;
+            int at = w0 + lane + turn * kLpThreads;
+            if (turn == turns - 1) {
+                if (!(w1 < g1 && (g1 - 1 - w0) % kLpThreads == lane)) continue;
+                at = g1 - 1;
+            } else if (turn == turns - 2) {
+                if (!(w0 > g0 && lane == 0)) continue;
+                at = g0;
+            } else if (at >= w1) {
+                continue;
+            }
+            float v[kN];
+            x.values(at, v);
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+                const int e = x.first(at) + j;
+                const uint32_t o = order_of(v[j]);
+                if (e >= 0 && e < x.n && o && key_of(o, (uint32_t)at) >= bound) {
+                    const int slot = atomicAdd(&count, 1);
+                    if (slot < kCandidates) list[slot] = key_of(o, (uint32_t)e);
+                }
+            }
+        }
+        __syncthreads();
+        uint64_t* partial = reinterpret_cast<uint64_t*>(static_cast<char*>(a.scratch) + ((int64_t)a.N * a.splits * sizeof(Sums) + 15) / 16 * 16) +
+                            (int64_t)blockIdx.x * a.k;
+        auto put = [&](int at, uint64_t key) {
+            if (a.splits > 1) {
+                partial[at] = key;
+            } else {
+                const bool some = key != 0;
+                a.top_ids[(int64_t)row * a.k + at] = some ? (int)~(uint32_t)key : -1;
+                const float v = some ? value_of((uint32_t)(key >> 32)) : -__builtin_huge_valf();
+                a.top_logp[(int64_t)row * a.k + at] = v == -__builtin_huge_valf() && shared_lse == shared_lse ? v : v - shared_lse;
+            }
+        };
+        if (count <= kCandidates) {
+            const int n = count;
+            for (int i = tid; i < n; i += kLpThreads) {
+                const uint64_t key = list[i];
+                int at = 0;
+                for (int j = 0; j < n; ++j) at += list[j] > key;
+                if (at < a.k) put(at, key);
+            }
+            for (int i = n + tid; i < a.k; i += kLpThreads) put(i, 0);
+        } else {
+            // Very many logits between the bound and the k-th best, all in the chosen lanes: one round over the share per token.
+            uint64_t last = ~0ull;
+            for (int round = 0; round < a.k; ++round) {
+                uint64_t top = 0;
+                for (int at = g0 + tid; at < g1; at += kLpThreads) {
+                    float v[kN];
+                    x.values(at, v);
+#pragma unroll
+                    for (int j = 0; j < kN; ++j) {
+                        const int e = x.first(at) + j;
+                        const uint64_t key = e >= 0 && e < x.n ? key_of(order_of(v[j]), (uint32_t)e) : 0;
+                        if (key < last && key > top) top = key;
+                    }
+                }
+                __syncthreads();
+                keys[tid] = top;
+                __syncthreads();
+                for (int half = kLpThreads / 2; half > 0; half >>= 1) {
+                    if (tid < half && keys[tid + half] > keys[tid]) keys[tid] = keys[tid + half];
+                    __syncthreads();
+                }
+                last = keys[0];
+                if (tid == 0) put(round, last);
+                if (last == 0) {
+                    for (int i = round + 1 + tid; i < a.k; i += kLpThreads) put(i, 0);
+                    break;
+                }
+            }
+        }
+    }
+}
+
+// Joins the shares of a row, in their order.
+template <typename E>
+__global__ __launch_bounds__(kLpThreads) void token_logprobs_join_kernel(LogprobArgs a) {
+    __shared__ uint64_t keys[kSplitMax * kTopMax];
+    __shared__ float shared_lse;
+    const int tid = threadIdx.x, row = blockIdx.x;
+    const Sums* sums = static_cast<const Sums*>(a.scratch) + (int64_t)row * a.splits;
+    if (tid < kWave) {
+        Sums t = {-__builtin_huge_valf(), 0.f, 0.f};
+        if (tid < a.splits) t = sums[tid];
+#pragma unroll
+        for (int off = 1; off < kWave; off <<= 1) {
+            const Sums o = {__shfl_xor(t.r, off, kWave), __shfl_xor(t.s, off, kWave), __shfl_xor(t.w, off, kWave)};
+            t = (tid & off) ? join(o, t) : join(t, o);
+        }
+        if (tid == 0) {
+            const int target = a.targets[row];
+            const bool given = target >= 0 && target < a.V;
+            const E* p = static_cast<const E*>(a.logits) + row * a.P;
+            shared_lse = write_row(a, row, t, given ? Granule<E>::one(p[target]) : 0.f, given);
+        }
+    }
+    if (a.k == 0) return;
+    const int n = a.splits * a.k;
+    const uint64_t* partial = reinterpret_cast<const uint64_t*>(static_cast<const char*>(a.scratch) + ((int64_t)a.N * a.splits * sizeof(Sums) + 15) / 16 * 16) +
+                              (int64_t)row * n;
+    for (int i = tid; i < n; i += kLpThreads) keys[i] = partial[i];
+    __syncthreads();
+    for (int i = tid; i < n; i += kLpThreads) {
+        const uint64_t key = keys[i];
+        // nothing: behind all keys, in the order of the places
+        int at = 0;
+        for (int j = 0; j < n && at < a.k; ++j) at += keys[j] > key || (keys[j] == key && j < i);
+        if (at >= a.k) continue;
+        a.top_ids[(int64_t)row * a.k + at] = key ? (int)~(uint32_t)key : -1;
+        const float v = key ? value_of((uint32_t)(key >> 32)) : -__builtin_huge_valf();
+        a.top_logp[(int64_t)row * a.k + at] = v == -__builtin_huge_valf() && shared_lse == shared_lse ? v : v - shared_lse;
+    }
+}
+
+// ---- gradient --------------------------------------------------------------------------------------------------------------
+constexpr int kGradTurns = 4;   // granules of a lane per item
+
+template <typename E, bool ENTROPY, bool ABSMAX>
+__global__ __launch_bounds__(kLpThreads) void token_logprobs_backward_kernel(LogprobGradArgs a) {
+    constexpr int kN = Granule<E>::kN;
+    const int tid = threadIdx.x;
+    uint32_t fold = sizeof(E) == 2 ? 0x7F807F80u : 0x7F800000u;
+    for (int64_t item = blockIdx.x; item < a.items; item += gridDim.x) {
+        const int row = (int)(item / a.chunks), chunk = (int)(item % a.chunks);
+        const Row<E> x(a.logits, row * a.P, (int)a.P);
+        E* out = static_cast<E*>(a.dlogits) + row * a.P;
+        const int target = a.targets[row];
+        const bool given = target >= 0 && target < a.V;
+        const float lse = a.lse[row], g = given ? a.dlogp[row] : 0.f;
+        float h = 0.f, shift = 0.f;
+        if constexpr (ENTROPY) h = a.dentropy[row], shift = a.entropy[row];
+        // no gradient enters, or the row has no probability: zeros, whatever the logits hold
+        const bool none = (g == 0.f && h == 0.f) || lse == -__builtin_huge_valf();
+        auto derive = [&](float v, int e) {
+            const float d = v - lse, p = __builtin_amdgcn_exp2f(d * kLog2eLp);
+            float c = -g;
+            if constexpr (ENTROPY) c -= h * (__builtin_fmaxf(d, -1e4f) + shift);
+            float r = p * c;
+            if (e == target) r += g;
+            return none || e >= a.V ? 0.f : r;
+        };
+        const int at0 = chunk * (kLpThreads * kGradTurns) + tid;
+        uint4 q[kGradTurns];
+        if (!none) {
+#pragma unroll
+            for (int u = 0; u < kGradTurns; ++u) {
+                const int at = at0 + u * kLpThreads;
+                if (at < x.granules && x.whole(at)) q[u] = x.load(at);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kGradTurns; ++u) {
+            const int at = at0 + u * kLpThreads;
+            if (at >= x.granules) continue;
+            const int e0 = x.first(at);
+            if (x.whole(at)) {
+                float v[kN];
+                if (none) {
+#pragma unroll
+                    for (int j = 0; j < kN; ++j) v[j] = 0.f;
+                } else {
+                    Granule<E>::unpack(q[u], v);
+#pragma unroll
+                    for (int j = 0; j < kN; ++j) v[j] = derive(v[j], e0 + j);
+                }
+                const uint4 w = Granule<E>::pack(v);
+                *reinterpret_cast<uint4*>(out + e0) = w;
+                if constexpr (ABSMAX) {
+                    if constexpr (sizeof(E) == 2) fold = fold_vec(fold, w);
+                    else {
+                        const uint32_t b[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) fold = min(fold, 0x7F800000u - (b[j] & 0x7FFFFFFFu));
+                    }
+                }
+            } else {
+                for (int j = 0; j < kN; ++j) {
+                    const int e = e0 + j;
+                    if (e < 0 || e >= x.n) continue;
+                    const E r = Granule<E>::round(none ? 0.f : derive(Granule<E>::one(x.p[e]), e));
+                    out[e] = r;
+                    if constexpr (ABSMAX) {
+                        if constexpr (sizeof(E) == 2) fold = fold_bf16x2(fold, (uint32_t)__builtin_bit_cast(uint16_t, r));
+                        else fold = min(fold, 0x7F800000u - (__builtin_bit_cast(uint32_t, r) & 0x7FFFFFFFu));
+                    }
+                }
+            }
+        }
+    }
+    if constexpr (ABSMAX) {
+        if constexpr (sizeof(E) == 2) {
+            const uint32_t lo = fold & 0xFFFFu, hi = fold >> 16;
+            block_min_to_atomic_max(a.abs_max, lo < hi ? lo : hi, 0x7F80u, 16);
+        } else {
+            block_min_to_atomic_max(a.abs_max, fold, 0x7F800000u, 0);
+        }
+    }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------
+// Shares of a row: enough workgroups to fill the chip when there are few rows, each with at least 4096 logits.
+static int logprob_splits(int N, int V) {
+    int64_t s = (1024 + (int64_t)N - 1) / N;
+    const int64_t most = ((int64_t)V + 4095) / 4096;
+    s = s < most ? s : most;
+    return (int)(s < 1 ? 1 : s > kSplitMax ? kSplitMax : s);
+}
+static int64_t logprob_scratch(int N, int V, int k) {
+    const int splits = logprob_splits(N, V);
+    return splits > 1 ? ((int64_t)N * splits * (int64_t)sizeof(Sums) + 15) / 16 * 16 + (int64_t)N * splits * k * 8 : 0;
+}
+
+template <typename E>
+static int token_logprobs_any(float* logp, float* entropy, float* lse, float* top_logp, int* top_ids, const E* logits, const int* targets,
+                              void* scratch, size_t scratch_bytes, int64_t N64, int V, int64_t P, int k, hipStream_t stream) {
+    const char* what = "token_logprobs";
+    LLMQ_REQUIRE(N64 >= 0 && N64 <= (1 << 24), "%s: 0 to 2^24 rows (got %lld)", what, (long long)N64);
+    const int N = (int)N64;
+    LLMQ_REQUIRE(V >= 1 && V <= (1 << 28) && P >= V && P <= (1 << 28), "%s: vocabulary %d, row length %lld: 1 <= V <= P <= 2^28 is wanted", what, V, (long long)P);
+    LLMQ_REQUIRE(k >= 0 && k <= kTopMax, "%s: at most %d alternatives (got %d)", what, kTopMax, k);
+    if (N == 0) return LLMQ_OK;
+    LLMQ_REQUIRE(logp && lse && logits && targets, "%s: null tensor pointer", what);
+    LLMQ_REQUIRE(k == 0 || (top_logp && top_ids), "%s: alternatives need both their tensors", what);
+    LLMQ_REQUIRE(aligned16(logits), "%s: logits must be 16-byte aligned", what);
+    const int64_t need = logprob_scratch(N, V, k);
+    LLMQ_REQUIRE(need == 0 || (scratch && aligned16(scratch) && scratch_bytes >= (size_t)need), "%s: scratch buffer too small or not 16-byte aligned (%zu bytes, %lld needed)",
+                 what, scratch_bytes, (long long)need);
+    LogprobArgs a = {};
+    a.logits = logits, a.targets = targets, a.logp = logp, a.entropy = entropy, a.lse = lse, a.top_logp = top_logp, a.top_ids = top_ids;
+    a.scratch = scratch, a.P = P, a.N = N, a.V = V, a.k = k, a.splits = logprob_splits(N, V);
+    auto launch = [&](auto kernel, int64_t blocks) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kLpThreads), 0, stream, a); };
+    const int64_t blocks = (int64_t)N * a.splits;
+    if (entropy) {
+        if (k) launch(token_logprobs_kernel<E, true, true>, blocks);
+        else launch(token_logprobs_kernel<E, true, false>, blocks);
+    } else {
+        if (k) launch(token_logprobs_kernel<E, false, true>, blocks);
+        else launch(token_logprobs_kernel<E, false, false>, blocks);
+    }
+    LLMQ_HIP_TRY(hipGetLastError());
+    if (a.splits > 1) {
+        launch(token_logprobs_join_kernel<E>, N);
+        LLMQ_HIP_TRY(hipGetLastError());
+    }
+    return LLMQ_OK;
+}
+
+template <typename E>
+static int token_logprobs_backward_any(E* dlogits, const float* dlogp, const float* dentropy, const E* logits, const int* targets,
+                                       const float* lse, const float* entropy, float* abs_max, int64_t N64, int V, int64_t P, hipStream_t stream) {
+    const char* what = "token_logprobs_backward";
+    LLMQ_REQUIRE(N64 >= 0 && N64 <= (1 << 24), "%s: 0 to 2^24 rows (got %lld)", what, (long long)N64);
+    LLMQ_REQUIRE(V >= 1 && V <= (1 << 28) && P >= V && P <= (1 << 28), "%s: vocabulary %d, row length %lld: 1 <= V <= P <= 2^28 is wanted", what, V, (long long)P);
+    LLMQ_REQUIRE(!dentropy || entropy || N64 == 0, "%s: dentropy needs the forward's entropy", what);
+    if (N64 > 0) {
+        LLMQ_REQUIRE(dlogits && dlogp && logits && targets && lse, "%s: null tensor pointer", what);
+        LLMQ_REQUIRE(aligned16(dlogits) && aligned16(logits), "%s: pointers must be 16-byte aligned", what);
+    }
+    if (abs_max) {
+        hipLaunchKernelGGL(reset_slot_kernel, dim3(1), dim3(1), 0, stream, reinterpret_cast<unsigned*>(abs_max));
+        LLMQ_HIP_TRY(hipGetLastError());
+    }
+    if (N64 == 0) return LLMQ_OK;
+    LogprobGradArgs a = {};
+    a.dlogits = dlogits, a.logits = logits, a.dlogp = dlogp, a.dentropy = dentropy, a.targets = targets, a.lse = lse, a.entropy = entropy;
+    a.abs_max = reinterpret_cast<unsigned*>(abs_max);
+    a.P = P, a.N = (int)N64, a.V = V;
+    const int64_t granules = P / Granule<E>::kN + 2;   // at most, wherever a row begins
+    a.chunks = (int)((granules + kLpThreads * kGradTurns - 1) / (kLpThreads * kGradTurns));
+    a.items = N64 * a.chunks;
+    const int64_t blocks = a.items < 8192 ? a.items : 8192;
+    auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kLpThreads), 0, stream, a); };
+    if (dentropy) {
+        if (abs_max) launch(token_logprobs_backward_kernel<E, true, true>);
+        else launch(token_logprobs_backward_kernel<E, true, false>);
+    } else {
+        if (abs_max) launch(token_logprobs_backward_kernel<E, false, true>);
+        else launch(token_logprobs_backward_kernel<E, false, false>);
+    }
+    LLMQ_HIP_TRY(hipGetLastError());
+    return LLMQ_OK;
+}
+
+}  // namespace llmq
+
+extern "C" int64_t llmq_token_logprobs_scratch_bytes(int64_t N, int V, int k) {
+    if (N <= 0 || N > (1 << 24) || V <= 0 || k < 0 || k > llmq::kTopMax) return 0;
+    return llmq::logprob_scratch((int)N, V, k);
+}
+extern "C" int llmq_token_logprobs_bf16(float* logp, float* entropy_or_null, float* lse, float* top_logp, int* top_ids, const uint16_t* logits,
+                                        const int* targets, void* scratch, size_t scratch_bytes, int64_t N, int V, int64_t P, int k, void* stream) {
+    return llmq::token_logprobs_any(logp, entropy_or_null, lse, top_logp, top_ids, logits, targets, scratch, scratch_bytes, N, V, P, k,
+                                    static_cast<hipStream_t>(stream));
+}
+extern "C" int llmq_token_logprobs_f32(float* logp, float* entropy_or_null, float* lse, float* top_logp, int* top_ids, const float* logits,
+                                       const int* targets, void* scratch, size_t scratch_bytes, int64_t N, int V, int64_t P, int k, void* stream) {
+    return llmq::token_logprobs_any(logp, entropy_or_null, lse, top_logp, top_ids, logits, targets, scratch, scratch_bytes, N, V, P, k,
+                                    static_cast<hipStream_t>(stream));
+}
+extern "C" int llmq_token_logprobs_backward_bf16(uint16_t* dlogits, const float* dlogp, const float* dentropy_or_null, const uint16_t* logits,
+                                                 const int* targets, const float* lse, const float* entropy_or_null, float* abs_max_or_null,
+                                                 int64_t N, int V, int64_t P, void* stream) {
+    return llmq::token_logprobs_backward_any(dlogits, dlogp, dentropy_or_null, logits, targets, lse, entropy_or_null, abs_max_or_null, N, V, P,
+                                             static_cast<hipStream_t>(stream));
+}
+extern "C" int llmq_token_logprobs_backward_f32(float* dlogits, const float* dlogp, const float* dentropy_or_null, const float* logits,
+                                                const int* targets, const float* lse, const float* entropy_or_null, float* abs_max_or_null,
+                                                int64_t N, int V, int64_t P, void* stream) {
+    return llmq::token_logprobs_backward_any(dlogits, dlogp, dentropy_or_null, logits, targets, lse, entropy_or_null, abs_max_or_null, N, V, P,
+                                             static_cast<hipStream_t>(stream));
+}

@@ -25,6 +25,9 @@ Names, argument order and in-place "out first" convention are the reference's:
     attention_forward(out, lse, qkv, abs_max, Nq, Nkv, first_key=None, softmax_scale=None, stream=0)
     attention_backward(dqkv, dout, out, lse, qkv, scratch, Nq, Nkv, first_key=None, softmax_scale=None, stream=0)
     get_attention_backward_scratch_size(B, T, Nq, Nkv, HD)
+    token_logprobs(logp, entropy, lse, top_logp, top_ids, logits, targets, scratch, vocab=None, stream=0)
+    token_logprobs_backward(dlogits, dlogp, dentropy, logits, targets, lse, entropy, abs_max, vocab=None, stream=0)
+    get_token_logprobs_scratch_size(N, V, k)
 `stream` is a raw hipStream_t handle (0 = torch's current stream).
 """
 import torch
@@ -466,3 +469,66 @@ def attention_backward(dqkv, dout, out, lse, qkv, scratch, Nq, Nkv, first_key=No
     with ctx:
         capi.check(capi.lib.llmq_attention_backward_bf16(d, g, o, l, x, f, s, scratch.numel() * scratch.element_size(), scale, B, T,
                                                          int(Nq), int(Nkv), HD, st))
+
+
+def _logprob_dims(logits, per_row, vocab):
+    """(rows, vocabulary, row length) of logits [..., P]; per_row: name -> tensor of one value a row (or None)."""
+    if logits.dim() < 2:
+        raise ValueError("logits must be [..., P]")
+    P = int(logits.shape[-1])
+    V = P if vocab is None else int(vocab)
+    if not 1 <= V <= P:
+        raise ValueError("vocab must lie between 1 and the row length %d (got %d)" % (P, V))
+    lead = tuple(logits.shape[:-1])
+    for name, t in per_row.items():
+        if t is not None and tuple(t.shape) != lead:
+            raise ValueError("%s must have one value for each row of logits" % name)
+    return logits.numel() // P, V, P
+
+
+def get_token_logprobs_scratch_size(N, V, k):
+    """Bytes of scratch token_logprobs needs for N rows of V logits and k alternatives (0: none, scratch may be None)."""
+    return int(capi.lib.llmq_token_logprobs_scratch_bytes(int(N), int(V), int(k)))
+
+
+def token_logprobs(logp, entropy, lse, top_logp, top_ids, logits, targets, scratch, vocab=None, stream=0):
+    """Log probabilities of the tokens `targets` (int32 [...]) under logits [..., P] (bf16 or fp32): logp, entropy (or None) and
+    lse [...] fp32, and the k most likely tokens of each row in falling order, top_logp [..., k] fp32 and top_ids [..., k] int32
+    (both None: not wanted; k <= 32; equal logits by token).  vocab: the columns that count (P unless given).  A target outside
+    [0, vocab) is ignored (logp 0).  scratch: device tensor of get_token_logprobs_scratch_size bytes, or None if that is 0."""
+    N, V, P = _logprob_dims(logits, {"logp": logp, "entropy": entropy, "lse": lse, "targets": targets}, vocab)
+    if (top_logp is None) != (top_ids is None):
+        raise ValueError("top_logp and top_ids go together")
+    k = 0
+    if top_ids is not None:
+        k = int(top_ids.shape[-1])
+        if top_ids.shape != top_logp.shape or tuple(top_ids.shape[:-1]) != tuple(logits.shape[:-1]):
+            raise ValueError("top_logp and top_ids must be [..., k]")
+    fn, dt = _producer_entry("token_logprobs", logits)
+    f32, i32 = (torch.float32,), (torch.int32,)
+    p = [_dev(logp, "logp", f32), _dev(entropy, "entropy", f32, optional=True), _dev(lse, "lse", f32),
+         _dev(top_logp, "top_logp", f32, optional=True), _dev(top_ids, "top_ids", i32, optional=True), _dev(logits, "logits", dt),
+         _dev(targets, "targets", i32), _dev(scratch, "scratch", optional=True)]
+    size = 0 if scratch is None else scratch.numel() * scratch.element_size()
+    ctx, st = _launch_context(stream, logits, logp, entropy, lse, top_logp, top_ids, targets, scratch)
+    with ctx:
+        capi.check(fn(*p, size, N, V, P, k, st))
+
+
+def token_logprobs_backward(dlogits, dlogp, dentropy, logits, targets, lse, entropy, abs_max, vocab=None, stream=0):
+    """dlogits (shape and type of logits; may be logits itself) from dlogp [...] and dentropy [...] (or None), with the forward's
+    lse and, for dentropy, entropy; abs_max (fp32 device scalar or None) receives max |dlogits|.  Columns from vocab on are
+    written as zeros."""
+    N, V, P = _logprob_dims(logits, {"dlogp": dlogp, "dentropy": dentropy, "targets": targets, "lse": lse, "entropy": entropy}, vocab)
+    if dlogits.shape != logits.shape:
+        raise ValueError("dlogits must have the shape of logits")
+    if dentropy is not None and entropy is None:
+        raise ValueError("dentropy needs the forward's entropy")
+    fn, dt = _producer_entry("token_logprobs_backward", logits)
+    f32 = (torch.float32,)
+    p = [_dev(dlogits, "dlogits", dt), _dev(dlogp, "dlogp", f32), _dev(dentropy, "dentropy", f32, optional=True),
+         _dev(logits, "logits", dt), _dev(targets, "targets", (torch.int32,)), _dev(lse, "lse", f32),
+         _dev(entropy, "entropy", f32, optional=True), _dev(abs_max, "abs_max", f32, optional=True)]
+    ctx, st = _launch_context(stream, logits, dlogits, dlogp, dentropy, targets, lse, entropy, abs_max)
+    with ctx:
+        capi.check(fn(*p, N, V, P, st))

@@ -25,6 +25,9 @@ order, defaults and mutation declarations on top of the gfx950 C ABI, so code wr
     attention_forward(out, lse, inp, absmax=None, Nq, Nkv, first_key=None, softmax_scale=0, stream=0)
     attention_backward(dinp, dout, out, lse, inp, scratch, Nq, Nkv, first_key=None, softmax_scale=0, stream=0)
     get_attention_backward_scratch_size(B, T, Nq, Nkv, HD)
+    token_logprobs(logp, entropy, lse, top_logp, top_ids, logits, targets, scratch, vocab=0, stream=0)
+    token_logprobs_backward(dlogits, dlogp, dentropy, logits, targets, lse, entropy, absmax=None, vocab=0, stream=0)
+    get_token_logprobs_scratch_size(N, V, k)
 
 matmul is in the torch sense (c = op(a) @ op(b), mode: TT=0, TN=1, NT=2, NN=3).  FP8 operands are served in
 mode NT (c[M,N] = a[M,K] @ b[N,K]^T, both K-contiguous: every shape with K % 16 == 0) and, for bf16 output on
@@ -162,6 +165,24 @@ def attention_backward(dinp: torch.Tensor, dout: torch.Tensor, out: torch.Tensor
 
 def get_attention_backward_scratch_size(B: int, T: int, Nq: int, Nkv: int, HD: int):
     return _k.get_attention_backward_scratch_size(B, T, Nq, Nkv, HD)
+
+
+@torch.library.custom_op("llmq::token_logprobs", mutates_args=("logp", "entropy", "lse", "top_logp", "top_ids", "scratch"))
+def token_logprobs(logp: torch.Tensor, entropy: torch.Tensor | None, lse: torch.Tensor, top_logp: torch.Tensor | None,
+                   top_ids: torch.Tensor | None, logits: torch.Tensor, targets: torch.Tensor, scratch: torch.Tensor | None,
+                   vocab: int = 0, stream: int = 0) -> None:
+    _k.token_logprobs(logp, entropy, lse, top_logp, top_ids, logits, targets, scratch, vocab or None, stream)
+
+
+@torch.library.custom_op("llmq::token_logprobs_backward", mutates_args=("dlogits", "absmax"))
+def token_logprobs_backward(dlogits: torch.Tensor, dlogp: torch.Tensor, dentropy: torch.Tensor | None, logits: torch.Tensor,
+                            targets: torch.Tensor, lse: torch.Tensor, entropy: torch.Tensor | None,
+                            absmax: torch.Tensor | None = None, vocab: int = 0, stream: int = 0) -> None:
+    _k.token_logprobs_backward(dlogits, dlogp, dentropy, logits, targets, lse, entropy, absmax, vocab or None, stream)
+
+
+def get_token_logprobs_scratch_size(N: int, V: int, k: int):
+    return _k.get_token_logprobs_scratch_size(N, V, k)
 
 
 def get_rmsnorm_backward_scratch_size(C: int):
