@@ -11,8 +11,8 @@
 // Forward: one pass with a running reference r and sums in base 2.  With d = (x - r) log2 e,
 //     s = sum 2^d,   w = sum d 2^d,   lse = r + log2(s) ln 2,   entropy = (log2 s - w / s) ln 2.
 // A lane's reference only follows a logit that has outgrown it by 11 (a factor of 6e4), so the sums are rarely rescaled; fp32
-// sums lose nothing by a common factor.  x - r is formed first: exact for neighbours, and no logit overflows, the type's lowest
-// value (a common mask) included.
+// sums lose nothing by a common factor.  d is one fused multiply-add, x log2 e - r log2 e; where r log2 e might overflow (a row of
+// the type's lowest value, a common mask) x - r is formed first.
 //
 // The k most likely tokens need no second pass over the row: each lane keeps the largest logit of its granules of 16 bytes and
 // the first granule that holds it.  The k-th best of the lanes' (value, granule) pairs bounds the k-th best logit from below, and
@@ -137,6 +137,18 @@ __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
 
 __device__ __forceinline__ float lse_of(const Sums& t) { return t.s == 0.f ? -__builtin_huge_valf() : t.r + __builtin_amdgcn_logf(t.s) * kLn2Lp; }
 
+// How many of n keys in LDS are larger than `key`.  n even, the list 16-byte aligned: two keys a read, eight reads in flight.
+__device__ __forceinline__ int count_larger(const uint64_t* keys, int n, uint64_t key) {
+    const ulonglong2* p = reinterpret_cast<const ulonglong2*>(keys);
+    int c = 0;
+#pragma unroll 8
+    for (int i = 0; i < n / 2; ++i) {
+        const ulonglong2 q = p[i];
+        c += (q.x > key) + (q.y > key);
+    }
+    return c;
+}
+
 // What one thread writes for a row.
 __device__ __forceinline__ float write_row(const LogprobArgs& a, int row, const Sums& t, float target, bool given) {
     const float lse = lse_of(t);
@@ -156,15 +168,18 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
     const Row<E> x(a.logits, row * a.P, a.V);
     const int g0 = (int)((int64_t)x.granules * split / a.splits), g1 = (int)((int64_t)x.granules * (split + 1) / a.splits);
 
+    // whole granules w0 .. w1 - 1, four loads in flight per lane; a lane walks its granules in rising order
+    const int w0 = g0 + (g0 < g1 && !x.whole(g0) ? 1 : 0), w1 = g1 - (w0 < g1 && !x.whole(g1 - 1) ? 1 : 0);
     Sums t = {-__builtin_huge_valf(), 0.f, 0.f};
-    float ref = 0.f, best = __builtin_nanf("");
-    int best_g = 0;
+    float ref = 0.f, ref2 = 0.f, best = -__builtin_huge_valf();
+    bool wide = false;   // a reference of the wave so large that its product with log2 e may overflow (masks of the lowest value)
+    int best_g = w0 > g0 && tid == 0 ? g0 : w0 + tid;
     auto take = [&](const float (&v)[kN], int g) {
         float top = v[0];
 #pragma unroll
         for (int j = 1; j < kN; ++j) top = __builtin_fmaxf(top, v[j]);
         if constexpr (TOP) {
-            if (top > best || best != best) best = top, best_g = g;   // NaN: nothing yet
+            if (top > best) best = top, best_g = g;
         }
         if (__any(top > t.r + 11.f)) {
             const float next = __builtin_fmaxf(t.r, top);
@@ -173,17 +188,25 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
                 t.w = (t.w + d * t.s) * f;
                 t.s *= f;
                 t.r = ref = next;
+                ref2 = ref * kLog2eLp;
+            }
+            wide = __any(!(__builtin_fabsf(ref) < 1e30f));
+        }
+        if (!wide) {
+#pragma unroll
+            for (int j = 0; j < kN; ++j) {
+                const float d = __builtin_fmaf(v[j], kLog2eLp, -ref2), e = __builtin_amdgcn_exp2f(d);
+                t.s += e;
+                if constexpr (ENTROPY) t.w = __builtin_fmaf(__builtin_fmaxf(d, -1e4f), e, t.w);   // 0 times -inf is nothing
+            }
+        } else {
+            for (int j = 0; j < kN; ++j) {
+                const float d = (v[j] - ref) * kLog2eLp, e = __builtin_amdgcn_exp2f(d);
+                t.s += e;
+                if constexpr (ENTROPY) t.w = __builtin_fmaf(__builtin_fmaxf(d, -1e4f), e, t.w);
             }
         }
-#pragma unroll
-        for (int j = 0; j < kN; ++j) {
-            const float d = (v[j] - ref) * kLog2eLp, e = __builtin_amdgcn_exp2f(d);
-            t.s += e;
-            if constexpr (ENTROPY) t.w = __builtin_fmaf(__builtin_fmaxf(d, -1e4f), e, t.w);   // 0 times -inf is nothing
-        }
     };
-    // whole granules w0 .. w1 - 1, four loads in flight per lane; a lane walks its granules in rising order
-    const int w0 = g0 + (g0 < g1 && !x.whole(g0) ? 1 : 0), w1 = g1 - (w0 < g1 && !x.whole(g1 - 1) ? 1 : 0);
     if (w0 > g0 && tid == 0) {
         float v[kN];
         x.values(g0, v);
@@ -234,17 +257,17 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
     }
 
     if constexpr (TOP) {
-        __shared__ uint64_t keys[kLpThreads];
-        __shared__ uint64_t list[kCandidates];
+        __shared__ __attribute__((aligned(16))) uint64_t keys[kLpThreads];
+        __shared__ __attribute__((aligned(16))) uint64_t list[kCandidates + 1];
         __shared__ int chosen[kTopMax];
         __shared__ int count, lanes;
         __shared__ uint64_t floor_key;
-        const uint64_t mine = key_of(order_of(best), (uint32_t)best_g);
+        const bool has = best_g < w1 || (w1 < g1 && (g1 - 1 - w0) % kLpThreads == tid);
+        const uint64_t mine = has ? key_of(order_of(best), (uint32_t)best_g) : 0;
         keys[tid] = mine;
         if (tid == 0) count = 0, lanes = 0, floor_key = 1;
         __syncthreads();
-        int rank = 0;
-        for (int i = 0; i < kLpThreads; ++i) rank += keys[i] > mine;
+        const int rank = count_larger(keys, kLpThreads, mine);
         if (mine && rank < a.k) {
             chosen[rank] = tid;
             atomicAdd(&lanes, 1);
@@ -292,10 +315,11 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
         };
         if (count <= kCandidates) {
             const int n = count;
+            if (tid == 0) list[n] = 0;   // a pad for the pairwise reads
+            __syncthreads();
             for (int i = tid; i < n; i += kLpThreads) {
                 const uint64_t key = list[i];
-                int at = 0;
-                for (int j = 0; j < n; ++j) at += list[j] > key;
+                const int at = count_larger(list, (n + 1) & ~1, key);
                 if (at < a.k) put(at, key);
             }
             for (int i = n + tid; i < a.k; i += kLpThreads) put(i, 0);
@@ -332,39 +356,61 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
     }
 }
 
-// Joins the shares of a row, in their order.
+// Joins the shares of a row, in their order.  Of the shares' keys only those count that reach a bound below the k-th best: the
+// k-th best of the shares' best, or the largest of the shares' k-th.
 template <typename E>
 __global__ __launch_bounds__(kLpThreads) void token_logprobs_join_kernel(LogprobArgs a) {
-    __shared__ uint64_t keys[kSplitMax * kTopMax];
+    __shared__ __attribute__((aligned(16))) uint64_t list[kSplitMax * kTopMax + 1];
+    __shared__ __attribute__((aligned(16))) uint64_t heads[kWave];
     __shared__ float shared_lse;
+    __shared__ int count;
+    __shared__ uint64_t floor_key;
     const int tid = threadIdx.x, row = blockIdx.x;
     const Sums* sums = static_cast<const Sums*>(a.scratch) + (int64_t)row * a.splits;
+    const int n = a.splits * a.k;
+    const uint64_t* partial = reinterpret_cast<const uint64_t*>(static_cast<const char*>(a.scratch) + ((int64_t)a.N * a.splits * sizeof(Sums) + 15) / 16 * 16) +
+                              (int64_t)row * n;
     if (tid < kWave) {
         Sums t = {-__builtin_huge_valf(), 0.f, 0.f};
         if (tid < a.splits) t = sums[tid];
+        const uint64_t best = a.k && tid < a.splits ? partial[tid * a.k] : 0;
+        uint64_t last = a.k && tid < a.splits ? partial[tid * a.k + a.k - 1] : 0;
 #pragma unroll
         for (int off = 1; off < kWave; off <<= 1) {
             const Sums o = {__shfl_xor(t.r, off, kWave), __shfl_xor(t.s, off, kWave), __shfl_xor(t.w, off, kWave)};
             t = (tid & off) ? join(o, t) : join(t, o);
+            const uint64_t other = __shfl_xor((unsigned long long)last, off, kWave);
+            last = other > last ? other : last;
         }
         if (tid == 0) {
             const int target = a.targets[row];
             const bool given = target >= 0 && target < a.V;
             const E* p = static_cast<const E*>(a.logits) + row * a.P;
             shared_lse = write_row(a, row, t, given ? Granule<E>::one(p[target]) : 0.f, given);
+            count = 0;
+            floor_key = last > 1 ? last : 1;
         }
+        heads[tid] = best;
     }
     if (a.k == 0) return;
-    const int n = a.splits * a.k;
-    const uint64_t* partial = reinterpret_cast<const uint64_t*>(static_cast<const char*>(a.scratch) + ((int64_t)a.N * a.splits * sizeof(Sums) + 15) / 16 * 16) +
-                              (int64_t)row * n;
-    for (int i = tid; i < n; i += kLpThreads) keys[i] = partial[i];
     __syncthreads();
+    if (tid < kWave && a.splits >= a.k) {
+        const uint64_t best = heads[tid];
+        if (best > floor_key && count_larger(heads, kWave, best) == a.k - 1) floor_key = best;
+    }
+    __syncthreads();
+    const uint64_t bound = floor_key;
     for (int i = tid; i < n; i += kLpThreads) {
-        const uint64_t key = keys[i];
-        // nothing: behind all keys, in the order of the places
-        int at = 0;
-        for (int j = 0; j < n && at < a.k; ++j) at += keys[j] > key || (keys[j] == key && j < i);
+        const uint64_t key = partial[i];
+        if (key >= bound) list[atomicAdd(&count, 1)] = key;
+    }
+    __syncthreads();
+    const int m = count;
+    if (tid == 0) list[m] = 0;
+    __syncthreads();
+    for (int i = tid; i < max(m, a.k); i += kLpThreads) {
+        const uint64_t key = i < m ? list[i] : 0;
+        const int at = i < m ? count_larger(list, (m + 1) & ~1, key) : i;
         if (at >= a.k) continue;
         a.top_ids[(int64_t)row * a.k + at] = key ? (int)~(uint32_t)key : -1;
         const float v = key ? value_of((uint32_t)(key >> 32)) : -__builtin_huge_valf();
@@ -460,7 +506,7 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_backward_kernel(Log
 // ---- host ------------------------------------------------------------------------------------------------------------------
 // Shares of a row: enough workgroups to fill the chip when there are few rows, each with at least 4096 logits.
 static int logprob_splits(int N, int V) {
-    int64_t s = (1024 + (int64_t)N - 1) / N;
+    int64_t s = (512 + (int64_t)N - 1) / N;
     const int64_t most = ((int64_t)V + 4095) / 4096;
     s = s < most ? s : most;
     return (int)(s < 1 ? 1 : s > kSplitMax ? kSplitMax : s);
