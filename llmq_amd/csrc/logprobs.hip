@@ -14,9 +14,15 @@
 // sums lose nothing by a common factor.  d is one fused multiply-add, x log2 e - r log2 e; where r log2 e might overflow (a row of
 // the type's lowest value, a common mask) x - r is formed first.
 //
-// The k most likely tokens need no second pass over the row: each lane keeps the largest logit of its granules of 16 bytes and
-// the first granule that holds it.  The k-th best of the lanes' (value, granule) pairs bounds the k-th best logit from below, and
-// only the k lanes that reach it can hold one of the k: their granules alone are read again, from the caches.
+// The k most likely tokens need no second pass over the row.  In the first turns (about the square root of all of a lane's
+// turns) each lane keeps the largest logit of its granules of 16 bytes and the first granule that holds it.  The k-th best of
+// the lanes' (value, granule) pairs bounds the k-th best logit from below, and of these turns only the k lanes that reach it can
+// hold one of the k.  From then on every granule with a logit above the bound is listed.  Those granules alone, of some hundreds
+// of turns a few hundred, are read again, from the caches; a full re-read of the k best lanes was 20 % of the time at k = 20.
+// Where the list overflows (logits that rise along the row) the lanes' best are taken over the whole row instead, and where that
+// finds too many, one pass per token.
+#include <type_traits>
+
 #include "common.hpp"
 #include "absmax_reduce.hpp"
 
@@ -46,8 +52,8 @@ struct LogprobGradArgs {
     const int* targets;
     const float *lse, *entropy;
     unsigned* abs_max;
-    int64_t P, items;
-    int N, V, chunks;
+    int64_t P;
+    int V, chunks;
 };
 
 // 16 bytes of logits as floats, and back.
@@ -158,29 +164,70 @@ __device__ __forceinline__ float write_row(const LogprobArgs& a, int row, const 
     return lse;
 }
 
+// The search for the k best of a workgroup's granules.
+struct TopSearch {
+    __attribute__((aligned(16))) uint64_t keys[kLpThreads];
+    __attribute__((aligned(16))) uint64_t list[kCandidates + 1];
+    int granules[kCandidates];
+    int chosen[kTopMax];
+    uint64_t floor_key;
+    int count, lanes, listed;
+};
+
+// The bound below the k-th best and the lanes that reach it, from each lane's best key (0: it has none).
+__device__ __forceinline__ uint64_t top_bound(TopSearch& t, uint64_t mine, int k) {
+    const int tid = threadIdx.x;
+    t.keys[tid] = mine;
+    if (tid == 0) t.count = 0, t.lanes = 0, t.listed = 0, t.floor_key = 1;
+    __syncthreads();
+    const int rank = count_larger(t.keys, kLpThreads, mine);
+    if (mine && rank < k) {
+        t.chosen[rank] = tid;
+        atomicAdd(&t.lanes, 1);
+        if (rank == k - 1) t.floor_key = mine;
+    }
+    __syncthreads();
+    return t.floor_key;
+}
+
+// Lists the logits of granule `at` that reach the bound.
+template <typename E>
+__device__ __forceinline__ void top_collect(TopSearch& t, const Row<E>& x, int at, uint64_t bound) {
+    float v[Granule<E>::kN];
+    x.values(at, v);
+#pragma unroll
+    for (int j = 0; j < Granule<E>::kN; ++j) {
+        const int e = x.first(at) + j;
+        const uint32_t o = order_of(v[j]);
+        if (e >= 0 && e < x.n && o && key_of(o, (uint32_t)at) >= bound) {
+            const int slot = atomicAdd(&t.count, 1);
+            if (slot < kCandidates) t.list[slot] = key_of(o, (uint32_t)e);
+        }
+    }
+}
+
 // One row (splits == 1) or one share of its granules per workgroup.
 template <typename E, bool ENTROPY, bool TOP>
 __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs a) {
-    constexpr int kN = Granule<E>::kN, kWaves = kLpThreads / kWave;
+    constexpr int kN = Granule<E>::kN, kWaves = kLpThreads / kWave, kInFlight = 4;
     __shared__ Sums wave_sums[kWaves];
     __shared__ float shared_lse;
     const int tid = threadIdx.x, row = blockIdx.x / a.splits, split = blockIdx.x % a.splits;
     const Row<E> x(a.logits, row * a.P, a.V);
+    // lane `tid` takes the granules g0 + tid + i * threads; the two that the row's ends may cut are in turn like the others
     const int g0 = (int)((int64_t)x.granules * split / a.splits), g1 = (int)((int64_t)x.granules * (split + 1) / a.splits);
 
-    // whole granules w0 .. w1 - 1, four loads in flight per lane; a lane walks its granules in rising order
-    const int w0 = g0 + (g0 < g1 && !x.whole(g0) ? 1 : 0), w1 = g1 - (w0 < g1 && !x.whole(g1 - 1) ? 1 : 0);
     Sums t = {-__builtin_huge_valf(), 0.f, 0.f};
     float ref = 0.f, ref2 = 0.f, best = -__builtin_huge_valf();
     bool wide = false;   // a reference of the wave so large that its product with log2 e may overflow (masks of the lowest value)
-    int best_g = w0 > g0 && tid == 0 ? g0 : w0 + tid;
-    auto take = [&](const float (&v)[kN], int g) {
+    int best_g = g0 + tid;
+    auto largest = [](const float (&v)[kN]) {
         float top = v[0];
 #pragma unroll
         for (int j = 1; j < kN; ++j) top = __builtin_fmaxf(top, v[j]);
-        if constexpr (TOP) {
-            if (top > best) best = top, best_g = g;
-        }
+        return top;
+    };
+    auto take = [&](const float (&v)[kN], float top) {
         if (__any(top > t.r + 11.f)) {
             const float next = __builtin_fmaxf(t.r, top);
             if (next > -__builtin_huge_valf()) {
@@ -207,32 +254,61 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
             }
         }
     };
-    if (w0 > g0 && tid == 0) {
-        float v[kN];
-        x.values(g0, v);
-        take(v, g0);
-    }
-    int g = w0 + tid;
-    for (; g + 3 * kLpThreads < w1; g += 4 * kLpThreads) {
-        uint4 q[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) q[u] = x.load(g + u * kLpThreads);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
+    // granules [from, to) of the workgroup, each lane's in rising order, `see`(largest logit, granule) before the sums
+    auto walk = [&](int from, int to, auto see) {
+        int g = from + tid;
+        const int inner = to - (to == g1 ? 1 : 0);   // the last granule of all may be cut
+        if (g < inner && !x.whole(g)) {              // and the first
             float v[kN];
-            Granule<E>::unpack(q[u], v);
-            take(v, g + u * kLpThreads);
+            x.values(g, v);
+            const float top = largest(v);
+            see(top, g);
+            take(v, top);
+            g += kLpThreads;
         }
-    }
-    for (; g < w1; g += kLpThreads) {
-        float v[kN];
-        Granule<E>::unpack(x.load(g), v);
-        take(v, g);
-    }
-    if (w1 < g1 && (g1 - 1 - w0) % kLpThreads == tid) {
-        float v[kN];
-        x.values(g1 - 1, v);
-        take(v, g1 - 1);
+        for (; g + (kInFlight - 1) * kLpThreads < inner; g += kInFlight * kLpThreads) {
+            uint4 q[kInFlight];
+#pragma unroll
+            for (int u = 0; u < kInFlight; ++u) q[u] = x.load(g + u * kLpThreads);
+#pragma unroll
+            for (int u = 0; u < kInFlight; ++u) {
+                float v[kN];
+                Granule<E>::unpack(q[u], v);
+                const float top = largest(v);
+                see(top, g + u * kLpThreads);
+                take(v, top);
+            }
+        }
+        for (; g < to; g += kLpThreads) {
+            float v[kN];
+            x.values(g, v);
+            const float top = largest(v);
+            see(top, g);
+            take(v, top);
+        }
+    };
+
+    __shared__ typename std::conditional<TOP, TopSearch, int>::type search;
+    int mid = g1;
+    uint64_t bound = 0;
+    if constexpr (TOP) {
+        const int turns = (g1 - g0 + kLpThreads - 1) / kLpThreads;
+        int first = kInFlight;
+        while (first * first < turns) first += kInFlight;
+        mid = min(g1, g0 + first * kLpThreads);
+        walk(g0, mid, [&](float top, int g) {
+            if (top > best) best = top, best_g = g;
+        });
+        bound = top_bound(search, g0 + tid < mid ? key_of(order_of(best), (uint32_t)best_g) : 0, a.k);
+        const float above = bound >> 32 ? value_of((uint32_t)(bound >> 32)) : -__builtin_huge_valf();
+        walk(mid, g1, [&](float top, int g) {
+            if (top > above) {
+                const int slot = atomicAdd(&search.listed, 1);
+                if (slot < kCandidates) search.granules[slot] = g;
+            }
+        });
+    } else {
+        walk(g0, g1, [](float, int) {});
     }
 
     Sums all = t;
@@ -257,48 +333,25 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
     }
 
     if constexpr (TOP) {
-        __shared__ __attribute__((aligned(16))) uint64_t keys[kLpThreads];
-        __shared__ __attribute__((aligned(16))) uint64_t list[kCandidates + 1];
-        __shared__ int chosen[kTopMax];
-        __shared__ int count, lanes;
-        __shared__ uint64_t floor_key;
-        const bool has = best_g < w1 || (w1 < g1 && (g1 - 1 - w0) % kLpThreads == tid);
-        const uint64_t mine = has ? key_of(order_of(best), (uint32_t)best_g) : 0;
-        keys[tid] = mine;
-        if (tid == 0) count = 0, lanes = 0, floor_key = 1;
-        __syncthreads();
-        const int rank = count_larger(keys, kLpThreads, mine);
-        if (mine && rank < a.k) {
-            chosen[rank] = tid;
-            atomicAdd(&lanes, 1);
-            if (rank == a.k - 1) floor_key = mine;
+        int end = mid;   // the chosen lanes' granules up to here are looked through
+        if (search.listed <= kCandidates) {
+            for (int i = tid; i < search.listed; i += kLpThreads) top_collect(search, x, search.granules[i], bound);
+        } else {
+            best = -__builtin_huge_valf(), best_g = g0 + tid;
+            for (int g = g0 + tid; g < g1; g += kLpThreads) {
+                float v[kN];
+                x.values(g, v);
+                const float top = largest(v);
+                if (top > best) best = top, best_g = g;
+            }
+            __syncthreads();
+            bound = top_bound(search, g0 + tid < g1 ? key_of(order_of(best), (uint32_t)best_g) : 0, a.k);
+            end = g1;
         }
-        __syncthreads();
-        const uint64_t bound = floor_key;
-        const int turns = (w1 - w0 + kLpThreads - 1) / kLpThreads + 2;   // and the two cut granules
-        for (int i = tid; i < lanes * turns; i += kLpThreads) {
-            const int lane = chosen[i / turns], turn = i % turns;
-            int at = w0 + lane + turn * kLpThreads;
-            if (turn == turns - 1) {
-                if (!(w1 < g1 && (g1 - 1 - w0) % kLpThreads == lane)) continue;
-                at = g1 - 1;
-            } else if (turn == turns - 2) {
-                if (!(w0 > g0 && lane == 0)) continue;
-                at = g0;
-            } else if (at >= w1) {
-                continue;
-            }
-            float v[kN];
-            x.values(at, v);
-#pragma unroll
-            for (int j = 0; j < kN; ++j) {
-                const int e = x.first(at) + j;
-                const uint32_t o = order_of(v[j]);
-                if (e >= 0 && e < x.n && o && key_of(o, (uint32_t)at) >= bound) {
-                    const int slot = atomicAdd(&count, 1);
-                    if (slot < kCandidates) list[slot] = key_of(o, (uint32_t)e);
-                }
-            }
+        const int turns = (end - g0 + kLpThreads - 1) / kLpThreads;
+        for (int i = tid; i < search.lanes * turns; i += kLpThreads) {
+            const int at = g0 + search.chosen[i / turns] + i % turns * kLpThreads;
+            if (at < end) top_collect(search, x, at, bound);
         }
         __syncthreads();
         uint64_t* partial = reinterpret_cast<uint64_t*>(static_cast<char*>(a.scratch) + ((int64_t)a.N * a.splits * sizeof(Sums) + 15) / 16 * 16) +
@@ -313,18 +366,17 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
                 a.top_logp[(int64_t)row * a.k + at] = v == -__builtin_huge_valf() && shared_lse == shared_lse ? v : v - shared_lse;
             }
         };
-        if (count <= kCandidates) {
-            const int n = count;
-            if (tid == 0) list[n] = 0;   // a pad for the pairwise reads
+        const int n = search.count;
+        if (n <= kCandidates) {
+            if (tid == 0) search.list[n] = 0;   // a pad for the pairwise reads
             __syncthreads();
             for (int i = tid; i < n; i += kLpThreads) {
-                const uint64_t key = list[i];
-                const int at = count_larger(list, (n + 1) & ~1, key);
+                const uint64_t key = search.list[i];
+                const int at = count_larger(search.list, (n + 1) & ~1, key);
                 if (at < a.k) put(at, key);
             }
             for (int i = n + tid; i < a.k; i += kLpThreads) put(i, 0);
         } else {
-            // Very many logits between the bound and the k-th best, all in the chosen lanes: one round over the share per token.
             uint64_t last = ~0ull;
             for (int round = 0; round < a.k; ++round) {
                 uint64_t top = 0;
@@ -339,13 +391,13 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
                     }
                 }
                 __syncthreads();
-                keys[tid] = top;
+                search.keys[tid] = top;
                 __syncthreads();
                 for (int half = kLpThreads / 2; half > 0; half >>= 1) {
-                    if (tid < half && keys[tid + half] > keys[tid]) keys[tid] = keys[tid + half];
+                    if (tid < half && search.keys[tid + half] > search.keys[tid]) search.keys[tid] = search.keys[tid + half];
                     __syncthreads();
                 }
-                last = keys[0];
+                last = search.keys[0];
                 if (tid == 0) put(round, last);
                 if (last == 0) {
                     for (int i = round + 1 + tid; i < a.k; i += kLpThreads) put(i, 0);
@@ -419,76 +471,75 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_join_kernel(Logprob
 }
 
 // ---- gradient --------------------------------------------------------------------------------------------------------------
-constexpr int kGradTurns = 4;   // granules of a lane per item
+constexpr int kGradTurns = 4;   // granules of a lane
 
 template <typename E, bool ENTROPY, bool ABSMAX>
 __global__ __launch_bounds__(kLpThreads) void token_logprobs_backward_kernel(LogprobGradArgs a) {
     constexpr int kN = Granule<E>::kN;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, row = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+    const Row<E> x(a.logits, row * a.P, (int)a.P);
+    E* out = static_cast<E*>(a.dlogits) + row * a.P;
+    const int at0 = chunk * (kLpThreads * kGradTurns) + tid;
+    // the logits are asked for before the row's scalars are waited for
+    uint4 q[kGradTurns];
+#pragma unroll
+    for (int u = 0; u < kGradTurns; ++u) {
+        const int at = at0 + u * kLpThreads;
+        if (at < x.granules && x.whole(at)) q[u] = load_nt(reinterpret_cast<const uint4*>(x.p + x.first(at)));
+    }
     uint32_t fold = sizeof(E) == 2 ? 0x7F807F80u : 0x7F800000u;
-    for (int64_t item = blockIdx.x; item < a.items; item += gridDim.x) {
-        const int row = (int)(item / a.chunks), chunk = (int)(item % a.chunks);
-        const Row<E> x(a.logits, row * a.P, (int)a.P);
-        E* out = static_cast<E*>(a.dlogits) + row * a.P;
-        const int target = a.targets[row];
-        const bool given = target >= 0 && target < a.V;
-        const float lse = a.lse[row], g = given ? a.dlogp[row] : 0.f;
-        float h = 0.f, shift = 0.f;
-        if constexpr (ENTROPY) h = a.dentropy[row], shift = a.entropy[row];
-        // no gradient enters, or the row has no probability: zeros, whatever the logits hold
-        const bool none = (g == 0.f && h == 0.f) || lse == -__builtin_huge_valf();
-        auto derive = [&](float v, int e) {
-            const float d = v - lse, p = __builtin_amdgcn_exp2f(d * kLog2eLp);
-            float c = -g;
-            if constexpr (ENTROPY) c -= h * (__builtin_fmaxf(d, -1e4f) + shift);
-            float r = p * c;
-            if (e == target) r += g;
-            return none || e >= a.V ? 0.f : r;
-        };
-        const int at0 = chunk * (kLpThreads * kGradTurns) + tid;
-        uint4 q[kGradTurns];
-        if (!none) {
+    const int target = a.targets[row];
+    const bool given = target >= 0 && target < a.V;
+    const float lse = a.lse[row], g = given ? a.dlogp[row] : 0.f;
+    float h = 0.f, shift = 0.f;
+    if constexpr (ENTROPY) h = a.dentropy[row], shift = a.entropy[row];
+    // no gradient enters, or the row has no probability: zeros, whatever the logits hold
+    const bool none = (g == 0.f && h == 0.f) || lse == -__builtin_huge_valf();
+    auto derive = [&](float v) {
+        const float d = v - lse, p = __builtin_amdgcn_exp2f(d * kLog2eLp);
+        float c = -g;
+        if constexpr (ENTROPY) c -= h * (__builtin_fmaxf(d, -1e4f) + shift);
+        return p * c;
+    };
 #pragma unroll
-            for (int u = 0; u < kGradTurns; ++u) {
-                const int at = at0 + u * kLpThreads;
-                if (at < x.granules && x.whole(at)) q[u] = x.load(at);
+    for (int u = 0; u < kGradTurns; ++u) {
+        const int at = at0 + u * kLpThreads;
+        if (at >= x.granules) continue;
+        const int e0 = x.first(at);
+        if (x.whole(at)) {
+            float v[kN];
+            Granule<E>::unpack(q[u], v);
+#pragma unroll
+            for (int j = 0; j < kN; ++j) v[j] = derive(v[j]);
+            if (given && (unsigned)(target - e0) < (unsigned)kN) {
+#pragma unroll
+                for (int j = 0; j < kN; ++j) v[j] += e0 + j == target ? g : 0.f;
             }
-        }
+            if (none || e0 + kN > a.V) {
 #pragma unroll
-        for (int u = 0; u < kGradTurns; ++u) {
-            const int at = at0 + u * kLpThreads;
-            if (at >= x.granules) continue;
-            const int e0 = x.first(at);
-            if (x.whole(at)) {
-                float v[kN];
-                if (none) {
-#pragma unroll
-                    for (int j = 0; j < kN; ++j) v[j] = 0.f;
+                for (int j = 0; j < kN; ++j) v[j] = none || e0 + j >= a.V ? 0.f : v[j];
+            }
+            const uint4 w = Granule<E>::pack(v);
+            store_nt(reinterpret_cast<uint4*>(out + e0), w);
+            if constexpr (ABSMAX) {
+                if constexpr (sizeof(E) == 2) {
+                    fold = fold_vec(fold, w);
                 } else {
-                    Granule<E>::unpack(q[u], v);
+                    const uint32_t b[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                    for (int j = 0; j < kN; ++j) v[j] = derive(v[j], e0 + j);
+                    for (int j = 0; j < 4; ++j) fold = min(fold, 0x7F800000u - (b[j] & 0x7FFFFFFFu));
                 }
-                const uint4 w = Granule<E>::pack(v);
-                *reinterpret_cast<uint4*>(out + e0) = w;
+            }
+        } else {
+            for (int j = 0; j < kN; ++j) {
+                const int e = e0 + j;
+                if (e < 0 || e >= x.n) continue;
+                const float v = none || e >= a.V ? 0.f : derive(Granule<E>::one(x.p[e])) + (e == target ? g : 0.f);
+                const E r = Granule<E>::round(v);
+                out[e] = r;
                 if constexpr (ABSMAX) {
-                    if constexpr (sizeof(E) == 2) fold = fold_vec(fold, w);
-                    else {
-                        const uint32_t b[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) fold = min(fold, 0x7F800000u - (b[j] & 0x7FFFFFFFu));
-                    }
-                }
-            } else {
-                for (int j = 0; j < kN; ++j) {
-                    const int e = e0 + j;
-                    if (e < 0 || e >= x.n) continue;
-                    const E r = Granule<E>::round(none ? 0.f : derive(Granule<E>::one(x.p[e]), e));
-                    out[e] = r;
-                    if constexpr (ABSMAX) {
-                        if constexpr (sizeof(E) == 2) fold = fold_bf16x2(fold, (uint32_t)__builtin_bit_cast(uint16_t, r));
-                        else fold = min(fold, 0x7F800000u - (__builtin_bit_cast(uint32_t, r) & 0x7FFFFFFFu));
-                    }
+                    if constexpr (sizeof(E) == 2) fold = fold_bf16x2(fold, (uint32_t)__builtin_bit_cast(uint16_t, r));
+                    else fold = min(fold, 0x7F800000u - (__builtin_bit_cast(uint32_t, r) & 0x7FFFFFFFu));
                 }
             }
         }
@@ -570,11 +621,11 @@ static int token_logprobs_backward_any(E* dlogits, const float* dlogp, const flo
     LogprobGradArgs a = {};
     a.dlogits = dlogits, a.logits = logits, a.dlogp = dlogp, a.dentropy = dentropy, a.targets = targets, a.lse = lse, a.entropy = entropy;
     a.abs_max = reinterpret_cast<unsigned*>(abs_max);
-    a.P = P, a.N = (int)N64, a.V = V;
+    a.P = P, a.V = V;
     const int64_t granules = P / Granule<E>::kN + 2;   // at most, wherever a row begins
     a.chunks = (int)((granules + kLpThreads * kGradTurns - 1) / (kLpThreads * kGradTurns));
-    a.items = N64 * a.chunks;
-    const int64_t blocks = a.items < 8192 ? a.items : 8192;
+    const int64_t blocks = N64 * a.chunks;
+    LLMQ_REQUIRE(blocks <= 0x7FFFFFFF, "%s: tensor too large", what);
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kLpThreads), 0, stream, a); };
     if (dentropy) {
         if (abs_max) launch(token_logprobs_backward_kernel<E, true, true>);

@@ -117,6 +117,16 @@ def test_top_tokens_of_rows_with_ties_and_orders(K, dtype):
                 assert torch.equal(top, torch.where(val == -math.inf, val, val - lse[:, None]))
 
 
+def test_top_tokens_of_rising_logits(K):
+    """Logits that rise along the row: every later granule lies above any earlier bound."""
+    V = 500009
+    x = torch.arange(V, device="cuda").float()[None] / 1024
+    for n in (1, 600):
+        _, _, lse, top, ids = forward(K, x.repeat(n, 1), torch.full((n,), 3, dtype=torch.int32, device="cuda"), V, 32)
+        assert torch.equal(ids, (V - 1 - torch.arange(32, device="cuda", dtype=torch.int32)).expand(n, 32))
+        assert torch.equal(top, x[:, -32:].flip(1) - lse[:, None])
+
+
 def test_top_tokens_when_the_chosen_lanes_hold_too_many(K):
     """More logits between the bound and the k-th best than the list holds: one lane's granules large in every turn."""
     V = 8 * 256 * 200
