@@ -9,6 +9,7 @@
 // token), a sliding window (t - w + 1) and padding (any value above t: the row is empty, out 0, lse -inf, no gradient).
 // (The reference's own kernels: src/kernels/attention.cu:20,152; its call sites src/models/llama_model.cpp:196-202.)
 #include <climits>
+#include <type_traits>
 
 #include "common.hpp"
 #include "absmax_reduce.hpp"
@@ -26,6 +27,7 @@ struct AttentionArgs {
     uint16_t* dqkv;
     float* lse2;             // backward scratch: lse in base 2, [B, Nq, T]
     float* delta;            // D, [B, Nq, T]
+    int* flags;              // per workgroup of the keys' kernel: whether a value was not finite
     int2* groups;            // with first_key: per 32 queries the smallest first key of a row that has any, the largest of all
     float* partial;          // dk, dv of each split: [splits][B, T, Nkv][2][head_dim], or NULL (one split, written to dqkv)
     int B, T, Nq, Nkv, head_dim, G;
@@ -38,7 +40,7 @@ constexpr int kKeys = 64;    // rows of a staged tile
 __device__ __forceinline__ int wave_min(int x) {
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) x = min(x, __shfl_xor(x, off, kWave));
-    return x;
+    return __builtin_amdgcn_readfirstlane(x);
 }
 __device__ __forceinline__ int wave_max(int x) { return ~wave_min(~x); }
 
@@ -60,38 +62,33 @@ __device__ __forceinline__ void load_columns(bf16x8 (&f)[HDP / 16], const uint16
     }
 }
 
-// Stores a transposed result (dimensions by positions) times `factor` as bf16 to `row`, this lane's position: the two lanes
-// of a position swap groups of four dimensions, so that each writes 16 bytes.  Returns the abs-max fold.
-template <int HDP>
-__device__ __forceinline__ uint32_t store_columns(uint16_t* row, const f32x16 (&acc)[HDP / 32], float factor, int lane, int head_dim,
-                                                  bool valid, uint32_t fold) {
-    const int h = lane >> 5;
+// Stores dimensions 32 db .. of a transposed result (dimensions by positions) times `factor` as bf16 to `row`, this lane's
+// position: the two lanes of a position swap groups of four dimensions, so that each writes 16 bytes.  Returns the abs-max fold.
+__device__ __forceinline__ uint32_t store_columns(uint16_t* row, const f32x16& acc, int db, float factor, int lane, int head_dim, bool valid,
+                                                  uint32_t fold) {
 #pragma unroll
-    for (int db = 0; db < HDP / 32; ++db) {
+    for (int g = 0; g < 2; ++g) {
+        uint32_t w[2][2];
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            uint32_t w[2][2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int i = 8 * g + 4 * e;
-                w[e][0] = pack_bf16(acc[db][i] * factor, acc[db][i + 1] * factor);
-                w[e][1] = pack_bf16(acc[db][i + 2] * factor, acc[db][i + 3] * factor);
-            }
-            const auto x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
-            const auto y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
-            const int d = db * 32 + 16 * g + 8 * h;
-            if (valid && d < head_dim) {
-                const uint4 v = make_uint4(x[0], y[0], x[1], y[1]);
-                *reinterpret_cast<uint4*>(row + d) = v;
-                fold = fold_vec(fold, v);
-            }
+        for (int e = 0; e < 2; ++e) {
+            const int i = 8 * g + 4 * e;
+            w[e][0] = pack_bf16(acc[i] * factor, acc[i + 1] * factor);
+            w[e][1] = pack_bf16(acc[i + 2] * factor, acc[i + 3] * factor);
+        }
+        const auto x = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+        const auto y = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+        const int d = db * 32 + 16 * g + 8 * (lane >> 5);
+        if (valid && d < head_dim) {
+            const uint4 v = make_uint4(x[0], y[0], x[1], y[1]);
+            *reinterpret_cast<uint4*>(row + d) = v;
+            fold = fold_vec(fold, v);
         }
     }
     return fold;
 }
 
-__device__ __forceinline__ bool all_finite(const f32x16& x, float carry = 0.f) {
-    float t = carry;
+__device__ __forceinline__ bool all_finite(const f32x16& x) {
+    float t = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) t = __builtin_fmaf(x[i], 0.f, t);
     return t == 0.f;
@@ -155,176 +152,318 @@ __device__ __forceinline__ void block_range(int& lo, int& hi, int wave_lo, int w
         lo = min(lo, ends[0][w]);
         hi = max(hi, ends[1][w]);
     }
+    lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
 }
 
-__device__ __forceinline__ void copies_landed() {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
+// Keeps what is derived from a lane's value out of registers that live across a loop or the loop's whole kernel: it is derived
+// again where it is used.
+__device__ __forceinline__ int here(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// ---- forward and the backward's queries: a workgroup's geometry ---------------------------------------------------------
+// A wave owns 32 queries (columns) and walks the keys (rows) in tiles of 64 that the workgroup's waves share in LDS.  What the
+// kernels and their careful forms have in common; `lds` holds two buffers of a key tile and a value tile.
+template <int HDP, int WAVES>
+struct QueryBlock {
+    typedef Tile<HDP, kKeys> T;
+    static constexpr int kThreads = WAVES * kWave, kSteps = HDP / 16, kDims = HDP / 32, kBlock = 32 * WAVES;
+    static constexpr int kLdsBytes = 4 * T::kBytes;
+
+    const AttentionArgs& a;
+    char* lds;
+    int tid, lane, b, kvh, head;
+    int64_t token, stride;      // elements of a token, bytes
+    const uint16_t *base, *kbase, *vbase;
+    QueryMask<1> mask;
+    int t_lo, t_hi;             // tiles of the workgroup (t_lo > t_hi: none)
+    int w_lo, w_hi;             // and of the wave
+
+    __device__ __forceinline__ QueryBlock(const AttentionArgs& args, char* lds_) : a(args), lds(lds_) {
+        tid = threadIdx.x, lane = tid % kWave;
+        const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+        // Workgroups go to the dies round-robin: the groups of heads that share keys are the fastest index, so that a group
+        // stays on one die's L2 where their number allows; the last queries, which have the most keys, come first.
+        const int ngroups = a.B * a.Nkv, nq = (a.T + kBlock - 1) / kBlock;
+        const int grp = blockIdx.x % ngroups, rest = blockIdx.x / ngroups;
+        b = grp / a.Nkv, kvh = grp % a.Nkv, head = kvh * a.G + rest % a.G;
+        const int q0 = (nq - 1 - rest / a.G) * kBlock + wave * 32;
+        token = (int64_t)(a.Nq + 2 * a.Nkv) * a.head_dim, stride = token * 2;
+        base = a.qkv + b * a.T * token;
+        kbase = base + (int64_t)(a.Nq + kvh) * a.head_dim;
+        vbase = kbase + (int64_t)a.Nkv * a.head_dim;
+        if (a.head_dim < HDP) {   // block_range ends with a barrier
+#pragma unroll
+            for (int i = 0; i < 4; ++i) T::template clear<kThreads>(lds + i * T::kBytes, tid);
+        }
+        mask.load(a, b, q0, lane);
+        int lo, hi;
+        block_range<WAVES>(lo, hi, mask.lo, mask.hi);
+        t_lo = lo <= hi ? lo / kKeys : 1, t_hi = lo <= hi ? hi / kKeys : 0;
+        w_lo = mask.lo <= mask.hi ? mask.lo / kKeys : INT_MAX, w_hi = mask.lo <= mask.hi ? mask.hi / kKeys : -1;
+    }
+    __device__ __forceinline__ char* keys(int buf) const { return lds + buf * T::kBytes; }
+    __device__ __forceinline__ char* values(int buf) const { return lds + (2 + buf) * T::kBytes; }
+    __device__ __forceinline__ void fetch(char* to, const uint16_t* from, int t) const {
+        const int id = here(tid);
+        T::template stage<kThreads>(to, from, T::template source<kThreads>(id, stride, a.head_dim), id, stride, t * kKeys, a.T);
+    }
+    __device__ __forceinline__ void load_rows(bf16x8 (&f)[kSteps], const uint16_t* tensor, int64_t row_elements) const {
+        load_columns<HDP>(f, tensor + min(mask.q[0], a.T - 1) * row_elements + (int64_t)head * a.head_dim, lane, a.head_dim);
+    }
+    __device__ __forceinline__ bool whole(int t) const { return mask.whole(t * kKeys, t * kKeys + kKeys - 1); }
+    __device__ __forceinline__ bool allowed(int t, int rb, int i) const { return mask.allowed(0, t * kKeys + tile_row(rb, i, lane)); }
+    // ones in the places that count, as an operand
+    __device__ __forceinline__ bf16x8 counted(int t, int rb, int u) const {
+        f32x16 in;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) in[i] = allowed(t, rb, i) ? 1.f : 0.f;
+        return operand(in, u);
+    }
+    __device__ __forceinline__ bool valid() const { return mask.q[0] < a.T; }
+    __device__ __forceinline__ int64_t statistic() const { return ((int64_t)b * a.Nq + head) * a.T + mask.q[0]; }
+    __device__ __forceinline__ uint16_t* out_row() const { return a.out + (((int64_t)b * a.T + mask.q[0]) * a.Nq + head) * a.head_dim; }
+    __device__ __forceinline__ uint16_t* dq_row() const { return a.dqkv + ((int64_t)b * a.T + mask.q[0]) * token + (int64_t)head * a.head_dim; }
+};
+
+// s = K q of a key tile
+template <int HDP>
+__device__ __forceinline__ void tile_scores(f32x16 (&s)[2], const char* keys, int row_lane, const bf16x8 (&qf)[HDP / 16]) {
+    typedef Tile<HDP, kKeys> T;
+    s[0] = zero16(), s[1] = zero16();
+#pragma unroll
+    for (int st = 0; st < HDP / 16; ++st)
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) s[rb] = mfma(T::rows(keys, row_lane, rb, st), qf[st], s[rb]);
+}
+template <typename Block>
+__device__ __forceinline__ void mask_scores(f32x16 (&s)[2], const Block& w, int t) {
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (!w.allowed(t, rb, i)) s[rb][i] = -__builtin_huge_valf();
 }
 
 // ---- forward ------------------------------------------------------------------------------------------------------------
-// A wave owns 32 NB queries (columns) and walks the keys (rows) in tiles of 64 that the workgroup's waves share in LDS, the next
-// tile copied while one is computed.
-template <int HDP, int NB, int WAVES>
-__global__ __launch_bounds__(WAVES * kWave, NB == 2 && HDP == 128 ? 1 : 2) void attention_forward_kernel(AttentionArgs a) {
-    typedef Tile<HDP, kKeys> T;
-    constexpr int kThreads = WAVES * kWave, kSteps = HDP / 16, kDims = HDP / 32;
-    __shared__ __attribute__((aligned(16))) char lds[2][2][T::kBytes];   // [buffer][key, value]
-    const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-
-    // Workgroups go to the dies round-robin: the groups of heads that share keys are the fastest index, so that a group
-    // stays on one die's L2 where their number allows; the last queries, which have the most keys, come first.
-    const int ngroups = a.B * a.Nkv, nq = (a.T + 32 * NB * WAVES - 1) / (32 * NB * WAVES);
-    const int grp = blockIdx.x % ngroups, rest = blockIdx.x / ngroups;
-    const int b = grp / a.Nkv, kvh = grp % a.Nkv, head = kvh * a.G + rest % a.G;
-    const int q0 = (nq - 1 - rest / a.G) * (32 * NB * WAVES) + wave * (32 * NB);
-
-    const int64_t token = (int64_t)(a.Nq + 2 * a.Nkv) * a.head_dim, stride = token * 2;
-    const uint16_t* base = a.qkv + b * a.T * token;
-    const uint16_t* kbase = base + (int64_t)(a.Nq + kvh) * a.head_dim;
-    const auto ksrc = T::template source<kThreads>(kbase, tid, stride, a.head_dim);
-    auto vsrc = ksrc;
-    vsrc.p += (int64_t)a.Nkv * a.head_dim * 2;
-
-    QueryMask<NB> mask;
-    mask.load(a, b, q0, lane);
-    int lo, hi;
-    block_range<WAVES>(lo, hi, mask.lo, mask.hi);
-    const int t_lo = lo / kKeys, t_hi = hi / kKeys;   // lo > hi where no row has a key
-
-    bf16x8 qf[NB][kSteps];
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-        load_columns<HDP>(qf[n], base + min(mask.q[n], a.T - 1) * token + (int64_t)head * a.head_dim, lane, a.head_dim);
-    const int row_lane = T::row_lane(lane), cols_lane = T::cols_lane(lane);
-
-    f32x16 o[NB][kDims];
-    float m[NB], sum[NB];
-    // A second, careful walk only where the first one ended in a value that is not finite.
+// The careful form of a workgroup in which a value was not finite: 32 dimensions at a time, with the product that keeps masked
+// places out.  The statistics stand: the scores see no values.  (As a function of its own it cost 20 us a launch: a kernel that
+// calls one reserves scratch memory.)
+template <int HDP, typename W>
+__device__ __forceinline__ uint32_t attention_forward_careful(const W& w, const bf16x8 (&qf)[W::kSteps], float ref, float inv) {
+    typedef typename W::T T;
+    uint32_t fold = 0x7F807F80u;
 #pragma nounroll
-    for (int careful = 0;; ++careful) {
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            m[n] = -__builtin_huge_valf();
-            sum[n] = 0.f;
-#pragma unroll
-            for (int db = 0; db < kDims; ++db) o[n][db] = zero16();
-        }
-        if (lo <= hi) {
-            T::template stage<kThreads>(lds[0][0], ksrc, tid, stride, t_lo * kKeys, a.T);
-            T::template stage<kThreads>(lds[0][1], vsrc, tid, stride, t_lo * kKeys, a.T);
+    for (int db = 0; db < W::kDims; ++db) {
+        f32x16 one = zero16();
+#pragma nounroll
+        for (int t = w.t_lo; t <= w.t_hi; ++t) {
+            w.fetch(w.keys(0), w.kbase, t);
+            w.fetch(w.values(0), w.vbase, t);
             copies_landed();
-        }
-#pragma nounroll
-        for (int t = t_lo; lo <= hi && t <= t_hi; ++t) {
-            const int buf = (t - t_lo) & 1, k0 = t * kKeys;
-            if (t < t_hi) {
-                T::template stage<kThreads>(lds[buf ^ 1][0], ksrc, tid, stride, k0 + kKeys, a.T);
-                T::template stage<kThreads>(lds[buf ^ 1][1], vsrc, tid, stride, k0 + kKeys, a.T);
-            }
-            if (mask.touches(k0, k0 + kKeys - 1)) {
-                const bool whole = mask.whole(k0, k0 + kKeys - 1);
-                f32x16 s[NB][2];
+            if (t >= w.w_lo && t <= w.w_hi) {
+                f32x16 s[2];
+                tile_scores<HDP>(s, w.keys(0), T::row_lane(here(w.lane)), qf);
+                mask_scores(s, w, t);
 #pragma unroll
                 for (int rb = 0; rb < 2; ++rb) {
 #pragma unroll
-                    for (int n = 0; n < NB; ++n) s[n][rb] = zero16();
+                    for (int i = 0; i < 16; ++i) s[rb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][i], w.a.scale2, -ref));
 #pragma unroll
-                    for (int st = 0; st < kSteps; ++st) {
-                        const bf16x8 kf = T::rows(lds[buf][0], row_lane, rb, st);
-#pragma unroll
-                        for (int n = 0; n < NB; ++n) s[n][rb] = mfma(kf, qf[n][st], s[n][rb]);
-                    }
-                }
-                if (!whole) {
-#pragma unroll
-                    for (int n = 0; n < NB; ++n)
-#pragma unroll
-                        for (int rb = 0; rb < 2; ++rb)
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                if (!mask.allowed(n, k0 + tile_row(rb, i, lane))) s[n][rb][i] = -__builtin_huge_valf();
-                }
-                bf16x8 pf[NB][4];
-#pragma unroll
-                for (int n = 0; n < NB; ++n) {
-                    float top = -__builtin_huge_valf();
-#pragma unroll
-                    for (int rb = 0; rb < 2; ++rb)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, s[n][rb][i]);
-                    top = halves_max(top);
-                    // The maximum that the exponentials are taken against follows only when one has outgrown it by 2^8: the
-                    // sums and the 16-bit probabilities lose nothing by a common factor of that size, and the accumulators
-                    // are rarely rescaled.
-                    if (__any((top - m[n]) * a.scale2 > 8.f)) {
-                        const float next = __builtin_fmaxf(m[n], top);
-                        const float factor = next == -__builtin_huge_valf() ? 1.f : __builtin_amdgcn_exp2f((m[n] - next) * a.scale2);
-                        m[n] = next;
-                        sum[n] *= factor;
-#pragma unroll
-                        for (int db = 0; db < kDims; ++db)
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) o[n][db][i] *= factor;
-                    }
-                    const float ref = m[n] == -__builtin_huge_valf() ? 0.f : m[n] * a.scale2;
-#pragma unroll
-                    for (int rb = 0; rb < 2; ++rb) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            s[n][rb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][rb][i], a.scale2, -ref));
-                            sum[n] += s[n][rb][i];
-                        }
-                        pf[n][2 * rb] = operand(s[n][rb], 0);
-                        pf[n][2 * rb + 1] = operand(s[n][rb], 1);
-                    }
-                }
-                if (careful == 0 || whole) {
-#pragma unroll
-                    for (int db = 0; db < kDims; ++db)
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            const bf16x8 vf = T::cols(lds[buf][1], cols_lane, db, u);
-#pragma unroll
-                            for (int n = 0; n < NB; ++n) o[n][db] = mfma(vf, pf[n][u], o[n][db]);
-                        }
-                } else {
-#pragma unroll
-                    for (int n = 0; n < NB; ++n)
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            f32x16 one;
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) one[i] = mask.allowed(n, k0 + tile_row(u / 2, i, lane)) ? 1.f : 0.f;
-                            const bf16x8 counts = operand(one, u & 1);
-#pragma unroll
-                            for (int db = 0; db < kDims; ++db)
-                                o[n][db] = careful_product(T::cols(lds[buf][1], cols_lane, db, u), pf[n][u], counts, o[n][db]);
-                        }
+                    for (int u = 0; u < 2; ++u)
+                        one = careful_product(T::cols(w.values(0), T::cols_lane(here(w.lane)), db, 2 * rb + u), operand(s[rb], u), w.counted(t, rb, u), one);
                 }
             }
-            copies_landed();
+            __syncthreads();
         }
-        if (careful) break;
-        bool fine = true;
+        fold = store_columns(w.out_row(), one, db, inv, w.lane, w.a.head_dim, w.valid(), fold);
+    }
+    return fold;
+}
+
+// Two waves per SIMD, and within a wave two tiles in flight: the exponentials of tile t are computed between the matrix
+// instructions of the scores of tile t + 1, so that neither unit waits for the other's latency.  Keys are copied two tiles
+// ahead and values one; one barrier a tile.
+template <int HDP, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, 2) void attention_forward_kernel(AttentionArgs a) {
+    typedef QueryBlock<HDP, WAVES> W;
+    typedef typename W::T T;
+    __shared__ __attribute__((aligned(16))) char lds[W::kLdsBytes];
+    const W w(a, lds);
+    bf16x8 qf[W::kSteps];
+    w.load_rows(qf, w.base, w.token);
+
+    f32x16 o[W::kDims], s[2];
+    float m = -__builtin_huge_valf(), sum[2] = {0.f, 0.f}, top = 0.f;
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+    for (int db = 0; db < W::kDims; ++db) o[db] = zero16();
+    const int row_lane_ = T::row_lane(w.lane), cols_lane_ = T::cols_lane(w.lane);
+
+#ifdef PIPE
+    if (w.t_lo <= w.t_hi) w.fetch(w.keys(w.t_lo & 1), w.kbase, w.t_lo);
+#pragma nounroll
+    for (int t = w.t_lo - 1; t <= w.t_hi; ++t) {   // first turn: the scores of the first tile only
+        copies_landed();
+        const char* next_keys = w.keys((t + 1) & 1);
+        char* values = w.values(t & 1);
+        if (t + 2 <= w.t_hi) w.fetch(w.keys(t & 1), w.kbase, t + 2);
+        if (t + 1 <= w.t_hi) w.fetch(w.values((t + 1) & 1), w.vbase, t + 1);
+        const bool now = t >= w.w_lo && t <= w.w_hi, next = t + 1 >= w.w_lo && t + 1 <= w.w_hi;
+        float ref = 0.f;
+        if (now) {
+            // The maximum that the exponentials are taken against follows only when one has outgrown it by 2^8: the sums and
+            // the 16-bit probabilities lose nothing by a common factor of that size, and the accumulators are rarely rescaled.
+            if (__any((top - m) * a.scale2 > 8.f)) {
+                const float to = __builtin_fmaxf(m, top);
+                const float factor = to == -__builtin_huge_valf() ? 1.f : __builtin_amdgcn_exp2f((m - to) * a.scale2);
+                m = to;
+                sum[0] *= factor, sum[1] *= factor;
 #pragma unroll
-            for (int db = 0; db < kDims; ++db) fine &= all_finite(o[n][db]);
-        if (!__syncthreads_or(!fine)) break;
+                for (int db = 0; db < W::kDims; ++db)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[db][i] *= factor;
+            }
+            ref = m == -__builtin_huge_valf() ? 0.f : m * a.scale2;
+        }
+        auto probabilities = [&](bf16x8 (&pf)[4]) {
+#pragma unroll
+            for (int rb = 0; rb < 2; ++rb) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[rb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][i], a.scale2, -ref));
+                    sum[i & 1] += s[rb][i];
+                }
+                pf[2 * rb] = operand(s[rb], 0);
+                pf[2 * rb + 1] = operand(s[rb], 1);
+            }
+        };
+        auto accumulate = [&](const bf16x8 (&pf)[4]) {
+            const int cols_lane = here(cols_lane_);
+#pragma unroll
+            for (int db = 0; db < W::kDims; ++db)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) o[db] = mfma(T::cols(values, cols_lane, db, u), pf[u], o[db]);
+        };
+        if (now && next) {
+            bf16x8 pf[4];
+            f32x16 ahead[2];
+            tile_scores<HDP>(ahead, next_keys, here(row_lane_), qf);
+            probabilities(pf);
+#ifdef SCHED
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+            for (int i = 0; i < 2 * W::kSteps; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, 5 * 128 / HDP, 0);
+                __builtin_amdgcn_sched_group_barrier(0x400, 2 * 128 / HDP, 0);
+            }
+#endif
+            accumulate(pf);
+#ifdef SCHED
+            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+            for (int i = 0; i < 4 * W::kDims; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            }
+#endif
+            s[0] = ahead[0], s[1] = ahead[1];
+        } else if (now) {
+            bf16x8 pf[4];
+            probabilities(pf);
+            accumulate(pf);
+        } else if (next) {
+            tile_scores<HDP>(s, next_keys, here(row_lane_), qf);
+        }
+        if (next) {
+            if (!w.whole(t + 1)) mask_scores(s, w, t + 1);
+            top = -__builtin_huge_valf();
+#pragma unroll
+            for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, s[rb][i]);
+            top = halves_max(top);
+        }
     }
 
-    uint32_t fold = 0x7F807F80u;
+#else
+    if (w.t_lo <= w.t_hi) {
+        w.fetch(w.keys(w.t_lo & 1), w.kbase, w.t_lo);
+        w.fetch(w.values(w.t_lo & 1), w.vbase, w.t_lo);
+    }
+#pragma nounroll
+    for (int t = w.t_lo; t <= w.t_hi; ++t) {
+        copies_landed();
+        const char* keys = w.keys(t & 1);
+        char* values = w.values(t & 1);
+        if (t < w.t_hi) {
+            w.fetch(w.keys((t + 1) & 1), w.kbase, t + 1);
+            w.fetch(w.values((t + 1) & 1), w.vbase, t + 1);
+        }
+        if (t < w.w_lo || t > w.w_hi) continue;
+        tile_scores<HDP>(s, keys, here(row_lane_), qf);
+#ifdef SCHED
+        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        const float l = halves_sum(sum[n]);
-        const bool valid = mask.q[n] < a.T;
-        const float factor = l == 0.f ? 0.f : 1.f / l;
-        fold = store_columns<HDP>(a.out + ((int64_t)b * a.T + mask.q[n]) * a.Nq * a.head_dim + (int64_t)head * a.head_dim, o[n], factor,
-                                  lane, a.head_dim, valid, fold);
-        if (valid && lane < 32)
-            a.lse[((int64_t)b * a.Nq + head) * a.T + mask.q[n]] =
-                m[n] == -__builtin_huge_valf() && l == 0.f ? m[n] : (m[n] * a.scale2 + __builtin_amdgcn_logf(l)) * kLn2;
+        for (int i = 0; i < W::kSteps; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
+#endif
+        if (!w.whole(t)) mask_scores(s, w, t);
+        top = -__builtin_huge_valf();
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, s[rb][i]);
+        top = halves_max(top);
+        // The maximum that the exponentials are taken against follows only when one has outgrown it by 2^8: the sums and
+        // the 16-bit probabilities lose nothing by a common factor of that size, and the accumulators are rarely rescaled.
+        if (__any((top - m) * a.scale2 > 8.f)) {
+            const float to = __builtin_fmaxf(m, top);
+            const float factor = to == -__builtin_huge_valf() ? 1.f : __builtin_amdgcn_exp2f((m - to) * a.scale2);
+            m = to;
+            sum[0] *= factor, sum[1] *= factor;
+#pragma unroll
+            for (int db = 0; db < W::kDims; ++db)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[db][i] *= factor;
+        }
+        const float ref = m == -__builtin_huge_valf() ? 0.f : m * a.scale2;
+        bf16x8 pf[4];
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[rb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][i], a.scale2, -ref));
+                sum[i & 1] += s[rb][i];
+            }
+            pf[2 * rb] = operand(s[rb], 0);
+            pf[2 * rb + 1] = operand(s[rb], 1);
+        }
+        const int cols_lane = here(cols_lane_);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int db = 0; db < W::kDims; ++db) o[db] = mfma(T::cols(values, cols_lane, db, u), pf[u], o[db]);
+    }
+
+#endif
+    const float l = halves_sum(sum[0] + sum[1]), inv = l == 0.f ? 0.f : 1.f / l;
+    if (w.valid() && w.lane < 32)
+        a.lse[w.statistic()] = m == -__builtin_huge_valf() && l == 0.f ? m : (m * a.scale2 + __builtin_amdgcn_logf(l)) * kLn2;
+    bool fine = true;
+#pragma unroll
+    for (int db = 0; db < W::kDims; ++db) fine &= all_finite(o[db]);
+    uint32_t fold = 0x7F807F80u;
+    if (!__syncthreads_or(!fine)) {
+        uint16_t* row = w.out_row();
+#pragma unroll
+        for (int db = 0; db < W::kDims; ++db) fold = store_columns(row, o[db], db, inv, w.lane, a.head_dim, w.valid(), fold);
+    } else {
+        fold = attention_forward_careful<HDP>(w, qf, m == -__builtin_huge_valf() ? 0.f : m * a.scale2, inv);
     }
     if (a.abs_max) {
         const uint32_t x = fold & 0xFFFFu, y = fold >> 16;
@@ -335,359 +474,387 @@ __global__ __launch_bounds__(WAVES * kWave, NB == 2 && HDP == 128 ? 1 : 2) void 
 // ---- backward: queries ---------------------------------------------------------------------------------------------------
 // dq, with D and the base-2 lse left for the other kernel.  The walk of the forward kernel with a third product:
 // transposed, s = K q, dp = V dout, dq = K^T ds.
-template <int HDP, int NB, int WAVES>
-__global__ __launch_bounds__(WAVES * kWave, NB == 2 && HDP == 128 ? 1 : 2) void attention_backward_q_kernel(AttentionArgs a) {
+
+// ds of 32 keys (row block rb) of a tile as operands, 0 in the places the mask excludes
+template <int HDP, typename Block>
+__device__ __forceinline__ void query_gradient(bf16x8 (&dsf)[2], const Block& w, const char* keys, const char* values, int row_lane, int t, int rb,
+                                               bool whole, const bf16x8 (&qf)[HDP / 16], const bf16x8 (&gf)[HDP / 16], float lse2, float delta) {
     typedef Tile<HDP, kKeys> T;
-    constexpr int kThreads = WAVES * kWave, kSteps = HDP / 16, kDims = HDP / 32;
-    __shared__ __attribute__((aligned(16))) char lds[2][2][T::kBytes];
-    const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-
-    const int ngroups = a.B * a.Nkv, nq = (a.T + 32 * NB * WAVES - 1) / (32 * NB * WAVES);
-    const int grp = blockIdx.x % ngroups, rest = blockIdx.x / ngroups;
-    const int b = grp / a.Nkv, kvh = grp % a.Nkv, head = kvh * a.G + rest % a.G;
-    const int q0 = (nq - 1 - rest / a.G) * (32 * NB * WAVES) + wave * (32 * NB);
-
-    const int64_t token = (int64_t)(a.Nq + 2 * a.Nkv) * a.head_dim, stride = token * 2;
-    const uint16_t* base = a.qkv + b * a.T * token;
-    const uint16_t* kbase = base + (int64_t)(a.Nq + kvh) * a.head_dim;
-    const auto ksrc = T::template source<kThreads>(kbase, tid, stride, a.head_dim);
-    auto vsrc = ksrc;
-    vsrc.p += (int64_t)a.Nkv * a.head_dim * 2;
-
-    QueryMask<NB> mask;
-    mask.load(a, b, q0, lane);
-    int lo, hi;
-    block_range<WAVES>(lo, hi, mask.lo, mask.hi);
-    const int t_lo = lo / kKeys, t_hi = hi / kKeys;
-
-    bf16x8 qf[NB][kSteps], gf[NB][kSteps];
-    float lse2[NB], delta[NB];
+    f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        const int q = min(mask.q[n], a.T - 1);
-        const int64_t at = ((int64_t)b * a.T + q) * a.Nq * a.head_dim + (int64_t)head * a.head_dim;
-        load_columns<HDP>(qf[n], base + q * token + (int64_t)head * a.head_dim, lane, a.head_dim);
-        load_columns<HDP>(gf[n], a.dout + at, lane, a.head_dim);
-        bf16x8 of[kSteps];
-        load_columns<HDP>(of, a.out + at, lane, a.head_dim);
-        float d = 0.f;
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) d = __builtin_fmaf((float)gf[n][s][j], (float)of[s][j], d);
-        delta[n] = halves_sum(d);
-        const int64_t stat = ((int64_t)b * a.Nq + head) * a.T;
-        lse2[n] = a.lse[stat + q] * kLog2e;
-        if (lane < 32 && mask.q[n] < a.T) {
-            a.delta[stat + q] = delta[n];
-            a.lse2[stat + q] = lse2[n];
-        }
-        // what the rows of this group may look at, for the walk over the queries; one head of the row writes it
-        if (a.first_key && head == 0) {
-            const bool in = mask.q[n] < a.T;
-            const int l = wave_min(in ? mask.first[n] : INT_MAX), f = wave_max(in ? mask.first[n] : 0);
-            const int g = (q0 >> 5) + n, ng = (a.T + 31) / 32;
-            if (lane == 0 && g < ng) a.groups[(int64_t)b * ng + g] = make_int2(l, f);
-        }
+    for (int st = 0; st < HDP / 16; ++st) {
+        s = mfma(T::rows(keys, row_lane, rb, st), qf[st], s);
+        dp = mfma(T::rows(values, row_lane, rb, st), gf[st], dp);
     }
-    const int row_lane = T::row_lane(lane), cols_lane = T::cols_lane(lane);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], w.a.scale2, -lse2));
+        s[i] = p * (dp[i] - delta);
+    }
+    if (!whole) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = w.allowed(t, rb, i) ? s[i] : 0.f;
+    }
+    dsf[0] = operand(s, 0);
+    dsf[1] = operand(s, 1);
+}
 
-    f32x16 dq[NB][kDims];
+template <int HDP, typename W>
+__device__ __forceinline__ void attention_backward_q_careful(const W& w, const bf16x8 (&qf)[W::kSteps], const bf16x8 (&gf)[W::kSteps], float lse2,
+                                                             float delta) {
+    typedef typename W::T T;
 #pragma nounroll
-    for (int careful = 0;; ++careful) {
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int db = 0; db < kDims; ++db) dq[n][db] = zero16();
-        if (lo <= hi) {
-            T::template stage<kThreads>(lds[0][0], ksrc, tid, stride, t_lo * kKeys, a.T);
-            T::template stage<kThreads>(lds[0][1], vsrc, tid, stride, t_lo * kKeys, a.T);
+    for (int db = 0; db < W::kDims; ++db) {
+        f32x16 one = zero16();
+#pragma nounroll
+        for (int t = w.t_lo; t <= w.t_hi; ++t) {
+            w.fetch(w.keys(0), w.kbase, t);
+            w.fetch(w.values(0), w.vbase, t);
             copies_landed();
-        }
+            if (t >= w.w_lo && t <= w.w_hi) {
 #pragma nounroll
-        for (int t = t_lo; lo <= hi && t <= t_hi; ++t) {
-            const int buf = (t - t_lo) & 1, k0 = t * kKeys;
-            if (t < t_hi) {
-                T::template stage<kThreads>(lds[buf ^ 1][0], ksrc, tid, stride, k0 + kKeys, a.T);
-                T::template stage<kThreads>(lds[buf ^ 1][1], vsrc, tid, stride, k0 + kKeys, a.T);
-            }
-            if (mask.touches(k0, k0 + kKeys - 1)) {
-                const bool whole = mask.whole(k0, k0 + kKeys - 1);
-#pragma unroll
                 for (int rb = 0; rb < 2; ++rb) {
-                    f32x16 s[NB], dp[NB];
+                    bf16x8 dsf[2];
+                    query_gradient<HDP>(dsf, w, w.keys(0), w.values(0), T::row_lane(here(w.lane)), t, rb, false, qf, gf, lse2, delta);
 #pragma unroll
-                    for (int n = 0; n < NB; ++n) s[n] = zero16(), dp[n] = zero16();
-#pragma unroll
-                    for (int st = 0; st < kSteps; ++st) {
-                        const bf16x8 kf = T::rows(lds[buf][0], row_lane, rb, st), vf = T::rows(lds[buf][1], row_lane, rb, st);
-#pragma unroll
-                        for (int n = 0; n < NB; ++n) {
-                            s[n] = mfma(kf, qf[n][st], s[n]);
-                            dp[n] = mfma(vf, gf[n][st], dp[n]);
-                        }
-                    }
-                    bf16x8 dsf[NB][2];
-#pragma unroll
-                    for (int n = 0; n < NB; ++n) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], a.scale2, -lse2[n]));
-                            s[n][i] = p * (dp[n][i] - delta[n]);
-                        }
-                        if (!whole) {
-#pragma unroll
-                            for (int i = 0; i < 16; ++i)
-                                if (!mask.allowed(n, k0 + tile_row(rb, i, lane))) s[n][i] = 0.f;
-                        }
-                        dsf[n][0] = operand(s[n], 0);
-                        dsf[n][1] = operand(s[n], 1);
-                    }
-                    if (careful == 0 || whole) {
-#pragma unroll
-                        for (int db = 0; db < kDims; ++db)
-#pragma unroll
-                            for (int u = 0; u < 2; ++u) {
-                                const bf16x8 kf = T::cols(lds[buf][0], cols_lane, db, 2 * rb + u);
-#pragma unroll
-                                for (int n = 0; n < NB; ++n) dq[n][db] = mfma(kf, dsf[n][u], dq[n][db]);
-                            }
-                    } else {
-#pragma unroll
-                        for (int n = 0; n < NB; ++n)
-#pragma unroll
-                            for (int u = 0; u < 2; ++u) {
-                                f32x16 one;
-#pragma unroll
-                                for (int i = 0; i < 16; ++i) one[i] = mask.allowed(n, k0 + tile_row(rb, i, lane)) ? 1.f : 0.f;
-                                const bf16x8 counts = operand(one, u);
-#pragma unroll
-                                for (int db = 0; db < kDims; ++db)
-                                    dq[n][db] = careful_product(T::cols(lds[buf][0], cols_lane, db, 2 * rb + u), dsf[n][u], counts,
-                                                                dq[n][db]);
-                            }
-                    }
+                    for (int u = 0; u < 2; ++u)
+                        one = careful_product(T::cols(w.keys(0), T::cols_lane(here(w.lane)), db, 2 * rb + u), dsf[u], w.counted(t, rb, u), one);
                 }
             }
-            copies_landed();
+            __syncthreads();
         }
-        if (careful) break;
-        bool fine = true;
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int db = 0; db < kDims; ++db) fine &= all_finite(dq[n][db]);
-        if (!__syncthreads_or(!fine)) break;
+        store_columns(w.dq_row(), one, db, w.a.scale, w.lane, w.a.head_dim, w.valid(), 0u);
     }
+}
+
+template <int HDP, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_q_kernel(AttentionArgs a) {
+    typedef QueryBlock<HDP, WAVES> W;
+    typedef typename W::T T;
+    __shared__ __attribute__((aligned(16))) char lds[W::kLdsBytes];
+    const W w(a, lds);
+
+    bf16x8 qf[W::kSteps], gf[W::kSteps];
+    w.load_rows(qf, w.base, w.token);
+    const int64_t out_row = (int64_t)a.Nq * a.head_dim;
+    w.load_rows(gf, a.dout + (int64_t)w.b * a.T * out_row, out_row);
+    float delta, lse2;
+    {
+        bf16x8 of[W::kSteps];
+        w.load_rows(of, a.out + (int64_t)w.b * a.T * out_row, out_row);
+        float d = 0.f;
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
-        store_columns<HDP>(a.dqkv + (b * a.T + (int64_t)mask.q[n]) * token + (int64_t)head * a.head_dim, dq[n], a.scale, lane, a.head_dim,
-                           mask.q[n] < a.T, 0u);
+        for (int s = 0; s < W::kSteps; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) d = __builtin_fmaf((float)gf[s][j], (float)of[s][j], d);
+        delta = halves_sum(d);
+        const int64_t stat = w.statistic();
+        lse2 = w.valid() ? a.lse[stat] * kLog2e : 0.f;
+        if (w.lane < 32 && w.valid()) {
+            a.delta[stat] = delta;
+            a.lse2[stat] = lse2;
+        }
+        // what the wave's rows may look at, for the walk over the queries; one head of the row writes it
+        if (a.first_key && w.head == 0 && w.valid() && w.lane == 0)
+            a.groups[(int64_t)w.b * ((a.T + 31) / 32) + w.mask.q[0] / 32] = make_int2(w.mask.lo, w.mask.first_max);
+    }
+    const int row_lane_ = T::row_lane(w.lane), cols_lane_ = T::cols_lane(w.lane);
+
+    f32x16 dq[W::kDims];
+#pragma unroll
+    for (int db = 0; db < W::kDims; ++db) dq[db] = zero16();
+    if (w.t_lo <= w.t_hi) {
+        w.fetch(w.keys(w.t_lo & 1), w.kbase, w.t_lo);
+        w.fetch(w.values(w.t_lo & 1), w.vbase, w.t_lo);
+    }
+#pragma nounroll
+    for (int t = w.t_lo; t <= w.t_hi; ++t) {
+        copies_landed();
+        char* keys = w.keys(t & 1);
+        const char* values = w.values(t & 1);
+        if (t < w.t_hi) {
+            w.fetch(w.keys((t + 1) & 1), w.kbase, t + 1);
+            w.fetch(w.values((t + 1) & 1), w.vbase, t + 1);
+        }
+        if (t < w.w_lo || t > w.w_hi) continue;
+        const bool whole = w.whole(t);
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+            bf16x8 dsf[2];
+            query_gradient<HDP>(dsf, w, keys, values, here(row_lane_), t, rb, whole, qf, gf, lse2, delta);
+            const int cols_lane = here(cols_lane_);
+#pragma unroll
+            for (int db = 0; db < W::kDims; ++db)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) dq[db] = mfma(T::cols(keys, cols_lane, db, 2 * rb + u), dsf[u], dq[db]);
+        }
+    }
+    bool fine = true;
+#pragma unroll
+    for (int db = 0; db < W::kDims; ++db) fine &= all_finite(dq[db]);
+    if (!__syncthreads_or(!fine)) {
+        uint16_t* row = w.dq_row();
+#pragma unroll
+        for (int db = 0; db < W::kDims; ++db) store_columns(row, dq[db], db, a.scale, w.lane, a.head_dim, w.valid(), 0u);
+    } else {
+        attention_backward_q_careful<HDP>(w, qf, gf, lse2, delta);
+    }
 }
 
 // ---- backward: keys and values -------------------------------------------------------------------------------------------
-// A wave owns 32 NB keys (columns) and walks the queries (rows) of every head of the group: s = Q k, dp = dout v,
-// dv = dout^T p, dk = Q^T ds.  A workgroup takes one of `splits` equal shares of the (head, query tile) pairs of its keys.
-template <int HDP, int NB, int WAVES>
-__global__ __launch_bounds__(WAVES * kWave, HDP == 128 ? 1 : 2) void attention_backward_kv_kernel(AttentionArgs a) {
-    typedef Tile<HDP, kKeys> T;
-    constexpr int kThreads = WAVES * kWave, kSteps = HDP / 16, kDims = HDP / 32, kBlock = 32 * NB * WAVES;
-    __shared__ __attribute__((aligned(16))) char lds[2][2][T::kBytes];      // [buffer][query, output gradient]
-    __shared__ __attribute__((aligned(16))) float stats[2][2][kKeys];       // [buffer][lse2, delta]
-    const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+// A wave owns 32 keys (columns) and walks the queries (rows), 32 at a time, of every head of the group: s = Q k, dp = dout v,
+// dv = dout^T p, dk = Q^T ds.  A workgroup takes one of `splits` equal shares of the (head, query tile) pairs of its keys.  The
+// accumulators fill half of the 256 registers that two waves per SIMD leave, the keys an eighth; the values stay in LDS.
+constexpr int kQueries = 32;
 
-    const int ngroups = a.B * a.Nkv;
-    const int grp = blockIdx.x % ngroups, rest = blockIdx.x / ngroups;
-    const int b = grp / a.Nkv, kvh = grp % a.Nkv, split = rest % a.splits, kt = rest / a.splits;   // the first keys have the most queries
-    const int kb0 = kt * kBlock, k0 = kb0 + wave * (32 * NB);
-    const int kb1 = min(kb0 + kBlock, a.T) - 1, k1 = min(k0 + 32 * NB, a.T) - 1;
+template <int HDP, int WAVES>
+struct KeyBlock {
+    static constexpr int kThreads = WAVES * kWave, kSteps = HDP / 16, kDims = HDP / 32, kBlock = 32 * WAVES;
+    typedef Tile<HDP, kQueries> T;
+    typedef Tile<HDP, kBlock> V;
+    // two buffers of a query tile and an output gradient tile, the values, two buffers of lse2, delta and first key
+    static constexpr int kValues = 4 * T::kBytes, kStats = kValues + V::kBytes, kLdsBytes = kStats + 2 * 3 * kQueries * 4;
 
-    const int64_t token = (int64_t)(a.Nq + 2 * a.Nkv) * a.head_dim, stride = token * 2, ostride = (int64_t)a.Nq * a.head_dim * 2;
-    const uint16_t* base = a.qkv + b * a.T * token;
+    const AttentionArgs& a;
+    char* lds;
+    int tid, lane, wave, b, kvh, split, k0, k1, ng;
+    int t_lo, tiles, first_pair, last_pair;
+    int64_t token, stride, ostride;
+    const uint16_t* base;
+    int key_;
 
-    // the query tiles that look at any of the workgroup's keys lie in [t_lo, t_hi]
-    const int ng = (a.T + 31) / 32;
-    int t_lo = kb0 / kKeys, t_hi = (a.T - 1) / kKeys;
-    if (a.first_key) {
-        int l = INT_MAX, h = -1;
-        for (int g = kb0 / 32 + tid; g < ng; g += kThreads)
-            if (a.groups[(int64_t)b * ng + g].x <= kb1) {
-                l = min(l, g);
-                h = max(h, g);
+    __device__ __forceinline__ KeyBlock(const AttentionArgs& args, char* lds_) : a(args), lds(lds_) {
+        tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+        const int ngroups = a.B * a.Nkv;
+        const int grp = blockIdx.x % ngroups, rest = blockIdx.x / ngroups;
+        b = grp / a.Nkv, kvh = grp % a.Nkv, split = rest % a.splits;
+        const int kb0 = rest / a.splits * kBlock, kb1 = min(kb0 + kBlock, a.T) - 1;   // the first keys, with the most queries, first
+        k0 = kb0 + wave * 32, k1 = min(k0 + 32, a.T) - 1;
+        key_ = k0 + (lane & 31);
+        token = (int64_t)(a.Nq + 2 * a.Nkv) * a.head_dim, stride = token * 2, ostride = (int64_t)a.Nq * a.head_dim * 2;
+        base = a.qkv + b * a.T * token;
+        if (a.head_dim < HDP) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) T::template clear<kThreads>(lds + i * T::kBytes, tid);
+            V::template clear<kThreads>(lds + kValues, tid);
+            __syncthreads();
+        }
+        // the query tiles that look at any of the workgroup's keys lie in [t_lo, t_lo + tiles)
+        ng = (a.T + 31) / 32;
+        t_lo = kb0 / kQueries;
+        int t_hi = ng - 1;
+        if (a.first_key) {
+            int l = INT_MAX, h = -1;
+            for (int g = t_lo + tid; g < ng; g += kThreads)
+                if (a.groups[(int64_t)b * ng + g].x <= kb1) {
+                    l = min(l, g);
+                    h = max(h, g);
+                }
+            block_range<WAVES>(l, h, wave_min(l), wave_max(h));
+            t_lo = l <= h ? l : 1;
+            t_hi = l <= h ? h : 0;
+        }
+        tiles = max(t_hi - t_lo + 1, 0);
+        const int64_t pairs = (int64_t)tiles * a.G;
+        first_pair = (int)(pairs * split / a.splits), last_pair = (int)(pairs * (split + 1) / a.splits);
+        V::template stage<kThreads>(lds + kValues, base + (int64_t)(a.Nq + a.Nkv + kvh) * a.head_dim,
+                                    V::template source<kThreads>(tid, stride, a.head_dim), tid, stride, kb0, a.T);
+    }
+    __device__ __forceinline__ void load_keys(bf16x8 (&kf)[kSteps]) const {
+        load_columns<HDP>(kf, base + min(key_, a.T - 1) * token + (int64_t)(a.Nq + kvh) * a.head_dim, lane, a.head_dim);
+    }
+    __device__ __forceinline__ char* queries(int buf) const { return lds + buf * T::kBytes; }
+    __device__ __forceinline__ char* gradients(int buf) const { return lds + (2 + buf) * T::kBytes; }
+    __device__ __forceinline__ const char* statistics(int buf, int which) const { return lds + kStats + (buf * 3 + which) * kQueries * 4; }
+    // head and first query of a pair
+    __device__ __forceinline__ void decode(int pair, int& head, int& q0) const {
+        const int h = pair / tiles;
+        head = kvh * a.G + h, q0 = (t_lo + pair - h * tiles) * kQueries;
+    }
+    __device__ __forceinline__ void fetch(int buf, int head, int q0) const {
+        const int id = here(tid), l = id % kWave;
+        T::template stage<kThreads>(queries(buf), base + (int64_t)head * a.head_dim, T::template source<kThreads>(id, stride, a.head_dim), id, stride,
+                                    q0, a.T);
+        T::template stage<kThreads>(gradients(buf), a.dout + ((int64_t)b * a.T * a.Nq + head) * a.head_dim,
+                                    T::template source<kThreads>(id, ostride, a.head_dim), id, ostride, q0, a.T);
+        if (wave < 3 && l < kQueries) {
+            const float* src = wave == 2 ? reinterpret_cast<const float*>(a.first_key) + (int64_t)b * a.T + q0 + l
+                                         : (wave == 0 ? a.lse2 : a.delta) + ((int64_t)b * a.Nq + head) * a.T + q0 + l;
+            if (q0 + l >= a.T || (wave == 2 && !a.first_key)) src = reinterpret_cast<const float*>(attention_zeros);
+            copy4(lds_address(statistics(buf, wave)), src);
+        }
+    }
+    // whether any of the tile's queries looks at one of the wave's keys, and whether all look at all
+    __device__ __forceinline__ bool touches(int q0, bool& whole) const {
+        int2 g = make_int2(0, 0);
+        if (a.first_key) {
+            g = a.groups[(int64_t)b * ng + (q0 >> 5)];
+            g = make_int2(__builtin_amdgcn_readfirstlane(g.x), __builtin_amdgcn_readfirstlane(g.y));
+        }
+        whole = q0 >= k1 && g.y <= k0;
+        return min(q0 + kQueries, a.T) - 1 >= k0 && g.x <= k1 && k0 < a.T;
+    }
+    // p and ds of the tile in `buf` as operands.  allowed: which of this lane's 16 rows may look at its key, where not `whole`.
+    // One branch around the mask alone: two forms of the step would meet with the accumulators in different registers.
+    __device__ __forceinline__ void gradient(bf16x8 (&pf)[2], bf16x8 (&dsf)[2], uint32_t& allowed, int buf, int q0, bool whole, int row_lane,
+                                             const bf16x8 (&kf)[kSteps]) const {
+        f32x16 s = zero16(), dp = zero16();
+        const char* value_rows = lds + kValues + wave * 32 * V::kRowBytes;
+#pragma unroll
+        for (int st = 0; st < kSteps; ++st) {
+            s = mfma(T::rows(queries(buf), row_lane, 0, st), kf[st], s);
+            dp = mfma(T::rows(gradients(buf), row_lane, 0, st), V::rows(value_rows, row_lane, 0, st), dp);
+        }
+        const int r0 = tile_row(0, 0, lane) * 4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float4 l4 = *reinterpret_cast<const float4*>(statistics(buf, 0) + r0 + 32 * j);
+            const float4 d4 = *reinterpret_cast<const float4*>(statistics(buf, 1) + r0 + 32 * j);
+            const float l[4] = {l4.x, l4.y, l4.z, l4.w}, d[4] = {d4.x, d4.y, d4.z, d4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int i = 4 * j + e;
+                s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, -l[e]));
+                dp[i] = s[i] * (dp[i] - d[e]);
             }
-        block_range<WAVES>(l, h, wave_min(l), wave_max(h));
-        t_lo = l <= h ? l / (kKeys / 32) : 1;
-        t_hi = l <= h ? h / (kKeys / 32) : 0;
-    }
-    const int tiles = max(t_hi - t_lo + 1, 0);
-    const int64_t pairs = (int64_t)tiles * a.G;
-    const int first_pair = (int)(pairs * split / a.splits), last_pair = (int)(pairs * (split + 1) / a.splits);
-
-    bf16x8 kf[NB][kSteps], vf[NB][kSteps];
-    int key[NB];
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        key[n] = k0 + 32 * n + (lane & 31);
-        const uint16_t* row = base + min(key[n], a.T - 1) * token + (int64_t)(a.Nq + kvh) * a.head_dim;
-        load_columns<HDP>(kf[n], row, lane, a.head_dim);
-        load_columns<HDP>(vf[n], row + (int64_t)a.Nkv * a.head_dim, lane, a.head_dim);
-    }
-    const int row_lane = T::row_lane(lane), cols_lane = T::cols_lane(lane);
-
-    auto qsrc = T::template source<kThreads>(base, tid, stride, a.head_dim);
-    auto gsrc = T::template source<kThreads>(a.dout + (int64_t)b * a.T * a.Nq * a.head_dim, tid, ostride, a.head_dim);
-    auto stage = [&](int buf, int pair) {
-        const int head = kvh * a.G + pair / tiles, q0 = (t_lo + pair % tiles) * kKeys;
-        auto q = qsrc, g = gsrc;
-        q.p += (int64_t)head * a.head_dim * 2;
-        g.p += (int64_t)head * a.head_dim * 2;
-        T::template stage<kThreads>(lds[buf][0], q, tid, stride, q0, a.T);
-        T::template stage<kThreads>(lds[buf][1], g, tid, ostride, q0, a.T);
-        if (wave < 2) {
-            const float* src = (wave == 0 ? a.lse2 : a.delta) + ((int64_t)b * a.Nq + head) * a.T + q0 + lane;
-            if (q0 + lane >= a.T) src = reinterpret_cast<const float*>(attention_zeros);
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                             (__attribute__((address_space(3))) void*)stats[buf][wave], 4, 0, 0);
         }
-    };
-
-    f32x16 dk[NB][kDims], dv[NB][kDims];
-#pragma nounroll
-    for (int careful = 0;; ++careful) {
+        allowed = 0xFFFFu;
+        if (!whole) {
+            const int key = here(key_);
+            allowed = 0;
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+            for (int j = 0; j < 4; ++j) {
+                const int4 f4 = *reinterpret_cast<const int4*>(statistics(buf, 2) + r0 + 32 * j);
+                const int first[4] = {f4.x, f4.y, f4.z, f4.w};
 #pragma unroll
-            for (int db = 0; db < kDims; ++db) dk[n][db] = zero16(), dv[n][db] = zero16();
-        if (first_pair < last_pair) {
-            stage(0, first_pair);
-            copies_landed();
-        }
-#pragma nounroll
-        for (int pair = first_pair; pair < last_pair; ++pair) {
-            const int buf = (pair - first_pair) & 1, q0 = (t_lo + pair % tiles) * kKeys;
-            if (pair + 1 < last_pair) stage(buf ^ 1, pair + 1);
-#pragma unroll
-            for (int rb = 0; rb < 2; ++rb) {
-                const int r0 = q0 + 32 * rb, r1 = min(r0 + 32, a.T) - 1;
-                int2 g = make_int2(0, 0);
-                if (a.first_key && r0 < a.T) g = a.groups[(int64_t)b * ng + (r0 >> 5)];
-                if (r0 >= a.T || r1 < k0 || g.x > k1 || k0 >= a.T) continue;
-                const bool whole = r0 >= k1 && g.y <= k0;
-                f32x16 s[NB], dp[NB];
-#pragma unroll
-                for (int n = 0; n < NB; ++n) s[n] = zero16(), dp[n] = zero16();
-#pragma unroll
-                for (int st = 0; st < kSteps; ++st) {
-                    const bf16x8 qf = T::rows(lds[buf][0], row_lane, rb, st), gf = T::rows(lds[buf][1], row_lane, rb, st);
-#pragma unroll
-                    for (int n = 0; n < NB; ++n) {
-                        s[n] = mfma(qf, kf[n][st], s[n]);
-                        dp[n] = mfma(gf, vf[n][st], dp[n]);
-                    }
-                }
-                float4 l4[4], d4[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    l4[j] = *reinterpret_cast<const float4*>(&stats[buf][0][tile_row(rb, 4 * j, lane)]);
-                    d4[j] = *reinterpret_cast<const float4*>(&stats[buf][1][tile_row(rb, 4 * j, lane)]);
-                }
-                uint32_t counts = 0xFFFFu;   // which of this lane's 16 rows may look at its key, for each block of keys
-                bf16x8 pf[NB][2], dsf[NB][2];
-                uint32_t allowed[NB];
-#pragma unroll
-                for (int n = 0; n < NB; ++n) {
-                    allowed[n] = counts;
-                    if (!whole) {
-                        allowed[n] = 0;
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int q = q0 + tile_row(rb, i, lane);
-                            const int first = a.first_key && q < a.T ? a.first_key[(int64_t)b * a.T + q] : 0;
-                            if (q >= key[n] && key[n] >= first && q < a.T) allowed[n] |= 1u << i;
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float l = i % 4 == 0 ? l4[i / 4].x : i % 4 == 1 ? l4[i / 4].y : i % 4 == 2 ? l4[i / 4].z : l4[i / 4].w;
-                        const float d = i % 4 == 0 ? d4[i / 4].x : i % 4 == 1 ? d4[i / 4].y : i % 4 == 2 ? d4[i / 4].z : d4[i / 4].w;
-                        s[n][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[n][i], a.scale2, -l));
-                        dp[n][i] = s[n][i] * (dp[n][i] - d);
-                    }
-                    if (!whole) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (!(allowed[n] >> i & 1)) s[n][i] = 0.f, dp[n][i] = 0.f;
-                    }
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        pf[n][u] = operand(s[n], u);
-                        dsf[n][u] = operand(dp[n], u);
-                    }
-                }
-                if (careful == 0 || whole) {
-#pragma unroll
-                    for (int db = 0; db < kDims; ++db)
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const bf16x8 gt = T::cols(lds[buf][1], cols_lane, db, 2 * rb + u);
-                            const bf16x8 qt = T::cols(lds[buf][0], cols_lane, db, 2 * rb + u);
-#pragma unroll
-                            for (int n = 0; n < NB; ++n) {
-                                dv[n][db] = mfma(gt, pf[n][u], dv[n][db]);
-                                dk[n][db] = mfma(qt, dsf[n][u], dk[n][db]);
-                            }
-                        }
-                } else {
-#pragma unroll
-                    for (int n = 0; n < NB; ++n)
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            f32x16 one;
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) one[i] = (allowed[n] >> i & 1) ? 1.f : 0.f;
-                            const bf16x8 ones = operand(one, u);
-#pragma unroll
-                            for (int db = 0; db < kDims; ++db) {
-                                dv[n][db] = careful_product(T::cols(lds[buf][1], cols_lane, db, 2 * rb + u), pf[n][u], ones, dv[n][db]);
-                                dk[n][db] = careful_product(T::cols(lds[buf][0], cols_lane, db, 2 * rb + u), dsf[n][u], ones, dk[n][db]);
-                            }
-                        }
+                for (int e = 0; e < 4; ++e) {
+                    const int i = 4 * j + e, q = q0 + tile_row(0, i, lane);
+                    const bool in = q >= key && key >= first[e] && q < a.T;
+                    allowed |= in ? 1u << i : 0u;
+                    s[i] = in ? s[i] : 0.f;
+                    dp[i] = in ? dp[i] : 0.f;
                 }
             }
-            copies_landed();
         }
-        if (careful) break;
-        bool fine = true;
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int db = 0; db < kDims; ++db) fine &= all_finite(dk[n][db]) && all_finite(dv[n][db]);
-        if (!__syncthreads_or(!fine)) break;
+        for (int u = 0; u < 2; ++u) {
+            pf[u] = operand(s, u);
+            dsf[u] = operand(dp, u);
+        }
     }
-
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        const bool valid = key[n] < a.T;
+    // dimensions 32 db ..: the partial sums of a split, or the gradients
+    __device__ __forceinline__ void put(int db, const f32x16& dk, const f32x16& dv) const {
+        const int key = here(key_);
+        const bool valid = key < a.T;
         if (a.partial) {
-            float* row = a.partial + ((((int64_t)split * a.B + b) * a.T + key[n]) * a.Nkv + kvh) * 2 * a.head_dim;
+            float* row = a.partial + ((((int64_t)split * a.B + b) * a.T + key) * a.Nkv + kvh) * 2 * a.head_dim;
 #pragma unroll
-            for (int db = 0; db < kDims; ++db)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int d = 32 * db + 8 * g + 4 * (lane >> 5);
-                    if (valid && d < a.head_dim) {
-                        *reinterpret_cast<float4*>(row + d) =
-                            make_float4(dk[n][db][4 * g], dk[n][db][4 * g + 1], dk[n][db][4 * g + 2], dk[n][db][4 * g + 3]);
-                        *reinterpret_cast<float4*>(row + a.head_dim + d) =
-                            make_float4(dv[n][db][4 * g], dv[n][db][4 * g + 1], dv[n][db][4 * g + 2], dv[n][db][4 * g + 3]);
-                    }
+            for (int g = 0; g < 4; ++g) {
+                const int d = 32 * db + 8 * g + 4 * (lane >> 5);
+                if (valid && d < a.head_dim) {
+                    *reinterpret_cast<float4*>(row + d) = make_float4(dk[4 * g], dk[4 * g + 1], dk[4 * g + 2], dk[4 * g + 3]);
+                    *reinterpret_cast<float4*>(row + a.head_dim + d) = make_float4(dv[4 * g], dv[4 * g + 1], dv[4 * g + 2], dv[4 * g + 3]);
                 }
+            }
         } else {
-            uint16_t* row = a.dqkv + ((int64_t)b * a.T + key[n]) * token + (int64_t)(a.Nq + kvh) * a.head_dim;
-            store_columns<HDP>(row, dk[n], a.scale, lane, a.head_dim, valid, 0u);
-            store_columns<HDP>(row + (int64_t)a.Nkv * a.head_dim, dv[n], 1.f, lane, a.head_dim, valid, 0u);
+            uint16_t* row = a.dqkv + ((int64_t)b * a.T + key) * token + (int64_t)(a.Nq + kvh) * a.head_dim;
+            store_columns(row, dk, db, a.scale, lane, a.head_dim, valid, 0u);
+            store_columns(row + (int64_t)a.Nkv * a.head_dim, dv, db, 1.f, lane, a.head_dim, valid, 0u);
         }
     }
+};
+
+template <int HDP, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_kernel(AttentionArgs a) {
+    typedef KeyBlock<HDP, WAVES> W;
+    typedef typename W::T T;
+    __shared__ __attribute__((aligned(16))) char lds[W::kLdsBytes];
+    const W w(a, lds);
+    bf16x8 kf[W::kSteps];
+    w.load_keys(kf);
+    const int row_lane_ = T::row_lane(w.lane), cols_lane_ = T::cols_lane(w.lane);
+
+    f32x16 dk[W::kDims], dv[W::kDims];
+#pragma unroll
+    for (int db = 0; db < W::kDims; ++db) dk[db] = zero16(), dv[db] = zero16();
+    int head, q0;
+    if (w.first_pair < w.last_pair) {
+        w.decode(w.first_pair, head, q0);
+        w.fetch(w.first_pair & 1, head, q0);
+    }
+#pragma nounroll
+    for (int pair = w.first_pair; pair < w.last_pair; ++pair) {
+        copies_landed();
+        const int buf = pair & 1, q = q0;
+        if (pair + 1 < w.last_pair) {
+            w.decode(pair + 1, head, q0);
+            w.fetch(buf ^ 1, head, q0);
+        }
+        bool whole;
+        if (!w.touches(q, whole)) continue;
+        bf16x8 pf[2], dsf[2];
+        uint32_t allowed;
+        w.gradient(pf, dsf, allowed, buf, q, whole, here(row_lane_), kf);
+        const int cols_lane = here(cols_lane_);
+#pragma unroll
+        for (int db = 0; db < W::kDims; ++db)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                dv[db] = mfma(T::cols(w.gradients(buf), cols_lane, db, u), pf[u], dv[db]);
+                dk[db] = mfma(T::cols(w.queries(buf), cols_lane, db, u), dsf[u], dk[db]);
+            }
+    }
+    copies_landed();   // the values, where the share is empty: no copy may outlive the workgroup
+    bool fine = true;
+#pragma unroll
+    for (int db = 0; db < W::kDims; ++db) fine &= all_finite(dk[db]) && all_finite(dv[db]);
+    const bool again = __syncthreads_or(!fine);
+    if (w.tid == 0) a.flags[blockIdx.x] = again;
+    if (!again) {
+#pragma unroll
+        for (int db = 0; db < W::kDims; ++db) w.put(db, dk[db], dv[db]);
+    }
+}
+
+// The careful form, a kernel of its own (in one with the loop above, its registers pushed accumulators of the loop out): the same
+// grid, of which the workgroups return whose result was finite.
+template <int HDP, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_careful_kernel(AttentionArgs a) {
+    typedef KeyBlock<HDP, WAVES> W;
+    typedef typename W::T T;
+    if (a.flags[blockIdx.x] == 0) return;
+    __shared__ __attribute__((aligned(16))) char lds[W::kLdsBytes];
+    const W w(a, lds);
+    bf16x8 kf[W::kSteps];
+    w.load_keys(kf);
+#pragma nounroll
+    for (int db = 0; db < W::kDims; ++db) {
+        f32x16 one_k = zero16(), one_v = zero16();
+#pragma nounroll
+        for (int pair = w.first_pair; pair < w.last_pair; ++pair) {
+            int head, q0;
+            w.decode(pair, head, q0);
+            w.fetch(0, head, q0);
+            copies_landed();
+            bool whole;
+            if (w.touches(q0, whole)) {
+                bf16x8 pf[2], dsf[2];
+                uint32_t allowed;
+                w.gradient(pf, dsf, allowed, 0, q0, false, T::row_lane(w.lane), kf);
+                f32x16 in;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) in[i] = (allowed >> i & 1) ? 1.f : 0.f;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    one_k = careful_product(T::cols(w.queries(0), T::cols_lane(w.lane), db, u), dsf[u], operand(in, u), one_k);
+                    one_v = careful_product(T::cols(w.gradients(0), T::cols_lane(w.lane), db, u), pf[u], operand(in, u), one_v);
+                }
+            }
+            __syncthreads();
+        }
+        w.put(db, one_k, one_v);
+    }
+    copies_landed();   // the values, where the share is empty
 }
 
 // Adds the splits' dk and dv in their order and rounds once.  A lane takes four values.
@@ -725,7 +892,7 @@ static int check_shape(const char* what, int B, int T, int Nq, int Nkv, int head
 // Shares of the walk over the queries: enough workgroups for two per compute unit, each with some tiles of work.
 static int kv_splits(int B, int T, int Nq, int Nkv, int keys) {
     const int64_t blocks = (int64_t)B * Nkv * ((T + keys - 1) / keys);
-    const int64_t pairs = (int64_t)((T + kKeys - 1) / kKeys) * (Nq / Nkv);
+    const int64_t pairs = (int64_t)((T + kQueries - 1) / kQueries) * (Nq / Nkv);
     int64_t s = (2 * kUnits + blocks - 1) / blocks;
     if (s > (pairs + 3) / 4) s = (pairs + 3) / 4;
     return (int)(s < 1 ? 1 : s > 16 ? 16 : s);
@@ -735,16 +902,19 @@ constexpr int kKvBlock = 128;
 
 struct BackwardPlan {
     int splits;
-    int64_t stats, groups, partial, bytes;   // bytes of each of the two statistics, the groups, the partial sums; all
+    int64_t blocks;                                 // workgroups of the keys' kernel
+    int64_t stats, flags, groups, partial, bytes;   // bytes of each of the two statistics, the flags, the groups, the partial sums; all
 };
 static BackwardPlan backward_plan(int B, int T, int Nq, int Nkv, int head_dim) {
     auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
     BackwardPlan p;
     p.splits = kv_splits(B, T, Nq, Nkv, kKvBlock);
     p.stats = up((int64_t)B * Nq * T * 4);
+    p.blocks = (int64_t)((T + kKvBlock - 1) / kKvBlock) * B * Nkv * p.splits;
+    p.flags = up(p.blocks * 4);
     p.groups = up((int64_t)B * ((T + 31) / 32) * 8);
     p.partial = p.splits > 1 ? up((int64_t)p.splits * B * T * Nkv * 2 * head_dim * 4) : 0;
-    p.bytes = 2 * p.stats + p.groups + p.partial;
+    p.bytes = 2 * p.stats + p.flags + p.groups + p.partial;
     return p;
 }
 
@@ -783,8 +953,8 @@ extern "C" int llmq_attention_forward_bf16(uint16_t* out, float* lse, const uint
     auto launch = [&](auto kernel, int queries, int threads) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)((T + queries - 1) / queries) * B * Nq), dim3(threads), 0, st, a);
     };
-    if (head_dim > 64) launch(attention_forward_kernel<128, 1, 4>, 128, 256);
-    else launch(attention_forward_kernel<64, 1, 4>, 128, 256);
+    if (head_dim > 64) launch(attention_forward_kernel<128, 4>, 128, 256);
+    else launch(attention_forward_kernel<64, 4>, 128, 256);
     LLMQ_HIP_TRY(hipGetLastError());
     return LLMQ_OK;
 }
@@ -813,22 +983,26 @@ extern "C" int llmq_attention_backward_bf16(uint16_t* dqkv, const uint16_t* dout
     char* s = static_cast<char*>(scratch);
     a.lse2 = reinterpret_cast<float*>(s);
     a.delta = reinterpret_cast<float*>(s + p.stats);
-    a.groups = reinterpret_cast<int2*>(s + 2 * p.stats);
-    a.partial = p.splits > 1 ? reinterpret_cast<float*>(s + 2 * p.stats + p.groups) : nullptr;
+    a.flags = reinterpret_cast<int*>(s + 2 * p.stats);
+    a.groups = reinterpret_cast<int2*>(s + 2 * p.stats + p.flags);
+    a.partial = p.splits > 1 ? reinterpret_cast<float*>(s + 2 * p.stats + p.flags + p.groups) : nullptr;
     a.splits = p.splits;
     auto launch = [&](auto kernel, int64_t blocks, int threads) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), 0, st, a);
     };
     const int64_t q_blocks = (int64_t)((T + 127) / 128) * B * Nq;
-    const int64_t kv_blocks = (int64_t)((T + kKvBlock - 1) / kKvBlock) * B * Nkv * p.splits;
     if (head_dim > 64) {
-        launch(attention_backward_q_kernel<128, 1, 4>, q_blocks, 256);
+        launch(attention_backward_q_kernel<128, 4>, q_blocks, 256);
         LLMQ_HIP_TRY(hipGetLastError());
-        launch(attention_backward_kv_kernel<128, 1, 4>, kv_blocks, 256);
+        launch(attention_backward_kv_kernel<128, 4>, p.blocks, 256);
+        LLMQ_HIP_TRY(hipGetLastError());
+        launch(attention_backward_kv_careful_kernel<128, 4>, p.blocks, 256);
     } else {
-        launch(attention_backward_q_kernel<64, 1, 4>, q_blocks, 256);
+        launch(attention_backward_q_kernel<64, 4>, q_blocks, 256);
         LLMQ_HIP_TRY(hipGetLastError());
-        launch(attention_backward_kv_kernel<64, 1, 4>, kv_blocks, 256);
+        launch(attention_backward_kv_kernel<64, 4>, p.blocks, 256);
+        LLMQ_HIP_TRY(hipGetLastError());
+        launch(attention_backward_kv_careful_kernel<64, 4>, p.blocks, 256);
     }
     LLMQ_HIP_TRY(hipGetLastError());
     if (p.splits > 1) {

@@ -25,8 +25,8 @@ typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
-// Source of the columns beyond head_dim and of the rows beyond the sequence: zeros, so that they add nothing and no value of
-// a neighbouring head or sequence, NaN or infinite, reaches a product.
+// Source of the rows beyond the sequence: zeros, so that they add nothing and no value of a neighbouring sequence, NaN or
+// infinite, reaches a product.
 __device__ const uint32_t __attribute__((aligned(16))) attention_zeros[4] = {0, 0, 0, 0};
 
 __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
@@ -56,43 +56,88 @@ __device__ __forceinline__ bf16x8 operand(const f32x16& x, int u) {
     return __builtin_bit_cast(bf16x8, w);
 }
 
-// A tile of ROWS rows of HDP bf16 in LDS, row-major, the 16-byte chunks of a row XORed with a function of the row: the 32 rows
-// that a fragment read takes at one chunk, and the 8 rows that a transposed read takes at four, then fall on different banks.
+// Copies from global memory straight into LDS, 16 or 4 bytes a lane, lane i to `lds` (one address for the wave) + 16 i or 4 i;
+// source: 32-bit lane offset from a scalar base, or one address a lane.  Inline assembly, because the compiler puts a wait for
+// every outstanding copy in front of the next LDS read, whatever it reads; what a kernel reads of a copy it reads behind
+// copies_landed().  The s_nop covers, whoever wrote the scalars, the five wait states between a vector instruction that writes a
+// scalar register and a memory instruction that reads it, and the one behind a write of M0.
+__device__ __forceinline__ uint32_t lds_address(const char* p) {
+    return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p);
+}
+__device__ __forceinline__ uint32_t to_m0(uint32_t lds) {
+    uint32_t m0;
+    asm volatile("s_mov_b32 %0, %1" : "={m0}"(m0) : "s"(lds));
+    return m0;
+}
+__device__ __forceinline__ void copy16(uint32_t lds, uint32_t offset, const char* wave_base) {
+    // (readfirstlane gives a signed int: its low word must not be sign-extended into the high one)
+    const uint64_t p = reinterpret_cast<uint64_t>(wave_base);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)p), hi = __builtin_amdgcn_readfirstlane((uint32_t)(p >> 32));
+    const uint64_t base = (uint64_t)hi << 32 | lo;
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "{m0}"(to_m0(lds)) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t lds, const char* p) {
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "{m0}"(to_m0(lds)) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t lds, const void* p) {
+    asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, off" : : "v"(p), "{m0}"(to_m0(lds)) : "memory");
+}
+// Waits for this wave's copies and for the other waves' to be waited for.
+__device__ __forceinline__ void copies_landed() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
+// A tile of ROWS rows of HDP bf16 in LDS, row-major, the 16-byte chunks of a row XORed with a function of the row.  A fragment
+// read takes one chunk of 32 rows, 16 rows a cycle; a transposed read takes four chunks of four rows a cycle: the low bits of the
+// row move the high bits of the chunk, so that the four rows' 64 bytes and the 16 rows' 16 bytes each cover all 64 banks once.
+// (With the row's bits XORed in order the transposed reads took 8 cycles instead of 2.)
 template <int HDP, int ROWS>
 struct Tile {
     static constexpr int kChunks = HDP / 8, kRowBytes = HDP * 2, kBytes = ROWS * kRowBytes;
 
-    static __device__ __forceinline__ int swizzle(int row) { return HDP == 128 ? (row & 15) : ((row >> 1) & 7); }
+    static __device__ __forceinline__ int swizzle(int row) {
+        return HDP == 128 ? ((row & 3) << 2 | ((row >> 2) & 3)) : ((row & 2) << 1 | ((row >> 2) & 3));
+    }
 
-    // Direct-to-LDS copies land linearly (lane i at 16 i), so the swizzle picks the source chunk.
+    // Direct-to-LDS copies land linearly (lane i at 16 i), so the swizzle picks the source chunk.  Lanes whose chunk lies beyond
+    // head_dim copy nothing: their places are cleared once (`clear`) and stay zero.
     struct Source {
-        const char* p;      // this lane's chunk of the tile's first rows
-        int row;            // and its row
+        uint32_t offset;    // of this lane's chunk from the tile's first row
+        int row;            // its row
         bool pad;           // a chunk beyond head_dim
     };
     template <int THREADS>
-    static __device__ __forceinline__ Source source(const uint16_t* head, int tid, int64_t stride_bytes, int head_dim) {
+    static __device__ __forceinline__ Source source(int tid, int64_t stride_bytes, int head_dim) {
         const int row = tid / kChunks, chunk = (tid % kChunks) ^ swizzle(row);
         Source s;
         s.row = row;
         s.pad = chunk * 8 >= head_dim;
-        s.p = reinterpret_cast<const char*>(head) + row * stride_bytes + chunk * 16;
+        s.offset = (uint32_t)(row * stride_bytes) + chunk * 16;
         return s;
     }
-    // rows row0 .. row0 + ROWS - 1 of the sequence, zeros from row `limit` on
     template <int THREADS>
-    static __device__ __forceinline__ void stage(char* lds, const Source& s, int tid, int64_t stride_bytes, int row0, int limit) {
+    static __device__ __forceinline__ void clear(char* lds, int tid) {
+        for (int i = tid * 16; i < kBytes; i += THREADS * 16) *reinterpret_cast<uint4*>(lds + i) = make_uint4(0, 0, 0, 0);
+    }
+    // rows row0 .. row0 + ROWS - 1 of the sequence whose row 0 is at `head`, zeros from row `limit` on
+    template <int THREADS>
+    static __device__ __forceinline__ void stage(char* lds, const uint16_t* head, const Source& s, int tid, int64_t stride_bytes, int row0, int limit) {
         constexpr int kStep = THREADS / kChunks;   // rows per copy instruction of the workgroup, a multiple of the swizzle's period
         static_assert(kStep % 16 == 0 && ROWS % kStep == 0, "the swizzle must repeat from copy to copy");
-        const char* base = s.p + (int64_t)row0 * stride_bytes;
-        char* dst = lds + (tid / kWave) * (kWave * 16);
-        const bool whole = row0 + ROWS <= limit;
+        const char* base = reinterpret_cast<const char*>(head) + (int64_t)row0 * stride_bytes;
+        const uint32_t dst = lds_address(lds + (tid / kWave) * (kWave * 16));
+        if (s.pad) return;
+        if (row0 + ROWS <= limit) {
 #pragma unroll
-        for (int i = 0; i < ROWS / kStep; ++i) {
-            const char* p = base + (int64_t)(i * kStep) * stride_bytes;
-            if (s.pad || (!whole && row0 + s.row + i * kStep >= limit)) p = reinterpret_cast<const char*>(attention_zeros);
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p,
-                                             (__attribute__((address_space(3))) void*)(dst + i * THREADS * 16), 16, 0, 0);
+            for (int i = 0; i < ROWS / kStep; ++i) copy16(dst + i * THREADS * 16, s.offset, base + (int64_t)(i * kStep) * stride_bytes);
+        } else {
+#pragma unroll
+            for (int i = 0; i < ROWS / kStep; ++i) {
+                const char* p = base + (int64_t)(i * kStep) * stride_bytes + s.offset;
+                if (row0 + s.row + i * kStep >= limit) p = reinterpret_cast<const char*>(attention_zeros);
+                copy16(dst + i * THREADS * 16, p);
+            }
         }
     }
 
@@ -111,8 +156,7 @@ struct Tile {
         return row * kRowBytes + ((chunk ^ swizzle(row)) << 4) + (lane & 1) * 8;
     }
     static __device__ __forceinline__ bf16x8 cols(char* lds, int lane_ofs, int db, int u) {
-        // eight rows further the swizzle differs in one bit: 8 for the wide rows, 4 for the narrow ones
-        constexpr int kFlip = HDP == 128 ? 128 : 64;
+        constexpr int kFlip = 32;   // eight rows further the swizzle differs in bit 1
         const int at = lane_ofs ^ (db << 6);
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(lds + at + u * 16 * kRowBytes));
         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(lds + (at ^ kFlip) + (u * 16 + 8) * kRowBytes));
