@@ -60,6 +60,9 @@ __device__ __forceinline__ void load_columns(bf16x8 (&f)[HDP / 16], const uint16
         const uint16_t* p = d < head_dim ? row + d : reinterpret_cast<const uint16_t*>(attention_zeros);
         f[s] = *reinterpret_cast<const bf16x8*>(p);
     }
+    // waited for here, not in every turn of the loop that uses them
+#pragma unroll
+    for (int s = 0; s < HDP / 16; ++s) asm volatile("" : "+v"(f[s]));
 }
 
 // Stores dimensions 32 db .. of a transposed result (dimensions by positions) times `factor` as bf16 to `row`, this lane's
@@ -163,26 +166,37 @@ __device__ __forceinline__ int here(int x) {
 }
 
 // ---- forward and the backward's queries: a workgroup's geometry ---------------------------------------------------------
-// A wave owns 32 queries (columns) and walks the keys (rows) in tiles of 64 that the workgroup's waves share in LDS.  What the
-// kernels and their careful forms have in common; `lds` holds two buffers of a key tile and a value tile.
+// A wave owns 32 queries (columns) and walks the keys (rows) in tiles of 64 that the workgroup's waves share in LDS: two buffers,
+// the next tile copied while one is computed.  A copy occupies the wave that issues it for about a hundred cycles when they come
+// in a row (eight of them were a quarter of a tile's time), so they are spread over the steps of the scores' product.  Behind the
+// last tile it is copied once more, so that the steps need no branch.
 template <int HDP, int WAVES>
 struct QueryBlock {
     typedef Tile<HDP, kKeys> T;
     static constexpr int kThreads = WAVES * kWave, kSteps = HDP / 16, kDims = HDP / 32, kBlock = 32 * WAVES;
     static constexpr int kLdsBytes = 4 * T::kBytes;
+    typedef TileCopy<HDP, kKeys, kThreads> Copy;
+    static constexpr int kCopies = 2 * Copy::kCopies;
+    static_assert(kCopies <= kSteps, "a copy a step");
 
     const AttentionArgs& a;
     char* lds;
+    uint32_t lds_at;            // address of the wave's share
     int tid, lane, b, kvh, head;
     int64_t token, stride;      // elements of a token, bytes
-    const uint16_t *base, *kbase, *vbase;
+    const uint16_t *base, *kbase;
+    Copy copy;
+    uint32_t ofs[Copy::kCopies];
+    const char *knext, *vnext;  // of the tile that is being copied
+    uint32_t to;                // and where
     QueryMask<1> mask;
     int t_lo, t_hi;             // tiles of the workgroup (t_lo > t_hi: none)
     int w_lo, w_hi;             // and of the wave
 
-    __device__ __forceinline__ QueryBlock(const AttentionArgs& args, char* lds_) : a(args), lds(lds_) {
+    __device__ __forceinline__ QueryBlock(const AttentionArgs& args, char* lds_) : a(args), lds(lds_), copy(threadIdx.x, args.head_dim) {
         tid = threadIdx.x, lane = tid % kWave;
         const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+        lds_at = lds_address(lds) + wave * 1024;
         // Workgroups go to the dies round-robin: the groups of heads that share keys are the fastest index, so that a group
         // stays on one die's L2 where their number allows; the last queries, which have the most keys, come first.
         const int ngroups = a.B * a.Nkv, nq = (a.T + kBlock - 1) / kBlock;
@@ -192,7 +206,6 @@ struct QueryBlock {
         token = (int64_t)(a.Nq + 2 * a.Nkv) * a.head_dim, stride = token * 2;
         base = a.qkv + b * a.T * token;
         kbase = base + (int64_t)(a.Nq + kvh) * a.head_dim;
-        vbase = kbase + (int64_t)a.Nkv * a.head_dim;
         if (a.head_dim < HDP) {   // block_range ends with a barrier
 #pragma unroll
             for (int i = 0; i < 4; ++i) T::template clear<kThreads>(lds + i * T::kBytes, tid);
@@ -202,12 +215,25 @@ struct QueryBlock {
         block_range<WAVES>(lo, hi, mask.lo, mask.hi);
         t_lo = lo <= hi ? lo / kKeys : 1, t_hi = lo <= hi ? hi / kKeys : 0;
         w_lo = mask.lo <= mask.hi ? mask.lo / kKeys : INT_MAX, w_hi = mask.lo <= mask.hi ? mask.hi / kKeys : -1;
+        copy.offsets(ofs, stride, 0, INT_MAX);
     }
     __device__ __forceinline__ char* keys(int buf) const { return lds + buf * T::kBytes; }
     __device__ __forceinline__ char* values(int buf) const { return lds + (2 + buf) * T::kBytes; }
-    __device__ __forceinline__ void fetch(char* to, const uint16_t* from, int t) const {
-        const int id = here(tid);
-        T::template stage<kThreads>(to, from, T::template source<kThreads>(id, stride, a.head_dim), id, stride, t * kKeys, a.T);
+    // copies of tile t (of the last one if it is behind it) into `buf`, one by one
+    __device__ __forceinline__ void aim(int buf, int t) {
+        const int row0 = min(t, t_hi) * kKeys;
+        if (row0 + kKeys > a.T) copy.offsets(ofs, stride, row0, a.T);   // the last tile of the sequence: none follows
+        knext = reinterpret_cast<const char*>(kbase) + row0 * stride;
+        vnext = knext + (int64_t)a.Nkv * a.head_dim * 2;
+        to = lds_at + buf * T::kBytes;
+    }
+    __device__ __forceinline__ void issue(int i) const {
+        if (i < Copy::kCopies) copy.copy(i, to, ofs, knext);
+        else if (i < kCopies) copy.copy(i - Copy::kCopies, to + 2 * T::kBytes, ofs, vnext);
+    }
+    __device__ __forceinline__ void issue_all() const {
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) issue(i);
     }
     __device__ __forceinline__ void load_rows(bf16x8 (&f)[kSteps], const uint16_t* tensor, int64_t row_elements) const {
         load_columns<HDP>(f, tensor + min(mask.q[0], a.T - 1) * row_elements + (int64_t)head * a.head_dim, lane, a.head_dim);
@@ -227,15 +253,27 @@ struct QueryBlock {
     __device__ __forceinline__ uint16_t* dq_row() const { return a.dqkv + ((int64_t)b * a.T + mask.q[0]) * token + (int64_t)head * a.head_dim; }
 };
 
-// s = K q of a key tile
-template <int HDP>
-__device__ __forceinline__ void tile_scores(f32x16 (&s)[2], const char* keys, int row_lane, const bf16x8 (&qf)[HDP / 16]) {
+constexpr int kAhead = 2;   // steps that fragments are read ahead of their matrix instructions
+
+// s = K q of a key tile; between(step) after each step
+template <int HDP, typename F>
+__device__ __forceinline__ void tile_scores(f32x16 (&s)[2], const char* keys, int row_lane, const bf16x8 (&qf)[HDP / 16], F between) {
     typedef Tile<HDP, kKeys> T;
+    constexpr int kSteps = HDP / 16;
+    bf16x8 kf[kSteps][2];
     s[0] = zero16(), s[1] = zero16();
 #pragma unroll
-    for (int st = 0; st < HDP / 16; ++st)
+    for (int st = -kAhead; st < kSteps; ++st) {
+        if (st + kAhead < kSteps) {
 #pragma unroll
-        for (int rb = 0; rb < 2; ++rb) s[rb] = mfma(T::rows(keys, row_lane, rb, st), qf[st], s[rb]);
+            for (int rb = 0; rb < 2; ++rb) kf[st + kAhead][rb] = T::rows(keys, row_lane, rb, st + kAhead);
+        }
+        if (st < 0) continue;
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) s[rb] = mfma(kf[st][rb], qf[st], s[rb]);
+        between(st);
+        __builtin_amdgcn_sched_barrier(0);
+    }
 }
 template <typename Block>
 __device__ __forceinline__ void mask_scores(f32x16 (&s)[2], const Block& w, int t) {
@@ -251,7 +289,7 @@ __device__ __forceinline__ void mask_scores(f32x16 (&s)[2], const Block& w, int 
 // places out.  The statistics stand: the scores see no values.  (As a function of its own it cost 20 us a launch: a kernel that
 // calls one reserves scratch memory.)
 template <int HDP, typename W>
-__device__ __forceinline__ uint32_t attention_forward_careful(const W& w, const bf16x8 (&qf)[W::kSteps], float ref, float inv) {
+__device__ __forceinline__ uint32_t attention_forward_careful(W& w, const bf16x8 (&qf)[W::kSteps], float ref, float inv) {
     typedef typename W::T T;
     uint32_t fold = 0x7F807F80u;
 #pragma nounroll
@@ -259,12 +297,12 @@ __device__ __forceinline__ uint32_t attention_forward_careful(const W& w, const 
         f32x16 one = zero16();
 #pragma nounroll
         for (int t = w.t_lo; t <= w.t_hi; ++t) {
-            w.fetch(w.keys(0), w.kbase, t);
-            w.fetch(w.values(0), w.vbase, t);
+            w.aim(0, t);
+            w.issue_all();
             copies_landed();
             if (t >= w.w_lo && t <= w.w_hi) {
                 f32x16 s[2];
-                tile_scores<HDP>(s, w.keys(0), T::row_lane(here(w.lane)), qf);
+                tile_scores<HDP>(s, w.keys(0), T::row_lane(here(w.lane)), qf, [](int) {});
                 mask_scores(s, w, t);
 #pragma unroll
                 for (int rb = 0; rb < 2; ++rb) {
@@ -282,138 +320,34 @@ __device__ __forceinline__ uint32_t attention_forward_careful(const W& w, const 
     return fold;
 }
 
-// Two waves per SIMD, and within a wave two tiles in flight: the exponentials of tile t are computed between the matrix
-// instructions of the scores of tile t + 1, so that neither unit waits for the other's latency.  Keys are copied two tiles
-// ahead and values one; one barrier a tile.
 template <int HDP, int WAVES>
 __global__ __launch_bounds__(WAVES * kWave, 2) void attention_forward_kernel(AttentionArgs a) {
     typedef QueryBlock<HDP, WAVES> W;
     typedef typename W::T T;
     __shared__ __attribute__((aligned(16))) char lds[W::kLdsBytes];
-    const W w(a, lds);
+    W w(a, lds);
     bf16x8 qf[W::kSteps];
     w.load_rows(qf, w.base, w.token);
 
     f32x16 o[W::kDims], s[2];
-    float m = -__builtin_huge_valf(), sum[2] = {0.f, 0.f}, top = 0.f;
+    float m = -__builtin_huge_valf(), sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int db = 0; db < W::kDims; ++db) o[db] = zero16();
     const int row_lane_ = T::row_lane(w.lane), cols_lane_ = T::cols_lane(w.lane);
 
-#ifdef PIPE
-    if (w.t_lo <= w.t_hi) w.fetch(w.keys(w.t_lo & 1), w.kbase, w.t_lo);
-#pragma nounroll
-    for (int t = w.t_lo - 1; t <= w.t_hi; ++t) {   // first turn: the scores of the first tile only
-        copies_landed();
-        const char* next_keys = w.keys((t + 1) & 1);
-        char* values = w.values(t & 1);
-        if (t + 2 <= w.t_hi) w.fetch(w.keys(t & 1), w.kbase, t + 2);
-        if (t + 1 <= w.t_hi) w.fetch(w.values((t + 1) & 1), w.vbase, t + 1);
-        const bool now = t >= w.w_lo && t <= w.w_hi, next = t + 1 >= w.w_lo && t + 1 <= w.w_hi;
-        float ref = 0.f;
-        if (now) {
-            // The maximum that the exponentials are taken against follows only when one has outgrown it by 2^8: the sums and
-            // the 16-bit probabilities lose nothing by a common factor of that size, and the accumulators are rarely rescaled.
-            if (__any((top - m) * a.scale2 > 8.f)) {
-                const float to = __builtin_fmaxf(m, top);
-                const float factor = to == -__builtin_huge_valf() ? 1.f : __builtin_amdgcn_exp2f((m - to) * a.scale2);
-                m = to;
-                sum[0] *= factor, sum[1] *= factor;
-#pragma unroll
-                for (int db = 0; db < W::kDims; ++db)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[db][i] *= factor;
-            }
-            ref = m == -__builtin_huge_valf() ? 0.f : m * a.scale2;
-        }
-        auto probabilities = [&](bf16x8 (&pf)[4]) {
-#pragma unroll
-            for (int rb = 0; rb < 2; ++rb) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    s[rb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][i], a.scale2, -ref));
-                    sum[i & 1] += s[rb][i];
-                }
-                pf[2 * rb] = operand(s[rb], 0);
-                pf[2 * rb + 1] = operand(s[rb], 1);
-            }
-        };
-        auto accumulate = [&](const bf16x8 (&pf)[4]) {
-            const int cols_lane = here(cols_lane_);
-#pragma unroll
-            for (int db = 0; db < W::kDims; ++db)
-#pragma unroll
-                for (int u = 0; u < 4; ++u) o[db] = mfma(T::cols(values, cols_lane, db, u), pf[u], o[db]);
-        };
-        if (now && next) {
-            bf16x8 pf[4];
-            f32x16 ahead[2];
-            tile_scores<HDP>(ahead, next_keys, here(row_lane_), qf);
-            probabilities(pf);
-#ifdef SCHED
-            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-            for (int i = 0; i < 2 * W::kSteps; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x002, 5 * 128 / HDP, 0);
-                __builtin_amdgcn_sched_group_barrier(0x400, 2 * 128 / HDP, 0);
-            }
-#endif
-            accumulate(pf);
-#ifdef SCHED
-            __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-            for (int i = 0; i < 4 * W::kDims; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-            }
-#endif
-            s[0] = ahead[0], s[1] = ahead[1];
-        } else if (now) {
-            bf16x8 pf[4];
-            probabilities(pf);
-            accumulate(pf);
-        } else if (next) {
-            tile_scores<HDP>(s, next_keys, here(row_lane_), qf);
-        }
-        if (next) {
-            if (!w.whole(t + 1)) mask_scores(s, w, t + 1);
-            top = -__builtin_huge_valf();
-#pragma unroll
-            for (int rb = 0; rb < 2; ++rb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, s[rb][i]);
-            top = halves_max(top);
-        }
-    }
-
-#else
     if (w.t_lo <= w.t_hi) {
-        w.fetch(w.keys(w.t_lo & 1), w.kbase, w.t_lo);
-        w.fetch(w.values(w.t_lo & 1), w.vbase, w.t_lo);
+        w.aim(w.t_lo & 1, w.t_lo);
+        w.issue_all();
     }
 #pragma nounroll
     for (int t = w.t_lo; t <= w.t_hi; ++t) {
         copies_landed();
         const char* keys = w.keys(t & 1);
         char* values = w.values(t & 1);
-        if (t < w.t_hi) {
-            w.fetch(w.keys((t + 1) & 1), w.kbase, t + 1);
-            w.fetch(w.values((t + 1) & 1), w.vbase, t + 1);
-        }
-        if (t < w.w_lo || t > w.w_hi) continue;
-        tile_scores<HDP>(s, keys, here(row_lane_), qf);
-#ifdef SCHED
-        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
-#pragma unroll
-        for (int i = 0; i < W::kSteps; ++i) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-        }
-#endif
+        w.aim((t + 1) & 1, t + 1);
+        tile_scores<HDP>(s, keys, here(row_lane_), qf, [&](int st) { w.issue(st); });
         if (!w.whole(t)) mask_scores(s, w, t);
-        top = -__builtin_huge_valf();
+        float top = -__builtin_huge_valf();
 #pragma unroll
         for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
@@ -450,7 +384,6 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_forward_kernel(Att
             for (int db = 0; db < W::kDims; ++db) o[db] = mfma(T::cols(values, cols_lane, db, u), pf[u], o[db]);
     }
 
-#endif
     const float l = halves_sum(sum[0] + sum[1]), inv = l == 0.f ? 0.f : 1.f / l;
     if (w.valid() && w.lane < 32)
         a.lse[w.statistic()] = m == -__builtin_huge_valf() && l == 0.f ? m : (m * a.scale2 + __builtin_amdgcn_logf(l)) * kLn2;
@@ -458,6 +391,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_forward_kernel(Att
 #pragma unroll
     for (int db = 0; db < W::kDims; ++db) fine &= all_finite(o[db]);
     uint32_t fold = 0x7F807F80u;
+    copies_landed();   // the surplus ones: no copy may outlive the workgroup
     if (!__syncthreads_or(!fine)) {
         uint16_t* row = w.out_row();
 #pragma unroll
@@ -475,16 +409,26 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_forward_kernel(Att
 // dq, with D and the base-2 lse left for the other kernel.  The walk of the forward kernel with a third product:
 // transposed, s = K q, dp = V dout, dq = K^T ds.
 
-// ds of 32 keys (row block rb) of a tile as operands, 0 in the places the mask excludes
-template <int HDP, typename Block>
+// ds of 32 keys (row block rb) of a tile as operands, 0 in the places the mask excludes; between(step) after each step
+template <int HDP, typename Block, typename F>
 __device__ __forceinline__ void query_gradient(bf16x8 (&dsf)[2], const Block& w, const char* keys, const char* values, int row_lane, int t, int rb,
-                                               bool whole, const bf16x8 (&qf)[HDP / 16], const bf16x8 (&gf)[HDP / 16], float lse2, float delta) {
+                                               bool whole, const bf16x8 (&qf)[HDP / 16], const bf16x8 (&gf)[HDP / 16], float lse2, float delta,
+                                               F between) {
     typedef Tile<HDP, kKeys> T;
+    constexpr int kSteps = HDP / 16;
     f32x16 s = zero16(), dp = zero16();
+    bf16x8 kf[kSteps], vf[kSteps];
 #pragma unroll
-    for (int st = 0; st < HDP / 16; ++st) {
-        s = mfma(T::rows(keys, row_lane, rb, st), qf[st], s);
-        dp = mfma(T::rows(values, row_lane, rb, st), gf[st], dp);
+    for (int st = -kAhead; st < kSteps; ++st) {
+        if (st + kAhead < kSteps) {
+            kf[st + kAhead] = T::rows(keys, row_lane, rb, st + kAhead);
+            vf[st + kAhead] = T::rows(values, row_lane, rb, st + kAhead);
+        }
+        if (st < 0) continue;
+        s = mfma(kf[st], qf[st], s);
+        dp = mfma(vf[st], gf[st], dp);
+        between(st);
+        __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -500,7 +444,7 @@ __device__ __forceinline__ void query_gradient(bf16x8 (&dsf)[2], const Block& w,
 }
 
 template <int HDP, typename W>
-__device__ __forceinline__ void attention_backward_q_careful(const W& w, const bf16x8 (&qf)[W::kSteps], const bf16x8 (&gf)[W::kSteps], float lse2,
+__device__ __forceinline__ void attention_backward_q_careful(W& w, const bf16x8 (&qf)[W::kSteps], const bf16x8 (&gf)[W::kSteps], float lse2,
                                                              float delta) {
     typedef typename W::T T;
 #pragma nounroll
@@ -508,14 +452,14 @@ __device__ __forceinline__ void attention_backward_q_careful(const W& w, const b
         f32x16 one = zero16();
 #pragma nounroll
         for (int t = w.t_lo; t <= w.t_hi; ++t) {
-            w.fetch(w.keys(0), w.kbase, t);
-            w.fetch(w.values(0), w.vbase, t);
+            w.aim(0, t);
+            w.issue_all();
             copies_landed();
             if (t >= w.w_lo && t <= w.w_hi) {
 #pragma nounroll
                 for (int rb = 0; rb < 2; ++rb) {
                     bf16x8 dsf[2];
-                    query_gradient<HDP>(dsf, w, w.keys(0), w.values(0), T::row_lane(here(w.lane)), t, rb, false, qf, gf, lse2, delta);
+                    query_gradient<HDP>(dsf, w, w.keys(0), w.values(0), T::row_lane(here(w.lane)), t, rb, false, qf, gf, lse2, delta, [](int) {});
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
                         one = careful_product(T::cols(w.keys(0), T::cols_lane(here(w.lane)), db, 2 * rb + u), dsf[u], w.counted(t, rb, u), one);
@@ -532,7 +476,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_q_kernel(
     typedef QueryBlock<HDP, WAVES> W;
     typedef typename W::T T;
     __shared__ __attribute__((aligned(16))) char lds[W::kLdsBytes];
-    const W w(a, lds);
+    W w(a, lds);
 
     bf16x8 qf[W::kSteps], gf[W::kSteps];
     w.load_rows(qf, w.base, w.token);
@@ -564,24 +508,22 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_q_kernel(
 #pragma unroll
     for (int db = 0; db < W::kDims; ++db) dq[db] = zero16();
     if (w.t_lo <= w.t_hi) {
-        w.fetch(w.keys(w.t_lo & 1), w.kbase, w.t_lo);
-        w.fetch(w.values(w.t_lo & 1), w.vbase, w.t_lo);
+        w.aim(w.t_lo & 1, w.t_lo);
+        w.issue_all();
     }
 #pragma nounroll
     for (int t = w.t_lo; t <= w.t_hi; ++t) {
         copies_landed();
         char* keys = w.keys(t & 1);
         const char* values = w.values(t & 1);
-        if (t < w.t_hi) {
-            w.fetch(w.keys((t + 1) & 1), w.kbase, t + 1);
-            w.fetch(w.values((t + 1) & 1), w.vbase, t + 1);
-        }
-        if (t < w.w_lo || t > w.w_hi) continue;
+        w.aim((t + 1) & 1, t + 1);
         const bool whole = w.whole(t);
 #pragma unroll
         for (int rb = 0; rb < 2; ++rb) {
             bf16x8 dsf[2];
-            query_gradient<HDP>(dsf, w, keys, values, here(row_lane_), t, rb, whole, qf, gf, lse2, delta);
+            query_gradient<HDP>(dsf, w, keys, values, here(row_lane_), t, rb, whole, qf, gf, lse2, delta, [&](int st) {
+                if (rb == 0) w.issue(st);
+            });
             const int cols_lane = here(cols_lane_);
 #pragma unroll
             for (int db = 0; db < W::kDims; ++db)
@@ -592,6 +534,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_q_kernel(
     bool fine = true;
 #pragma unroll
     for (int db = 0; db < W::kDims; ++db) fine &= all_finite(dq[db]);
+    copies_landed();
     if (!__syncthreads_or(!fine)) {
         uint16_t* row = w.dq_row();
 #pragma unroll
@@ -614,17 +557,28 @@ struct KeyBlock {
     typedef Tile<HDP, kBlock> V;
     // two buffers of a query tile and an output gradient tile, the values, two buffers of lse2, delta and first key
     static constexpr int kValues = 4 * T::kBytes, kStats = kValues + V::kBytes, kLdsBytes = kStats + 2 * 3 * kQueries * 4;
+    typedef TileCopy<HDP, kQueries, kThreads> Copy;
+    static constexpr int kCopies = 2 * Copy::kCopies + 1;
+    static_assert(kCopies <= kSteps, "a copy a step");
 
     const AttentionArgs& a;
     char* lds;
+    uint32_t lds_at;
     int tid, lane, wave, b, kvh, split, k0, k1, ng;
     int t_lo, tiles, first_pair, last_pair;
     int64_t token, stride, ostride;
     const uint16_t* base;
     int key_;
+    Copy copy;
+    uint32_t qofs[Copy::kCopies], gofs[Copy::kCopies];
+    const char *qnext, *gnext;   // of the tile that is being copied
+    const float* snext;
+    uint32_t to, sto;            // and where
+    uint64_t slanes;
 
-    __device__ __forceinline__ KeyBlock(const AttentionArgs& args, char* lds_) : a(args), lds(lds_) {
+    __device__ __forceinline__ KeyBlock(const AttentionArgs& args, char* lds_) : a(args), lds(lds_), copy(threadIdx.x, args.head_dim) {
         tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+        lds_at = lds_address(lds) + wave * 1024;
         const int ngroups = a.B * a.Nkv;
         const int grp = blockIdx.x % ngroups, rest = blockIdx.x / ngroups;
         b = grp / a.Nkv, kvh = grp % a.Nkv, split = rest % a.splits;
@@ -657,8 +611,18 @@ struct KeyBlock {
         tiles = max(t_hi - t_lo + 1, 0);
         const int64_t pairs = (int64_t)tiles * a.G;
         first_pair = (int)(pairs * split / a.splits), last_pair = (int)(pairs * (split + 1) / a.splits);
-        V::template stage<kThreads>(lds + kValues, base + (int64_t)(a.Nq + a.Nkv + kvh) * a.head_dim,
-                                    V::template source<kThreads>(tid, stride, a.head_dim), tid, stride, kb0, a.T);
+        copy.offsets(qofs, stride, 0, INT_MAX);
+        copy.offsets(gofs, ostride, 0, INT_MAX);
+        slanes = wave < 3 ? 0xFFFFFFFFull : 0;
+        if (first_pair < last_pair) {
+            typedef TileCopy<HDP, kBlock, kThreads> ValueCopy;
+            const ValueCopy vcopy(tid, a.head_dim);
+            uint32_t vofs[ValueCopy::kCopies];
+            vcopy.offsets(vofs, stride, kb0, a.T);
+            const char* v = reinterpret_cast<const char*>(base + (int64_t)(a.Nq + a.Nkv + kvh) * a.head_dim) + kb0 * stride;
+#pragma unroll
+            for (int i = 0; i < ValueCopy::kCopies; ++i) vcopy.copy(i, lds_at + kValues, vofs, v);
+        }
     }
     __device__ __forceinline__ void load_keys(bf16x8 (&kf)[kSteps]) const {
         load_columns<HDP>(kf, base + min(key_, a.T - 1) * token + (int64_t)(a.Nq + kvh) * a.head_dim, lane, a.head_dim);
@@ -666,44 +630,71 @@ struct KeyBlock {
     __device__ __forceinline__ char* queries(int buf) const { return lds + buf * T::kBytes; }
     __device__ __forceinline__ char* gradients(int buf) const { return lds + (2 + buf) * T::kBytes; }
     __device__ __forceinline__ const char* statistics(int buf, int which) const { return lds + kStats + (buf * 3 + which) * kQueries * 4; }
-    // head and first query of a pair
-    __device__ __forceinline__ void decode(int pair, int& head, int& q0) const {
+    // Head and first query of a pair (of the last one if it is behind it) and what its queries may look at.
+    struct Pair {
+        int head, q0;
+        int2 group;
+    };
+    __device__ __forceinline__ Pair decode(int pair) const {
+        pair = min(pair, last_pair - 1);
         const int h = pair / tiles;
-        head = kvh * a.G + h, q0 = (t_lo + pair - h * tiles) * kQueries;
+        Pair p;
+        p.head = kvh * a.G + h, p.q0 = (t_lo + pair - h * tiles) * kQueries;
+        p.group = make_int2(0, 0);
+        if (a.first_key) p.group = a.groups[(int64_t)b * ng + (p.q0 >> 5)];
+        return p;
     }
-    __device__ __forceinline__ void fetch(int buf, int head, int q0) const {
-        const int id = here(tid), l = id % kWave;
-        T::template stage<kThreads>(queries(buf), base + (int64_t)head * a.head_dim, T::template source<kThreads>(id, stride, a.head_dim), id, stride,
-                                    q0, a.T);
-        T::template stage<kThreads>(gradients(buf), a.dout + ((int64_t)b * a.T * a.Nq + head) * a.head_dim,
-                                    T::template source<kThreads>(id, ostride, a.head_dim), id, ostride, q0, a.T);
-        if (wave < 3 && l < kQueries) {
-            const float* src = wave == 2 ? reinterpret_cast<const float*>(a.first_key) + (int64_t)b * a.T + q0 + l
-                                         : (wave == 0 ? a.lse2 : a.delta) + ((int64_t)b * a.Nq + head) * a.T + q0 + l;
-            if (q0 + l >= a.T || (wave == 2 && !a.first_key)) src = reinterpret_cast<const float*>(attention_zeros);
-            copy4(lds_address(statistics(buf, wave)), src);
+    __device__ __forceinline__ void aim(int buf, const Pair& p) {
+        if (p.q0 + kQueries > a.T || qnext_clamped) {   // the last tile of the sequence, and the one behind it
+            copy.offsets(qofs, stride, p.q0, a.T);
+            copy.offsets(gofs, ostride, p.q0, a.T);
+            qnext_clamped = p.q0 + kQueries > a.T;
         }
+        qnext = reinterpret_cast<const char*>(base + (int64_t)p.head * a.head_dim) + p.q0 * stride;
+        gnext = reinterpret_cast<const char*>(a.dout + ((int64_t)b * a.T * a.Nq + p.head) * a.head_dim) + p.q0 * ostride;
+        const int q = min(p.q0 + (lane & 31), a.T - 1);
+        const int64_t row = ((int64_t)b * a.Nq + p.head) * a.T;
+        snext = wave == 0 ? a.lse2 + row + q : wave == 1 || !a.first_key ? a.delta + row + q
+                                                                         : reinterpret_cast<const float*>(a.first_key) + (int64_t)b * a.T + q;
+        to = lds_at + buf * T::kBytes;
+        sto = lds_at - wave * 1024 + kStats + (buf * 3 + min(wave, 2)) * kQueries * 4;
+    }
+    bool qnext_clamped = false;
+    __device__ __forceinline__ void issue(int i) const {
+        if (i < Copy::kCopies) copy.copy(i, to, qofs, qnext);
+        else if (i < 2 * Copy::kCopies) copy.copy(i - Copy::kCopies, to + 2 * T::kBytes, gofs, gnext);
+        else if (i < kCopies) copy4(sto, snext, slanes);
+    }
+    __device__ __forceinline__ void issue_all() const {
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) issue(i);
     }
     // whether any of the tile's queries looks at one of the wave's keys, and whether all look at all
-    __device__ __forceinline__ bool touches(int q0, bool& whole) const {
-        int2 g = make_int2(0, 0);
-        if (a.first_key) {
-            g = a.groups[(int64_t)b * ng + (q0 >> 5)];
-            g = make_int2(__builtin_amdgcn_readfirstlane(g.x), __builtin_amdgcn_readfirstlane(g.y));
-        }
-        whole = q0 >= k1 && g.y <= k0;
-        return min(q0 + kQueries, a.T) - 1 >= k0 && g.x <= k1 && k0 < a.T;
+    __device__ __forceinline__ bool touches(const Pair& p, bool& whole) const {
+        const int lo = __builtin_amdgcn_readfirstlane(p.group.x), top = __builtin_amdgcn_readfirstlane(p.group.y);
+        whole = p.q0 >= k1 && top <= k0 && p.q0 + kQueries <= a.T;
+        return min(p.q0 + kQueries, a.T) - 1 >= k0 && lo <= k1 && k0 < a.T;
     }
     // p and ds of the tile in `buf` as operands.  allowed: which of this lane's 16 rows may look at its key, where not `whole`.
     // One branch around the mask alone: two forms of the step would meet with the accumulators in different registers.
+    template <typename F>
     __device__ __forceinline__ void gradient(bf16x8 (&pf)[2], bf16x8 (&dsf)[2], uint32_t& allowed, int buf, int q0, bool whole, int row_lane,
-                                             const bf16x8 (&kf)[kSteps]) const {
+                                             const bf16x8 (&kf)[kSteps], F between) const {
         f32x16 s = zero16(), dp = zero16();
         const char* value_rows = lds + kValues + wave * 32 * V::kRowBytes;
+        bf16x8 qf[kSteps], gf[kSteps], vf[kSteps];
 #pragma unroll
-        for (int st = 0; st < kSteps; ++st) {
-            s = mfma(T::rows(queries(buf), row_lane, 0, st), kf[st], s);
-            dp = mfma(T::rows(gradients(buf), row_lane, 0, st), V::rows(value_rows, row_lane, 0, st), dp);
+        for (int st = -kAhead; st < kSteps; ++st) {
+            if (st + kAhead < kSteps) {
+                qf[st + kAhead] = T::rows(queries(buf), row_lane, 0, st + kAhead);
+                gf[st + kAhead] = T::rows(gradients(buf), row_lane, 0, st + kAhead);
+                vf[st + kAhead] = V::rows(value_rows, row_lane, 0, st + kAhead);
+            }
+            if (st < 0) continue;
+            s = mfma(qf[st], kf[st], s);
+            dp = mfma(gf[st], vf[st], dp);
+            between(st);
+            __builtin_amdgcn_sched_barrier(0);
         }
         const int r0 = tile_row(0, 0, lane) * 4;
 #pragma unroll
@@ -729,7 +720,7 @@ struct KeyBlock {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int i = 4 * j + e, q = q0 + tile_row(0, i, lane);
-                    const bool in = q >= key && key >= first[e] && q < a.T;
+                    const bool in = q >= key && (!a.first_key || key >= first[e]) && q < a.T;
                     allowed |= in ? 1u << i : 0u;
                     s[i] = in ? s[i] : 0.f;
                     dp[i] = in ? dp[i] : 0.f;
@@ -769,7 +760,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_kernel
     typedef KeyBlock<HDP, WAVES> W;
     typedef typename W::T T;
     __shared__ __attribute__((aligned(16))) char lds[W::kLdsBytes];
-    const W w(a, lds);
+    W w(a, lds);
     bf16x8 kf[W::kSteps];
     w.load_keys(kf);
     const int row_lane_ = T::row_lane(w.lane), cols_lane_ = T::cols_lane(w.lane);
@@ -777,24 +768,27 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_kernel
     f32x16 dk[W::kDims], dv[W::kDims];
 #pragma unroll
     for (int db = 0; db < W::kDims; ++db) dk[db] = zero16(), dv[db] = zero16();
-    int head, q0;
+    typename W::Pair next;
     if (w.first_pair < w.last_pair) {
-        w.decode(w.first_pair, head, q0);
-        w.fetch(w.first_pair & 1, head, q0);
+        next = w.decode(w.first_pair);
+        w.aim(w.first_pair & 1, next);
+        w.issue_all();
     }
 #pragma nounroll
     for (int pair = w.first_pair; pair < w.last_pair; ++pair) {
         copies_landed();
-        const int buf = pair & 1, q = q0;
-        if (pair + 1 < w.last_pair) {
-            w.decode(pair + 1, head, q0);
-            w.fetch(buf ^ 1, head, q0);
-        }
+        const int buf = pair & 1;
+        const typename W::Pair now = next;
+        next = w.decode(pair + 1);
+        w.aim(buf ^ 1, next);
         bool whole;
-        if (!w.touches(q, whole)) continue;
+        if (!w.touches(now, whole)) {
+            w.issue_all();
+            continue;
+        }
         bf16x8 pf[2], dsf[2];
         uint32_t allowed;
-        w.gradient(pf, dsf, allowed, buf, q, whole, here(row_lane_), kf);
+        w.gradient(pf, dsf, allowed, buf, now.q0, whole, here(row_lane_), kf, [&](int st) { w.issue(st); });
         const int cols_lane = here(cols_lane_);
 #pragma unroll
         for (int db = 0; db < W::kDims; ++db)
@@ -804,10 +798,10 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_kernel
                 dk[db] = mfma(T::cols(w.queries(buf), cols_lane, db, u), dsf[u], dk[db]);
             }
     }
-    copies_landed();   // the values, where the share is empty: no copy may outlive the workgroup
     bool fine = true;
 #pragma unroll
     for (int db = 0; db < W::kDims; ++db) fine &= all_finite(dk[db]) && all_finite(dv[db]);
+    copies_landed();
     const bool again = __syncthreads_or(!fine);
     if (w.tid == 0) a.flags[blockIdx.x] = again;
     if (!again) {
@@ -824,7 +818,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_carefu
     typedef typename W::T T;
     if (a.flags[blockIdx.x] == 0) return;
     __shared__ __attribute__((aligned(16))) char lds[W::kLdsBytes];
-    const W w(a, lds);
+    W w(a, lds);
     bf16x8 kf[W::kSteps];
     w.load_keys(kf);
 #pragma nounroll
@@ -832,15 +826,15 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_carefu
         f32x16 one_k = zero16(), one_v = zero16();
 #pragma nounroll
         for (int pair = w.first_pair; pair < w.last_pair; ++pair) {
-            int head, q0;
-            w.decode(pair, head, q0);
-            w.fetch(0, head, q0);
+            const typename W::Pair now = w.decode(pair);
+            w.aim(0, now);
+            w.issue_all();
             copies_landed();
             bool whole;
-            if (w.touches(q0, whole)) {
+            if (w.touches(now, whole)) {
                 bf16x8 pf[2], dsf[2];
                 uint32_t allowed;
-                w.gradient(pf, dsf, allowed, 0, q0, false, T::row_lane(w.lane), kf);
+                w.gradient(pf, dsf, allowed, 0, now.q0, false, T::row_lane(w.lane), kf, [](int) {});
                 f32x16 in;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) in[i] = (allowed >> i & 1) ? 1.f : 0.f;
@@ -854,7 +848,6 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_carefu
         }
         w.put(db, one_k, one_v);
     }
-    copies_landed();   // the values, where the share is empty
 }
 
 // Adds the splits' dk and dv in their order and rounds once.  A lane takes four values.

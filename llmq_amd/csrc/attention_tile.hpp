@@ -25,8 +25,7 @@ typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
 
-// Source of the rows beyond the sequence: zeros, so that they add nothing and no value of a neighbouring sequence, NaN or
-// infinite, reaches a product.
+// Source of a fragment's dimensions beyond head_dim.
 __device__ const uint32_t __attribute__((aligned(16))) attention_zeros[4] = {0, 0, 0, 0};
 
 __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
@@ -56,11 +55,12 @@ __device__ __forceinline__ bf16x8 operand(const f32x16& x, int u) {
     return __builtin_bit_cast(bf16x8, w);
 }
 
-// Copies from global memory straight into LDS, 16 or 4 bytes a lane, lane i to `lds` (one address for the wave) + 16 i or 4 i;
-// source: 32-bit lane offset from a scalar base, or one address a lane.  Inline assembly, because the compiler puts a wait for
-// every outstanding copy in front of the next LDS read, whatever it reads; what a kernel reads of a copy it reads behind
-// copies_landed().  The s_nop covers, whoever wrote the scalars, the five wait states between a vector instruction that writes a
-// scalar register and a memory instruction that reads it, and the one behind a write of M0.
+// Copies from global memory straight into LDS, 16 or 4 bytes a lane, lane i to `lds` (one address for the wave) + 16 i or 4 i, by
+// the lanes of `lanes`; source: a 32-bit lane offset from a scalar base, or one address a lane.  Inline assembly, because the
+// compiler puts a wait for every outstanding copy in front of the next LDS read, whatever it reads; what a kernel reads of a copy
+// it reads behind copies_landed().  All lanes are active where a kernel calls these (its branches are the wave's).  The s_nop
+// covers, whoever wrote the scalars, the five wait states between a vector instruction that writes a scalar register and a memory
+// instruction that reads it, and the one behind a write of M0.
 __device__ __forceinline__ uint32_t lds_address(const char* p) {
     return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p);
 }
@@ -69,18 +69,18 @@ __device__ __forceinline__ uint32_t to_m0(uint32_t lds) {
     asm volatile("s_mov_b32 %0, %1" : "={m0}"(m0) : "s"(lds));
     return m0;
 }
-__device__ __forceinline__ void copy16(uint32_t lds, uint32_t offset, const char* wave_base) {
-    // (readfirstlane gives a signed int: its low word must not be sign-extended into the high one)
-    const uint64_t p = reinterpret_cast<uint64_t>(wave_base);
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)p), hi = __builtin_amdgcn_readfirstlane((uint32_t)(p >> 32));
-    const uint64_t base = (uint64_t)hi << 32 | lo;
-    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(offset), "s"(base), "{m0}"(to_m0(lds)) : "memory");
+// (readfirstlane gives a signed int: its low word must not be sign-extended into the high one)
+__device__ __forceinline__ uint64_t scalar(uint64_t x) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+    return (uint64_t)hi << 32 | lo;
 }
-__device__ __forceinline__ void copy16(uint32_t lds, const char* p) {
-    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(p), "{m0}"(to_m0(lds)) : "memory");
+__device__ __forceinline__ void copy16(uint32_t lds, uint32_t offset, const char* base, uint64_t lanes) {
+    asm volatile("s_mov_b64 exec, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1\n\ts_mov_b64 exec, -1"
+                 : : "v"(offset), "s"(scalar(reinterpret_cast<uint64_t>(base))), "s"(lanes), "{m0}"(to_m0(lds)) : "memory");
 }
-__device__ __forceinline__ void copy4(uint32_t lds, const void* p) {
-    asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, off" : : "v"(p), "{m0}"(to_m0(lds)) : "memory");
+__device__ __forceinline__ void copy4(uint32_t lds, const void* p, uint64_t lanes) {
+    asm volatile("s_mov_b64 exec, %1\n\ts_nop 4\n\tglobal_load_lds_dword %0, off\n\ts_mov_b64 exec, -1"
+                 : : "v"(p), "s"(lanes), "{m0}"(to_m0(lds)) : "memory");
 }
 // Waits for this wave's copies and for the other waves' to be waited for.
 __device__ __forceinline__ void copies_landed() {
@@ -100,45 +100,9 @@ struct Tile {
         return HDP == 128 ? ((row & 3) << 2 | ((row >> 2) & 3)) : ((row & 2) << 1 | ((row >> 2) & 3));
     }
 
-    // Direct-to-LDS copies land linearly (lane i at 16 i), so the swizzle picks the source chunk.  Lanes whose chunk lies beyond
-    // head_dim copy nothing: their places are cleared once (`clear`) and stay zero.
-    struct Source {
-        uint32_t offset;    // of this lane's chunk from the tile's first row
-        int row;            // its row
-        bool pad;           // a chunk beyond head_dim
-    };
-    template <int THREADS>
-    static __device__ __forceinline__ Source source(int tid, int64_t stride_bytes, int head_dim) {
-        const int row = tid / kChunks, chunk = (tid % kChunks) ^ swizzle(row);
-        Source s;
-        s.row = row;
-        s.pad = chunk * 8 >= head_dim;
-        s.offset = (uint32_t)(row * stride_bytes) + chunk * 16;
-        return s;
-    }
     template <int THREADS>
     static __device__ __forceinline__ void clear(char* lds, int tid) {
         for (int i = tid * 16; i < kBytes; i += THREADS * 16) *reinterpret_cast<uint4*>(lds + i) = make_uint4(0, 0, 0, 0);
-    }
-    // rows row0 .. row0 + ROWS - 1 of the sequence whose row 0 is at `head`, zeros from row `limit` on
-    template <int THREADS>
-    static __device__ __forceinline__ void stage(char* lds, const uint16_t* head, const Source& s, int tid, int64_t stride_bytes, int row0, int limit) {
-        constexpr int kStep = THREADS / kChunks;   // rows per copy instruction of the workgroup, a multiple of the swizzle's period
-        static_assert(kStep % 16 == 0 && ROWS % kStep == 0, "the swizzle must repeat from copy to copy");
-        const char* base = reinterpret_cast<const char*>(head) + (int64_t)row0 * stride_bytes;
-        const uint32_t dst = lds_address(lds + (tid / kWave) * (kWave * 16));
-        if (s.pad) return;
-        if (row0 + ROWS <= limit) {
-#pragma unroll
-            for (int i = 0; i < ROWS / kStep; ++i) copy16(dst + i * THREADS * 16, s.offset, base + (int64_t)(i * kStep) * stride_bytes);
-        } else {
-#pragma unroll
-            for (int i = 0; i < ROWS / kStep; ++i) {
-                const char* p = base + (int64_t)(i * kStep) * stride_bytes + s.offset;
-                if (row0 + s.row + i * kStep >= limit) p = reinterpret_cast<const char*>(attention_zeros);
-                copy16(dst + i * THREADS * 16, p);
-            }
-        }
     }
 
     // Left-hand operand, rows of the tile by head dimension: lane -> row 32 rb + l % 32, chunk 2 step + l / 32.
@@ -162,6 +126,35 @@ struct Tile {
         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(lds + (at ^ kFlip) + (u * 16 + 8) * kRowBytes));
         const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
         return __builtin_bit_cast(bf16x8, (u32x4){a.x, a.y, b.x, b.y});
+    }
+};
+
+// A lane's part in copying tiles of ROWS rows by THREADS threads, in kCopies copies.  Copies land linearly in LDS, so the swizzle
+// picks the source chunk.  Lanes whose chunk lies beyond head_dim copy nothing: their places are cleared once and stay zero.  Rows
+// from `limit` on repeat the last one: they are masked.
+template <int HDP, int ROWS, int THREADS>
+struct TileCopy {
+    typedef Tile<HDP, ROWS> T;
+    static constexpr int kStep = THREADS / T::kChunks, kCopies = ROWS / kStep;   // rows of a copy
+    static_assert(kStep % 16 == 0 && ROWS % kStep == 0, "the swizzle must repeat from copy to copy");
+    int row;
+    uint32_t chunk;    // bytes into the row
+    uint64_t lanes;
+
+    __device__ __forceinline__ TileCopy(int tid, int head_dim) {
+        row = tid / T::kChunks;
+        const int c = (tid % T::kChunks) ^ T::swizzle(row);
+        chunk = c * 16;
+        lanes = scalar(__ballot(c * 8 < head_dim));
+    }
+    // offsets from the tile's first row, row0
+    __device__ __forceinline__ void offsets(uint32_t (&ofs)[kCopies], int64_t stride_bytes, int row0, int limit) const {
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) ofs[i] = (uint32_t)min(row + i * kStep, limit - 1 - row0) * (uint32_t)stride_bytes + chunk;
+    }
+    // one copy; lds: address of the tile plus the wave's share, 1024 bytes for each of its number
+    __device__ __forceinline__ void copy(int i, uint32_t lds, const uint32_t (&ofs)[kCopies], const char* base) const {
+        copy16(lds + i * THREADS * 16, ofs[i], base, lanes);
     }
 };
 
