@@ -546,8 +546,10 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_q_kernel(
 
 // ---- backward: keys and values -------------------------------------------------------------------------------------------
 // A wave owns 32 keys (columns) and walks the queries (rows), 32 at a time, of every head of the group: s = Q k, dp = dout v,
-// dv = dout^T p, dk = Q^T ds.  A workgroup takes one of `splits` equal shares of the (head, query tile) pairs of its keys.  The
-// accumulators fill half of the 256 registers that two waves per SIMD leave, the keys an eighth; the values stay in LDS.
+// dv = dout^T p, dk = Q^T ds.  A workgroup takes one of `splits` equal shares of the (query tile, head) pairs of its keys, from the
+// last query back, the heads of a tile one after the other: the workgroups of a group of heads then read the same tiles at about
+// the same time, and one die's L2 serves them all.  The accumulators fill half of the 256 registers that two waves per SIMD leave,
+// the keys an eighth; the values stay in LDS.
 constexpr int kQueries = 32;
 
 template <int HDP, int WAVES>
@@ -565,15 +567,17 @@ struct KeyBlock {
     char* lds;
     uint32_t lds_at;
     int tid, lane, wave, b, kvh, split, k0, k1, ng;
-    int t_lo, tiles, first_pair, last_pair;
+    int first_pair, last_pair;
     int64_t token, stride, ostride;
     const uint16_t* base;
     int key_;
     Copy copy;
-    uint32_t qofs[Copy::kCopies], gofs[Copy::kCopies];
-    const char *qnext, *gnext;   // of the tile that is being copied
-    const float* snext;
-    uint32_t to, sto;            // and where
+    uint32_t qofs[Copy::kCopies], gofs[Copy::kCopies], sofs;
+    int head_, tile_;                         // of the pair that is being copied
+    bool clamped;
+    const char *qnext, *gnext, *snext;        // its sources
+    int64_t shead;                            // from one head's statistics to the next
+    uint32_t to, sto;                         // and destinations
     uint64_t slanes;
 
     __device__ __forceinline__ KeyBlock(const AttentionArgs& args, char* lds_) : a(args), lds(lds_), copy(threadIdx.x, args.head_dim) {
@@ -593,10 +597,9 @@ struct KeyBlock {
             V::template clear<kThreads>(lds + kValues, tid);
             __syncthreads();
         }
-        // the query tiles that look at any of the workgroup's keys lie in [t_lo, t_lo + tiles)
+        // the query tiles that look at any of the workgroup's keys lie in [t_lo, t_hi]
         ng = (a.T + 31) / 32;
-        t_lo = kb0 / kQueries;
-        int t_hi = ng - 1;
+        int t_lo = kb0 / kQueries, t_hi = ng - 1;
         if (a.first_key) {
             int l = INT_MAX, h = -1;
             for (int g = t_lo + tid; g < ng; g += kThreads)
@@ -608,11 +611,17 @@ struct KeyBlock {
             t_lo = l <= h ? l : 1;
             t_hi = l <= h ? h : 0;
         }
-        tiles = max(t_hi - t_lo + 1, 0);
-        const int64_t pairs = (int64_t)tiles * a.G;
+        const int64_t pairs = (int64_t)max(t_hi - t_lo + 1, 0) * a.G;
         first_pair = (int)(pairs * split / a.splits), last_pair = (int)(pairs * (split + 1) / a.splits);
-        copy.offsets(qofs, stride, 0, INT_MAX);
-        copy.offsets(gofs, ostride, 0, INT_MAX);
+        tile_ = t_hi - first_pair / a.G, head_ = first_pair % a.G;
+        clamped = true;
+        const int64_t head = kvh * a.G + head_, q0 = (int64_t)tile_ * kQueries, row = ((int64_t)b * a.Nq + head) * a.T;
+        qnext = reinterpret_cast<const char*>(base + head * a.head_dim) + q0 * stride;
+        gnext = reinterpret_cast<const char*>(a.dout + ((int64_t)b * a.T * a.Nq + head) * a.head_dim) + q0 * ostride;
+        snext = wave == 0 ? reinterpret_cast<const char*>(a.lse2 + row + q0)
+                : wave == 1 || !a.first_key ? reinterpret_cast<const char*>(a.delta + row + q0)
+                                            : reinterpret_cast<const char*>(a.first_key + (int64_t)b * a.T + q0);
+        shead = wave == 2 && a.first_key ? 0 : (int64_t)a.T * 4;
         slanes = wave < 3 ? 0xFFFFFFFFull : 0;
         if (first_pair < last_pair) {
             typedef TileCopy<HDP, kBlock, kThreads> ValueCopy;
@@ -630,40 +639,46 @@ struct KeyBlock {
     __device__ __forceinline__ char* queries(int buf) const { return lds + buf * T::kBytes; }
     __device__ __forceinline__ char* gradients(int buf) const { return lds + (2 + buf) * T::kBytes; }
     __device__ __forceinline__ const char* statistics(int buf, int which) const { return lds + kStats + (buf * 3 + which) * kQueries * 4; }
-    // Head and first query of a pair (of the last one if it is behind it) and what its queries may look at.
+    // The first query of a pair and what its queries may look at.
     struct Pair {
-        int head, q0;
+        int q0;
         int2 group;
     };
-    __device__ __forceinline__ Pair decode(int pair) const {
-        pair = min(pair, last_pair - 1);
-        const int h = pair / tiles;
+    __device__ __forceinline__ Pair aimed() const {
         Pair p;
-        p.head = kvh * a.G + h, p.q0 = (t_lo + pair - h * tiles) * kQueries;
+        p.q0 = tile_ * kQueries;
         p.group = make_int2(0, 0);
-        if (a.first_key) p.group = a.groups[(int64_t)b * ng + (p.q0 >> 5)];
+        if (a.first_key) p.group = a.groups[(int64_t)b * ng + tile_];
         return p;
     }
-    __device__ __forceinline__ void aim(int buf, const Pair& p) {
-        if (p.q0 + kQueries > a.T || qnext_clamped) {   // the last tile of the sequence, and the one behind it
-            copy.offsets(qofs, stride, p.q0, a.T);
-            copy.offsets(gofs, ostride, p.q0, a.T);
-            qnext_clamped = p.q0 + kQueries > a.T;
+    // copies of the pair into `buf`, one by one
+    __device__ __forceinline__ void aim(int buf) {
+        const int q0 = tile_ * kQueries;
+        if (clamped) {   // the last tile of the sequence comes first
+            copy.offsets(qofs, stride, q0, a.T);
+            copy.offsets(gofs, ostride, q0, a.T);
+            sofs = min(lane & 31, a.T - 1 - q0) * 4;
+            clamped = q0 + kQueries > a.T;
         }
-        qnext = reinterpret_cast<const char*>(base + (int64_t)p.head * a.head_dim) + p.q0 * stride;
-        gnext = reinterpret_cast<const char*>(a.dout + ((int64_t)b * a.T * a.Nq + p.head) * a.head_dim) + p.q0 * ostride;
-        const int q = min(p.q0 + (lane & 31), a.T - 1);
-        const int64_t row = ((int64_t)b * a.Nq + p.head) * a.T;
-        snext = wave == 0 ? a.lse2 + row + q : wave == 1 || !a.first_key ? a.delta + row + q
-                                                                         : reinterpret_cast<const float*>(a.first_key) + (int64_t)b * a.T + q;
         to = lds_at + buf * T::kBytes;
         sto = lds_at - wave * 1024 + kStats + (buf * 3 + min(wave, 2)) * kQueries * 4;
     }
-    bool qnext_clamped = false;
+    // on to the next pair; behind the last one it stays
+    __device__ __forceinline__ void advance(bool more) {
+        if (!more) return;
+        const int64_t dim = a.head_dim * 2;
+        if (++head_ < a.G) {
+            qnext += dim, gnext += dim, snext += shead;
+        } else {
+            head_ = 0, --tile_;
+            const int64_t back = (a.G - 1) * dim;
+            qnext -= back + kQueries * stride, gnext -= back + kQueries * ostride, snext -= (a.G - 1) * shead + kQueries * 4;
+        }
+    }
     __device__ __forceinline__ void issue(int i) const {
         if (i < Copy::kCopies) copy.copy(i, to, qofs, qnext);
         else if (i < 2 * Copy::kCopies) copy.copy(i - Copy::kCopies, to + 2 * T::kBytes, gofs, gnext);
-        else if (i < kCopies) copy4(sto, snext, slanes);
+        else if (i < kCopies) copy4(sto, sofs, snext, slanes);
     }
     __device__ __forceinline__ void issue_all() const {
 #pragma unroll
@@ -770,8 +785,8 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_kernel
     for (int db = 0; db < W::kDims; ++db) dk[db] = zero16(), dv[db] = zero16();
     typename W::Pair next;
     if (w.first_pair < w.last_pair) {
-        next = w.decode(w.first_pair);
-        w.aim(w.first_pair & 1, next);
+        next = w.aimed();
+        w.aim(w.first_pair & 1);
         w.issue_all();
     }
 #pragma nounroll
@@ -779,8 +794,9 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_kernel
         copies_landed();
         const int buf = pair & 1;
         const typename W::Pair now = next;
-        next = w.decode(pair + 1);
-        w.aim(buf ^ 1, next);
+        w.advance(pair + 1 < w.last_pair);
+        next = w.aimed();
+        w.aim(buf ^ 1);
         bool whole;
         if (!w.touches(now, whole)) {
             w.issue_all();
@@ -818,16 +834,17 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_carefu
     typedef typename W::T T;
     if (a.flags[blockIdx.x] == 0) return;
     __shared__ __attribute__((aligned(16))) char lds[W::kLdsBytes];
-    W w(a, lds);
+    const W start(a, lds);
     bf16x8 kf[W::kSteps];
-    w.load_keys(kf);
+    start.load_keys(kf);
 #pragma nounroll
     for (int db = 0; db < W::kDims; ++db) {
         f32x16 one_k = zero16(), one_v = zero16();
+        W w = start;
 #pragma nounroll
         for (int pair = w.first_pair; pair < w.last_pair; ++pair) {
-            const typename W::Pair now = w.decode(pair);
-            w.aim(0, now);
+            const typename W::Pair now = w.aimed();
+            w.aim(0);
             w.issue_all();
             copies_landed();
             bool whole;
@@ -845,6 +862,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_carefu
                 }
             }
             __syncthreads();
+            w.advance(pair + 1 < w.last_pair);
         }
         w.put(db, one_k, one_v);
     }

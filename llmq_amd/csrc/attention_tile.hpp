@@ -56,7 +56,7 @@ __device__ __forceinline__ bf16x8 operand(const f32x16& x, int u) {
 }
 
 // Copies from global memory straight into LDS, 16 or 4 bytes a lane, lane i to `lds` (one address for the wave) + 16 i or 4 i, by
-// the lanes of `lanes`; source: a 32-bit lane offset from a scalar base, or one address a lane.  Inline assembly, because the
+// the lanes of `lanes`; source: a 32-bit lane offset from a scalar base.  Inline assembly, because the
 // compiler puts a wait for every outstanding copy in front of the next LDS read, whatever it reads; what a kernel reads of a copy
 // it reads behind copies_landed().  All lanes are active where a kernel calls these (its branches are the wave's).  The s_nop
 // covers, whoever wrote the scalars, the five wait states between a vector instruction that writes a scalar register and a memory
@@ -78,9 +78,9 @@ __device__ __forceinline__ void copy16(uint32_t lds, uint32_t offset, const char
     asm volatile("s_mov_b64 exec, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1\n\ts_mov_b64 exec, -1"
                  : : "v"(offset), "s"(scalar(reinterpret_cast<uint64_t>(base))), "s"(lanes), "{m0}"(to_m0(lds)) : "memory");
 }
-__device__ __forceinline__ void copy4(uint32_t lds, const void* p, uint64_t lanes) {
-    asm volatile("s_mov_b64 exec, %1\n\ts_nop 4\n\tglobal_load_lds_dword %0, off\n\ts_mov_b64 exec, -1"
-                 : : "v"(p), "s"(lanes), "{m0}"(to_m0(lds)) : "memory");
+__device__ __forceinline__ void copy4(uint32_t lds, uint32_t offset, const char* base, uint64_t lanes) {
+    asm volatile("s_mov_b64 exec, %2\n\ts_nop 4\n\tglobal_load_lds_dword %0, %1\n\ts_mov_b64 exec, -1"
+                 : : "v"(offset), "s"(scalar(reinterpret_cast<uint64_t>(base))), "s"(lanes), "{m0}"(to_m0(lds)) : "memory");
 }
 // Waits for this wave's copies and for the other waves' to be waited for.
 __device__ __forceinline__ void copies_landed() {
