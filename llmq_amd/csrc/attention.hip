@@ -546,9 +546,9 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_q_kernel(
 
 // ---- backward: keys and values -------------------------------------------------------------------------------------------
 // A wave owns 32 keys (columns) and walks the queries (rows), 32 at a time, of every head of the group: s = Q k, dp = dout v,
-// dv = dout^T p, dk = Q^T ds.  A workgroup takes one of `splits` equal shares of the (query tile, head) pairs of its keys, from the
-// last query back, the heads of a tile one after the other: the workgroups of a group of heads then read the same tiles at about
-// the same time, and one die's L2 serves them all.  The accumulators fill half of the 256 registers that two waves per SIMD leave,
+// dv = dout^T p, dk = Q^T ds.  The (query tile, head) pairs are walked from the last query back, the heads of a tile one after
+// the other, and a workgroup takes every `splits`-th: the workgroups of a group of heads then read the same tiles at about the
+// same time, and one die's L2 serves them all.  The accumulators fill half of the 256 registers that two waves per SIMD leave,
 // the keys an eighth; the values stay in LDS.
 constexpr int kQueries = 32;
 
@@ -567,7 +567,7 @@ struct KeyBlock {
     char* lds;
     uint32_t lds_at;
     int tid, lane, wave, b, kvh, split, k0, k1, ng;
-    int first_pair, last_pair;
+    int turns;                                // pairs of the workgroup
     int64_t token, stride, ostride;
     const uint16_t* base;
     int key_;
@@ -576,7 +576,8 @@ struct KeyBlock {
     int head_, tile_;                         // of the pair that is being copied
     bool clamped;
     const char *qnext, *gnext, *snext;        // its sources
-    int64_t shead;                            // from one head's statistics to the next
+    int head_step, tile_step;                 // `splits` in heads and tiles
+    int64_t qstep, gstep, sstep, qcarry, gcarry, scarry;   // what that moves the sources, and a carry from the heads besides
     uint32_t to, sto;                         // and destinations
     uint64_t slanes;
 
@@ -612,8 +613,9 @@ struct KeyBlock {
             t_hi = l <= h ? h : 0;
         }
         const int64_t pairs = (int64_t)max(t_hi - t_lo + 1, 0) * a.G;
-        first_pair = (int)(pairs * split / a.splits), last_pair = (int)(pairs * (split + 1) / a.splits);
-        tile_ = t_hi - first_pair / a.G, head_ = first_pair % a.G;
+        turns = pairs > split ? (int)((pairs - split + a.splits - 1) / a.splits) : 0;
+        tile_ = t_hi - split / a.G, head_ = split % a.G;
+        head_step = a.splits % a.G, tile_step = a.splits / a.G;
         clamped = true;
         const int64_t head = kvh * a.G + head_, q0 = (int64_t)tile_ * kQueries, row = ((int64_t)b * a.Nq + head) * a.T;
         qnext = reinterpret_cast<const char*>(base + head * a.head_dim) + q0 * stride;
@@ -621,9 +623,12 @@ struct KeyBlock {
         snext = wave == 0 ? reinterpret_cast<const char*>(a.lse2 + row + q0)
                 : wave == 1 || !a.first_key ? reinterpret_cast<const char*>(a.delta + row + q0)
                                             : reinterpret_cast<const char*>(a.first_key + (int64_t)b * a.T + q0);
-        shead = wave == 2 && a.first_key ? 0 : (int64_t)a.T * 4;
+        const int64_t dim = a.head_dim * 2, shead = wave == 2 && a.first_key ? 0 : (int64_t)a.T * 4;
+        qcarry = -a.G * dim - kQueries * stride, gcarry = -a.G * dim - kQueries * ostride, scarry = -a.G * shead - kQueries * 4;
+        qstep = head_step * dim - tile_step * kQueries * stride, gstep = head_step * dim - tile_step * kQueries * ostride;
+        sstep = head_step * shead - tile_step * kQueries * 4;
         slanes = wave < 3 ? 0xFFFFFFFFull : 0;
-        if (first_pair < last_pair) {
+        if (turns > 0) {
             typedef TileCopy<HDP, kBlock, kThreads> ValueCopy;
             const ValueCopy vcopy(tid, a.head_dim);
             uint32_t vofs[ValueCopy::kCopies];
@@ -666,13 +671,11 @@ struct KeyBlock {
     // on to the next pair; behind the last one it stays
     __device__ __forceinline__ void advance(bool more) {
         if (!more) return;
-        const int64_t dim = a.head_dim * 2;
-        if (++head_ < a.G) {
-            qnext += dim, gnext += dim, snext += shead;
-        } else {
-            head_ = 0, --tile_;
-            const int64_t back = (a.G - 1) * dim;
-            qnext -= back + kQueries * stride, gnext -= back + kQueries * ostride, snext -= (a.G - 1) * shead + kQueries * 4;
+        head_ += head_step, tile_ -= tile_step;
+        qnext += qstep, gnext += gstep, snext += sstep;
+        if (head_ >= a.G) {
+            head_ -= a.G, --tile_;
+            qnext += qcarry, gnext += gcarry, snext += scarry;
         }
     }
     __device__ __forceinline__ void issue(int i) const {
@@ -784,17 +787,17 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_kernel
 #pragma unroll
     for (int db = 0; db < W::kDims; ++db) dk[db] = zero16(), dv[db] = zero16();
     typename W::Pair next;
-    if (w.first_pair < w.last_pair) {
+    if (w.turns > 0) {
         next = w.aimed();
-        w.aim(w.first_pair & 1);
+        w.aim(0);
         w.issue_all();
     }
 #pragma nounroll
-    for (int pair = w.first_pair; pair < w.last_pair; ++pair) {
+    for (int turn = 0; turn < w.turns; ++turn) {
         copies_landed();
-        const int buf = pair & 1;
+        const int buf = turn & 1;
         const typename W::Pair now = next;
-        w.advance(pair + 1 < w.last_pair);
+        w.advance(turn + 1 < w.turns);
         next = w.aimed();
         w.aim(buf ^ 1);
         bool whole;
@@ -842,7 +845,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_carefu
         f32x16 one_k = zero16(), one_v = zero16();
         W w = start;
 #pragma nounroll
-        for (int pair = w.first_pair; pair < w.last_pair; ++pair) {
+        for (int turn = 0; turn < w.turns; ++turn) {
             const typename W::Pair now = w.aimed();
             w.aim(0);
             w.issue_all();
@@ -862,7 +865,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_carefu
                 }
             }
             __syncthreads();
-            w.advance(pair + 1 < w.last_pair);
+            w.advance(turn + 1 < w.turns);
         }
         w.put(db, one_k, one_v);
     }
@@ -900,7 +903,12 @@ static int check_shape(const char* what, int B, int T, int Nq, int Nkv, int head
     return LLMQ_OK;
 }
 
-// Shares of the walk over the queries: enough workgroups for two per compute unit, each with some tiles of work.
+// Keys of a workgroup of the keys' kernel: as many waves as copy a tile of 32 queries with one load a thread.  Above 64 dimensions
+// eight, which read the queries half as often as four: 1 x 8192 1925 -> 1640 us, documents 283 -> 214, but 8 x 1024 331 -> 340.
+static int kv_block(int head_dim) { return head_dim > 64 ? 256 : 128; }
+
+// Shares of the walk over the queries: enough workgroups for two per compute unit, each with some pairs of work (one per unit:
+// 1 x 8192 2180 us, 8 x 1024 370; three: 1710 and 369).
 static int kv_splits(int B, int T, int Nq, int Nkv, int keys) {
     const int64_t blocks = (int64_t)B * Nkv * ((T + keys - 1) / keys);
     const int64_t pairs = (int64_t)((T + kQueries - 1) / kQueries) * (Nq / Nkv);
@@ -908,8 +916,6 @@ static int kv_splits(int B, int T, int Nq, int Nkv, int keys) {
     if (s > (pairs + 3) / 4) s = (pairs + 3) / 4;
     return (int)(s < 1 ? 1 : s > 16 ? 16 : s);
 }
-
-constexpr int kKvBlock = 128;
 
 struct BackwardPlan {
     int splits;
@@ -919,9 +925,10 @@ struct BackwardPlan {
 static BackwardPlan backward_plan(int B, int T, int Nq, int Nkv, int head_dim) {
     auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
     BackwardPlan p;
-    p.splits = kv_splits(B, T, Nq, Nkv, kKvBlock);
+    const int keys = kv_block(head_dim);
+    p.splits = kv_splits(B, T, Nq, Nkv, keys);
     p.stats = up((int64_t)B * Nq * T * 4);
-    p.blocks = (int64_t)((T + kKvBlock - 1) / kKvBlock) * B * Nkv * p.splits;
+    p.blocks = (int64_t)((T + keys - 1) / keys) * B * Nkv * p.splits;
     p.flags = up(p.blocks * 4);
     p.groups = up((int64_t)B * ((T + 31) / 32) * 8);
     p.partial = p.splits > 1 ? up((int64_t)p.splits * B * T * Nkv * 2 * head_dim * 4) : 0;
@@ -1005,9 +1012,9 @@ extern "C" int llmq_attention_backward_bf16(uint16_t* dqkv, const uint16_t* dout
     if (head_dim > 64) {
         launch(attention_backward_q_kernel<128, 4>, q_blocks, 256);
         LLMQ_HIP_TRY(hipGetLastError());
-        launch(attention_backward_kv_kernel<128, 4>, p.blocks, 256);
+        launch(attention_backward_kv_kernel<128, 8>, p.blocks, 512);
         LLMQ_HIP_TRY(hipGetLastError());
-        launch(attention_backward_kv_careful_kernel<128, 4>, p.blocks, 256);
+        launch(attention_backward_kv_careful_kernel<128, 8>, p.blocks, 512);
     } else {
         launch(attention_backward_q_kernel<64, 4>, q_blocks, 256);
         LLMQ_HIP_TRY(hipGetLastError());

@@ -76,11 +76,11 @@ __device__ __forceinline__ uint64_t scalar(uint64_t x) {
 }
 __device__ __forceinline__ void copy16(uint32_t lds, uint32_t offset, const char* base, uint64_t lanes) {
     asm volatile("s_mov_b64 exec, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1\n\ts_mov_b64 exec, -1"
-                 : : "v"(offset), "s"(scalar(reinterpret_cast<uint64_t>(base))), "s"(lanes), "{m0}"(to_m0(lds)) : "memory");
+                 : : "v"(offset), "s"(scalar(reinterpret_cast<uint64_t>(base))), "s"(scalar(lanes)), "{m0}"(to_m0(lds)) : "memory");
 }
 __device__ __forceinline__ void copy4(uint32_t lds, uint32_t offset, const char* base, uint64_t lanes) {
     asm volatile("s_mov_b64 exec, %2\n\ts_nop 4\n\tglobal_load_lds_dword %0, %1\n\ts_mov_b64 exec, -1"
-                 : : "v"(offset), "s"(scalar(reinterpret_cast<uint64_t>(base))), "s"(lanes), "{m0}"(to_m0(lds)) : "memory");
+                 : : "v"(offset), "s"(scalar(reinterpret_cast<uint64_t>(base))), "s"(scalar(lanes)), "{m0}"(to_m0(lds)) : "memory");
 }
 // Waits for this wave's copies and for the other waves' to be waited for.
 __device__ __forceinline__ void copies_landed() {
