@@ -425,8 +425,6 @@ int llmq_adamw_update_f32(float* params, const float* grads, float* m, float* v,
  * an allowed place is not finite, the outputs it enters are not finite either (NaN, also where the formula gives an infinity).
  * abs_max_or_null: reset, then max |out|, bit-identical to llmq_abs_max_bf16(out).  head_dim: a multiple of 8 up to 128;
  * softmax_scale > 0.  out must not be qkv.
- * Replaces: attention_forward_cudnn(nv_bfloat16* out, float* stats, const nv_bfloat16* inp, ...)  (cuDNN-frontend graphs,
- *           src/kernels/cudnn_att.cpp) and the reference's own kernel, src/kernels/attention.cu:20 (head_dim 64 / 128).
  */
 int llmq_attention_forward_bf16(uint16_t* out, float* lse, const uint16_t* qkv, const int* first_key_or_null,
                                 float* abs_max_or_null, float softmax_scale, int B, int T, int Nq, int Nkv, int head_dim,
@@ -440,8 +438,6 @@ int llmq_attention_forward_bf16(uint16_t* out, float* lse, const uint16_t* qkv, 
  * fixed order (deterministic), every element of dqkv is written.  Masked places as in the forward pass.
  * scratch: at least llmq_attention_backward_scratch_bytes(B, T, Nq, Nkv, head_dim) bytes, 16-byte aligned, overwritten by every
  * call; calls that share it must be stream ordered.  dqkv must be a tensor of its own.
- * Replaces: attention_backward_cudnn(nv_bfloat16* dqkvr, const float* stats, const nv_bfloat16* out, const nv_bfloat16* dout,
- *           const nv_bfloat16* qkvr, ...)  (src/kernels/cudnn_att.cpp) and src/kernels/attention.cu:152.
  */
 int64_t llmq_attention_backward_scratch_bytes(int B, int T, int Nq, int Nkv, int head_dim);
 int llmq_attention_backward_bf16(uint16_t* dqkv, const uint16_t* dout, const uint16_t* out, const float* lse,
@@ -449,7 +445,7 @@ int llmq_attention_backward_bf16(uint16_t* dqkv, const uint16_t* dout, const uin
                                  float softmax_scale, int B, int T, int Nq, int Nkv, int head_dim, void* stream);
 
 /*
- * Log probabilities of given tokens.  logits: N rows of V values, P >= V elements apart (padded vocabulary: columns V .. P-1
+ * Log probabilities of given tokens.  logits: N < 2^24 rows of V values, P >= V elements apart (padded vocabulary: columns V .. P-1
  * are not looked at); targets: int32 [N].  Per row:
  *     lse = ln sum_v exp(x_v);  logp = x_t - lse (0 where t is not in [0, V): an ignored row);
  *     entropy_or_null = lse - sum_v p_v x_v;
@@ -460,7 +456,6 @@ int llmq_attention_backward_bf16(uint16_t* dqkv, const uint16_t* dout, const uin
  * row that holds NaN or +inf has NaN for lse, logp and entropy.  All sums fp32 in a fixed order (deterministic).
  * scratch: at least llmq_token_logprobs_scratch_bytes(N, V, k) bytes (0 for many rows: may be NULL), 16-byte aligned,
  * overwritten by every call; calls that share it must be stream ordered.  logits 16-byte aligned, any P.
- * Counterpart in the reference: the loss half of fused_classifier, src/kernels/fused_classifier.cu:92,246 (one target a row).
  */
 int64_t llmq_token_logprobs_scratch_bytes(int64_t N, int V, int k);
 int llmq_token_logprobs_bf16(float* logp, float* entropy_or_null, float* lse, float* top_logp, int* top_ids,
@@ -478,7 +473,6 @@ int llmq_token_logprobs_f32(float* logp, float* entropy_or_null, float* lse, flo
  * whose lse is -inf.
  * dlogits may be logits (in place).  abs_max_or_null: reset, then max |dlogits| over all columns, bit-identical to llmq_abs_max
  * of the tensor.  The loss -mean logp has dlogp = -1 / N.
- * Counterpart in the reference: the gradient half of fused_classifier, src/kernels/fused_classifier.cu:92.
  */
 int llmq_token_logprobs_backward_bf16(uint16_t* dlogits, const float* dlogp, const float* dentropy_or_null,
                                       const uint16_t* logits, const int* targets, const float* lse, const float* entropy_or_null,

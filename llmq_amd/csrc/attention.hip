@@ -7,7 +7,6 @@
 //     dq_t = scale sum_k ds k_k      dk_k = scale sum_{h, t} ds q_t      dv_k = sum_{h, t} p dout_t
 // (the sums of dk and dv run over the query heads of the group).  first_key expresses packed documents (the document's first
 // token), a sliding window (t - w + 1) and padding (any value above t: the row is empty, out 0, lse -inf, no gradient).
-// (The reference's own kernels: src/kernels/attention.cu:20,152; its call sites src/models/llama_model.cpp:196-202.)
 #include <climits>
 #include <type_traits>
 
@@ -100,7 +99,7 @@ __device__ __forceinline__ bool all_finite(const f32x16& x) {
 // What a wave's 32 NB queries may look at.
 template <int NB>
 struct QueryMask {
-    int q[NB], first[NB];   // this lane's positions and their first keys (INT_MAX: empty)
+    int q[NB], first[NB];   // this lane's positions and their first keys (INT_MAX: empty, or behind the last row)
     int lo, hi;             // smallest first key and largest position of the wave's rows that are not empty (lo > hi: none)
     int first_max, q_min;   // a tile [k0, k1] is whole for the wave if k0 >= first_max and k1 <= q_min
 
@@ -124,6 +123,8 @@ struct QueryMask {
                     else top = max(top, q[n]);
                     l = min(l, first[n]);
                     m = max(m, first[n]);
+                } else {
+                    first[n] = INT_MAX;
                 }
             }
             lo = wave_min(l);
@@ -215,14 +216,16 @@ struct QueryBlock {
         block_range<WAVES>(lo, hi, mask.lo, mask.hi);
         t_lo = lo <= hi ? lo / kKeys : 1, t_hi = lo <= hi ? hi / kKeys : 0;
         w_lo = mask.lo <= mask.hi ? mask.lo / kKeys : INT_MAX, w_hi = mask.lo <= mask.hi ? mask.hi / kKeys : -1;
-        copy.offsets(ofs, stride, 0, INT_MAX);
+        start();
     }
+    // before a walk over the tiles
+    __device__ __forceinline__ void start() { copy.offsets(ofs, stride, 0, INT_MAX); }
     __device__ __forceinline__ char* keys(int buf) const { return lds + buf * T::kBytes; }
     __device__ __forceinline__ char* values(int buf) const { return lds + (2 + buf) * T::kBytes; }
     // copies of tile t (of the last one if it is behind it) into `buf`, one by one
     __device__ __forceinline__ void aim(int buf, int t) {
         const int row0 = min(t, t_hi) * kKeys;
-        if (row0 + kKeys > a.T) copy.offsets(ofs, stride, row0, a.T);   // the last tile of the sequence: none follows
+        if (row0 + kKeys > a.T) copy.offsets(ofs, stride, row0, a.T);   // the last tile of the sequence: none follows in this walk
         knext = reinterpret_cast<const char*>(kbase) + row0 * stride;
         vnext = knext + (int64_t)a.Nkv * a.head_dim * 2;
         to = lds_at + buf * T::kBytes;
@@ -295,6 +298,7 @@ __device__ __forceinline__ uint32_t attention_forward_careful(W& w, const bf16x8
 #pragma nounroll
     for (int db = 0; db < W::kDims; ++db) {
         f32x16 one = zero16();
+        w.start();
 #pragma nounroll
         for (int t = w.t_lo; t <= w.t_hi; ++t) {
             w.aim(0, t);
@@ -450,6 +454,7 @@ __device__ __forceinline__ void attention_backward_q_careful(W& w, const bf16x8 
 #pragma nounroll
     for (int db = 0; db < W::kDims; ++db) {
         f32x16 one = zero16();
+        w.start();
 #pragma nounroll
         for (int t = w.t_lo; t <= w.t_hi; ++t) {
             w.aim(0, t);
@@ -493,7 +498,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_q_kernel(
             for (int j = 0; j < 8; ++j) d = __builtin_fmaf((float)gf[s][j], (float)of[s][j], d);
         delta = halves_sum(d);
         const int64_t stat = w.statistic();
-        lse2 = w.valid() ? a.lse[stat] * kLog2e : 0.f;
+        lse2 = a.lse[w.valid() ? stat : stat - w.mask.q[0] + a.T - 1] * kLog2e;   // rows behind the last one repeat it
         if (w.lane < 32 && w.valid()) {
             a.delta[stat] = delta;
             a.lse2[stat] = lse2;
@@ -566,8 +571,9 @@ struct KeyBlock {
     const AttentionArgs& a;
     char* lds;
     uint32_t lds_at;
-    int tid, lane, wave, b, kvh, split, k0, k1, ng;
-    int turns;                                // pairs of the workgroup
+    int tid, lane, wave, b, kvh, k0, k1, ng;
+    float* partial;                           // the share's partial sums, or null: the gradients
+    int turns;                                // pairs of the share
     int64_t token, stride, ostride;
     const uint16_t* base;
     int key_;
@@ -581,13 +587,14 @@ struct KeyBlock {
     uint32_t to, sto;                         // and destinations
     uint64_t slanes;
 
-    __device__ __forceinline__ KeyBlock(const AttentionArgs& args, char* lds_) : a(args), lds(lds_), copy(threadIdx.x, args.head_dim) {
+    // Keys kb0 .. of the batch row and head `group`, share `split` of `splits`.
+    __device__ __forceinline__ KeyBlock(const AttentionArgs& args, char* lds_, int group, int kb0, int split, int splits)
+        : a(args), lds(lds_), copy(threadIdx.x, args.head_dim) {
         tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
         lds_at = lds_address(lds) + wave * 1024;
-        const int ngroups = a.B * a.Nkv;
-        const int grp = blockIdx.x % ngroups, rest = blockIdx.x / ngroups;
-        b = grp / a.Nkv, kvh = grp % a.Nkv, split = rest % a.splits;
-        const int kb0 = rest / a.splits * kBlock, kb1 = min(kb0 + kBlock, a.T) - 1;   // the first keys, with the most queries, first
+        b = group / a.Nkv, kvh = group % a.Nkv;
+        partial = splits > 1 ? a.partial + (int64_t)split * a.B * a.T * a.Nkv * 2 * a.head_dim : nullptr;
+        const int kb1 = min(kb0 + kBlock, a.T) - 1;
         k0 = kb0 + wave * 32, k1 = min(k0 + 32, a.T) - 1;
         key_ = k0 + (lane & 31);
         token = (int64_t)(a.Nq + 2 * a.Nkv) * a.head_dim, stride = token * 2, ostride = (int64_t)a.Nq * a.head_dim * 2;
@@ -613,9 +620,9 @@ struct KeyBlock {
             t_hi = l <= h ? h : 0;
         }
         const int64_t pairs = (int64_t)max(t_hi - t_lo + 1, 0) * a.G;
-        turns = pairs > split ? (int)((pairs - split + a.splits - 1) / a.splits) : 0;
+        turns = pairs > split ? (int)((pairs - split + splits - 1) / splits) : 0;
         tile_ = t_hi - split / a.G, head_ = split % a.G;
-        head_step = a.splits % a.G, tile_step = a.splits / a.G;
+        head_step = splits % a.G, tile_step = splits / a.G;
         clamped = true;
         const int64_t head = kvh * a.G + head_, q0 = (int64_t)tile_ * kQueries, row = ((int64_t)b * a.Nq + head) * a.T;
         qnext = reinterpret_cast<const char*>(base + head * a.head_dim) + q0 * stride;
@@ -755,8 +762,8 @@ struct KeyBlock {
     __device__ __forceinline__ void put(int db, const f32x16& dk, const f32x16& dv) const {
         const int key = here(key_);
         const bool valid = key < a.T;
-        if (a.partial) {
-            float* row = a.partial + ((((int64_t)split * a.B + b) * a.T + key) * a.Nkv + kvh) * 2 * a.head_dim;
+        if (partial) {
+            float* row = partial + (((int64_t)b * a.T + key) * a.Nkv + kvh) * 2 * a.head_dim;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const int d = 32 * db + 8 * g + 4 * (lane >> 5);
@@ -778,7 +785,8 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_kernel
     typedef KeyBlock<HDP, WAVES> W;
     typedef typename W::T T;
     __shared__ __attribute__((aligned(16))) char lds[W::kLdsBytes];
-    W w(a, lds);
+    const int groups = a.B * a.Nkv, rest = blockIdx.x / groups;   // the first keys, with the most queries, first
+    W w(a, lds, blockIdx.x % groups, rest / a.splits * W::kBlock, rest % a.splits, a.splits);
     bf16x8 kf[W::kSteps];
     w.load_keys(kf);
     const int row_lane_ = T::row_lane(w.lane), cols_lane_ = T::cols_lane(w.lane);
@@ -829,15 +837,58 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_kernel
     }
 }
 
-// The careful form, a kernel of its own (in one with the loop above, its registers pushed accumulators of the loop out): the same
-// grid, of which the workgroups return whose result was finite.
+// Share `split` of the elements of keys kb0 ..: a lane takes four values of each split at a time, four such groups in flight.
+template <int KEYS, int THREADS>
+__device__ __forceinline__ void join_splits(const AttentionArgs& a, int group, int kb0, int split) {
+    const int per = 2 * a.head_dim / 4, n = min(KEYS, a.T - kb0) * per, step = a.splits * THREADS;
+    const int b = group / a.Nkv, kvh = group % a.Nkv;
+    const int64_t all = (int64_t)a.B * a.T * a.Nkv * per, token = (int64_t)(a.Nq + 2 * a.Nkv) * a.head_dim;
+    const float4* first = reinterpret_cast<const float4*>(a.partial) + (((int64_t)b * a.T + kb0) * a.Nkv + kvh) * per;
+    uint16_t* rows = a.dqkv + ((int64_t)b * a.T + kb0) * token + (int64_t)(a.Nq + kvh) * a.head_dim;
+    for (int i = split * THREADS + threadIdx.x; i < n; i += 4 * step) {
+        int key[4], at[4];
+        float4 x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int j = min(i + u * step, n - 1);
+            key[u] = j / per, at[u] = j % per;
+            x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        for (int s = 0; s < a.splits; ++s)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float4 y = first[s * all + (int64_t)key[u] * a.Nkv * per + at[u]];
+                x[u].x += y.x, x[u].y += y.y, x[u].z += y.z, x[u].w += y.w;
+            }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (i + u * step >= n) break;
+            const bool value = 4 * at[u] >= a.head_dim;
+            const float f = value ? 1.f : a.scale;
+            uint16_t* row = rows + key[u] * token + (value ? (int64_t)(a.Nkv - 1) * a.head_dim : 0) + 4 * at[u];
+            *reinterpret_cast<uint2*>(row) = make_uint2(pack_bf16(x[u].x * f, x[u].y * f), pack_bf16(x[u].z * f, x[u].w * f));
+        }
+    }
+}
+
+// What the keys' kernel leaves: the workgroups of a block of keys add its splits' dk and dv in their order and round once, each a
+// share of the elements.  Where a sum was not finite, the first of them computes the whole block again in the careful form (in one
+// kernel with the loop above, its registers pushed accumulators of that loop out).
 template <int HDP, int WAVES>
-__global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_careful_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_join_kernel(AttentionArgs a) {
     typedef KeyBlock<HDP, WAVES> W;
     typedef typename W::T T;
-    if (a.flags[blockIdx.x] == 0) return;
+    const int groups = a.B * a.Nkv, group = blockIdx.x % groups, rest = blockIdx.x / groups;
+    const int split = rest % a.splits, kb0 = rest / a.splits * W::kBlock;
+    int again = 0;
+    for (int s = 0; s < a.splits; ++s) again |= a.flags[(rest - split + s) * groups + group];
+    if (!again) {
+        if (a.splits > 1) join_splits<W::kBlock, W::kThreads>(a, group, kb0, split);
+        return;
+    }
+    if (split > 0) return;
     __shared__ __attribute__((aligned(16))) char lds[W::kLdsBytes];
-    const W start(a, lds);
+    const W start(a, lds, group, kb0, 0, 1);
     bf16x8 kf[W::kSteps];
     start.load_keys(kf);
 #pragma nounroll
@@ -871,25 +922,6 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_carefu
     }
 }
 
-// Adds the splits' dk and dv in their order and rounds once.  A lane takes four values.
-__global__ __launch_bounds__(256) void attention_join_kernel(AttentionArgs a) {
-    const int per = 2 * a.head_dim / 4;
-    const int64_t n = (int64_t)a.B * a.T * a.Nkv * per, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    const int at = (int)(i % per) * 4, kvh = (int)(i / per % a.Nkv);
-    const int64_t bt = i / per / a.Nkv;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < a.splits; ++s) {
-        const float4 y = reinterpret_cast<const float4*>(a.partial)[s * n + i];
-        x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
-    }
-    const bool value = at >= a.head_dim;
-    const float f = value ? 1.f : a.scale;
-    const int64_t token = (int64_t)(a.Nq + 2 * a.Nkv) * a.head_dim;
-    uint16_t* row = a.dqkv + bt * token + (int64_t)(a.Nq + kvh + (value ? a.Nkv : 0)) * a.head_dim + (value ? at - a.head_dim : at);
-    *reinterpret_cast<uint2*>(row) = make_uint2(pack_bf16(x.x * f, x.y * f), pack_bf16(x.z * f, x.w * f));
-}
-
 // ---- host ----------------------------------------------------------------------------------------------------------------
 constexpr int kUnits = 256;   // compute units the splits are sized for: fixed, so that results do not depend on the partition
 
@@ -899,7 +931,9 @@ static int check_shape(const char* what, int B, int T, int Nq, int Nkv, int head
     LLMQ_REQUIRE(head_dim >= 8 && head_dim <= 128 && head_dim % 8 == 0, "%s: head_dim must be a multiple of 8 from 8 to 128 (got %d)", what, head_dim);
     LLMQ_REQUIRE((int64_t)Nq + 2 * (int64_t)Nkv <= 65536, "%s: too many heads", what);
     LLMQ_REQUIRE(T <= (1 << 30), "%s: sequence too long", what);
-    LLMQ_REQUIRE((int64_t)B * T <= 0x7FFFFFFF && (int64_t)B * Nq * (((int64_t)T + 31) / 32) <= 0x7FFFFFFF, "%s: tensor too large", what);
+    // the grid's threads (256 for 128 queries of a head) fit 32 bits
+    LLMQ_REQUIRE((int64_t)B * T <= 0x7FFFFFFF && (int64_t)B * Nq <= INT_MAX && (int64_t)B * Nq * ((T + 127) / 128) < (1 << 24),
+                 "%s: tensor too large", what);
     return LLMQ_OK;
 }
 
@@ -907,8 +941,9 @@ static int check_shape(const char* what, int B, int T, int Nq, int Nkv, int head
 // eight, which read the queries half as often as four: 1 x 8192 1925 -> 1640 us, documents 283 -> 214, but 8 x 1024 331 -> 340.
 static int kv_block(int head_dim) { return head_dim > 64 ? 256 : 128; }
 
-// Shares of the walk over the queries: enough workgroups for two per compute unit, each with some pairs of work (one per unit:
-// 1 x 8192 2180 us, 8 x 1024 370; three: 1710 and 369).
+// Shares of the walk over the queries: enough workgroups for two per compute unit, each with four pairs of work at least
+// (one per unit: 1 x 8192 2180 us, 8 x 1024 370; three: 1710 and 369.  Eight pairs: 1 x 40 20.5 -> 24.4 us; two: 19.5, but
+// 2 x 129 27.6 -> 28.4).
 static int kv_splits(int B, int T, int Nq, int Nkv, int keys) {
     const int64_t blocks = (int64_t)B * Nkv * ((T + keys - 1) / keys);
     const int64_t pairs = (int64_t)((T + kQueries - 1) / kQueries) * (Nq / Nkv);
@@ -1014,19 +1049,14 @@ extern "C" int llmq_attention_backward_bf16(uint16_t* dqkv, const uint16_t* dout
         LLMQ_HIP_TRY(hipGetLastError());
         launch(attention_backward_kv_kernel<128, 8>, p.blocks, 512);
         LLMQ_HIP_TRY(hipGetLastError());
-        launch(attention_backward_kv_careful_kernel<128, 8>, p.blocks, 512);
+        launch(attention_backward_join_kernel<128, 8>, p.blocks, 512);
     } else {
         launch(attention_backward_q_kernel<64, 4>, q_blocks, 256);
         LLMQ_HIP_TRY(hipGetLastError());
         launch(attention_backward_kv_kernel<64, 4>, p.blocks, 256);
         LLMQ_HIP_TRY(hipGetLastError());
-        launch(attention_backward_kv_careful_kernel<64, 4>, p.blocks, 256);
+        launch(attention_backward_join_kernel<64, 4>, p.blocks, 256);
     }
     LLMQ_HIP_TRY(hipGetLastError());
-    if (p.splits > 1) {
-        const int64_t n = (int64_t)B * T * Nkv * (2 * head_dim / 4);
-        launch(attention_join_kernel, (n + 255) / 256, 256);
-        LLMQ_HIP_TRY(hipGetLastError());
-    }
     return LLMQ_OK;
 }

@@ -3,8 +3,6 @@
 // Per row of logits x[0 .. V) (bf16 or fp32; rows are P >= V elements apart) and its token t:
 //     lse = ln sum_v exp(x_v);  logp = x_t - lse;  entropy = lse - sum_v p_v x_v,  p_v = exp(x_v - lse)
 //     dx_v = dlogp (1[v = t] - p_v) - dentropy p_v (x_v - lse + entropy)
-// (The reference's counterpart is its fused classifier, src/kernels/fused_classifier.cu:92,246,307: loss and gradient of one
-// target per row; entropy and alternatives have none.)
 //
 // HBM bound: the forward reads the logits once (2 or 4 bytes each), the gradient reads and writes them once.
 //
@@ -571,7 +569,7 @@ template <typename E>
 static int token_logprobs_any(float* logp, float* entropy, float* lse, float* top_logp, int* top_ids, const E* logits, const int* targets,
                               void* scratch, size_t scratch_bytes, int64_t N64, int V, int64_t P, int k, hipStream_t stream) {
     const char* what = "token_logprobs";
-    LLMQ_REQUIRE(N64 >= 0 && N64 <= (1 << 24), "%s: 0 to 2^24 rows (got %lld)", what, (long long)N64);
+    LLMQ_REQUIRE(N64 >= 0 && N64 < (1 << 24), "%s: fewer than 2^24 rows are wanted (got %lld)", what, (long long)N64);
     const int N = (int)N64;
     LLMQ_REQUIRE(V >= 1 && V <= (1 << 28) && P >= V && P <= (1 << 28), "%s: vocabulary %d, row length %lld: 1 <= V <= P <= 2^28 is wanted", what, V, (long long)P);
     LLMQ_REQUIRE(k >= 0 && k <= kTopMax, "%s: at most %d alternatives (got %d)", what, kTopMax, k);
@@ -606,7 +604,7 @@ template <typename E>
 static int token_logprobs_backward_any(E* dlogits, const float* dlogp, const float* dentropy, const E* logits, const int* targets,
                                        const float* lse, const float* entropy, float* abs_max, int64_t N64, int V, int64_t P, hipStream_t stream) {
     const char* what = "token_logprobs_backward";
-    LLMQ_REQUIRE(N64 >= 0 && N64 <= (1 << 24), "%s: 0 to 2^24 rows (got %lld)", what, (long long)N64);
+    LLMQ_REQUIRE(N64 >= 0 && N64 < (1 << 24), "%s: fewer than 2^24 rows are wanted (got %lld)", what, (long long)N64);
     LLMQ_REQUIRE(V >= 1 && V <= (1 << 28) && P >= V && P <= (1 << 28), "%s: vocabulary %d, row length %lld: 1 <= V <= P <= 2^28 is wanted", what, V, (long long)P);
     LLMQ_REQUIRE(!dentropy || entropy || N64 == 0, "%s: dentropy needs the forward's entropy", what);
     if (N64 > 0) {
@@ -625,7 +623,7 @@ static int token_logprobs_backward_any(E* dlogits, const float* dlogp, const flo
     const int64_t granules = P / Granule<E>::kN + 2;   // at most, wherever a row begins
     a.chunks = (int)((granules + kLpThreads * kGradTurns - 1) / (kLpThreads * kGradTurns));
     const int64_t blocks = N64 * a.chunks;
-    LLMQ_REQUIRE(blocks <= 0x7FFFFFFF, "%s: tensor too large", what);
+    LLMQ_REQUIRE(blocks < (1 << 24), "%s: tensor too large", what);   // the threads of a grid fit 32 bits
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kLpThreads), 0, stream, a); };
     if (dentropy) {
         if (abs_max) launch(token_logprobs_backward_kernel<E, true, true>);
@@ -641,7 +639,7 @@ static int token_logprobs_backward_any(E* dlogits, const float* dlogp, const flo
 }  // namespace llmq
 
 extern "C" int64_t llmq_token_logprobs_scratch_bytes(int64_t N, int V, int k) {
-    if (N <= 0 || N > (1 << 24) || V <= 0 || k < 0 || k > llmq::kTopMax) return 0;
+    if (N <= 0 || N >= (1 << 24) || V <= 0 || k < 0 || k > llmq::kTopMax) return 0;
     return llmq::logprob_scratch((int)N, V, k);
 }
 extern "C" int llmq_token_logprobs_bf16(float* logp, float* entropy_or_null, float* lse, float* top_logp, int* top_ids, const uint16_t* logits,

@@ -30,6 +30,8 @@ Names, argument order and in-place "out first" convention are the reference's:
     get_token_logprobs_scratch_size(N, V, k)
 `stream` is a raw hipStream_t handle (0 = torch's current stream).
 """
+import contextlib
+
 import torch
 
 from . import capi
@@ -410,7 +412,9 @@ def _launch_context(stream, *tensors):
         if dev is not None and t.device != dev:
             raise ValueError("all tensors must be on one device (got %s and %s)" % (dev, t.device))
         dev = t.device
-    return torch.cuda.device(dev), stream if stream else torch.cuda.current_stream(dev).cuda_stream
+    ctx = contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    # the handle itself: building a Stream object for it takes 2.6 us, a quarter of a short call
+    return ctx, stream if stream else torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def _attention_dims(qkv, per_query, Nq, Nkv, first_key, softmax_scale):

@@ -241,3 +241,145 @@ def test_gradient_against_differences(K):
         diff = (loss(x.double() + eps * step) - loss(x.double() - eps * step)) / (2 * eps)
         # central differences: eps^2 / 6 of a third derivative of order sum |step|^3 p; fp32 roundings of the gradient
         assert abs(diff - (grad.double() * step).sum().item()) <= 1e-5 * (1 + grad.abs().double().mul(step.abs()).sum().item())
+
+
+def test_results_repeat_and_streams_and_graphs_agree(K):
+    """The same bits from call to call, on another stream, and from every replay of captured calls that share their scratch, with
+    the program's own work on the same tensors between the replays."""
+    for N, V, k in ((1, 70001, 20), (2, 4100, 0), (700, 1003, 5)):
+        x, t = make(N, V, V, torch.bfloat16)
+        data = x.clone()
+        side = torch.cuda.Stream()
+        new = lambda *s: torch.empty(s, device="cuda")  # noqa: E731
+        logp, ent, lse, grad, am = new(N), new(N), new(N), torch.empty_like(x), new(1)
+        top, ids = (new(N, k), torch.empty((N, k), dtype=torch.int32, device="cuda")) if k else (None, None)
+        scratch = torch.empty(K.get_token_logprobs_scratch_size(N, V, k) + 16, dtype=torch.uint8, device="cuda")
+        ones = torch.ones(N, device="cuda")
+
+        def step():
+            K.token_logprobs(logp, ent, lse, top, ids, x, t, scratch, V)
+            K.token_logprobs_backward(grad, ones, ones, x, t, lse, ent, am, V)
+
+        step()
+        graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+        for g in graphs:
+            with torch.cuda.graph(g):
+                step()
+        for turn in range(4):
+            x.copy_(data if turn % 2 == 0 else data * 0.5)
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                want = [y for y in forward(K, x, t, V, k) if y is not None]
+                dx = torch.empty_like(x)
+                K.token_logprobs_backward(dx, ones, ones, x, t, want[2], want[1], None, V)
+            torch.cuda.current_stream().wait_stream(side)
+            for y in (logp, ent, lse, grad, am):
+                y.fill_(math.nan)
+            scratch.fill_(0xFF)
+            graphs[turn // 2].replay()
+            got = [y for y in (logp, ent, lse, top, ids) if y is not None]
+            assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(grad, dx)
+            assert am.item() == grad.abs().max().item()
+            step()
+            assert torch.equal(grad, dx)
+
+
+def test_logits_of_more_than_four_gibibytes(K):
+    """The last rows of logits that pass 2^32 bytes equal the same rows alone, bit for bit (a row is summed by one workgroup from
+    512 rows on)."""
+    N, V, tail = 15000, 151936, 600
+    x = torch.zeros((N, V), dtype=torch.bfloat16, device="cuda")
+    part, t1 = make(tail, V, V, torch.bfloat16)
+    x[-tail:] = part
+    t = torch.zeros(N, dtype=torch.int32, device="cuda")
+    t[-tail:] = t1
+    got, want = forward(K, x, t, V, 3), forward(K, part, t1, V, 3)
+    assert all(torch.equal(a[-tail:], b) for a, b in zip(got, want))
+    assert torch.allclose(got[2][:-tail], torch.full((), math.log(V), device="cuda"), rtol=1e-6, atol=0)
+    ones = torch.ones(N, device="cuda")
+    dpart = torch.empty_like(part)
+    K.token_logprobs_backward(dpart, ones[:tail], ones[:tail], part, t1, want[2], want[1], None, V)
+    K.token_logprobs_backward(x, ones, ones, x, t, got[2], got[1], None, V)
+    assert torch.equal(x[-tail:], dpart)
+
+
+def test_empty_calls(K):
+    x, t = torch.empty((0, 9), device="cuda"), torch.empty(0, dtype=torch.int32, device="cuda")
+    e, am = torch.empty(0, device="cuda"), torch.full((1,), 3.0, device="cuda")
+    K.token_logprobs(e, e, e, None, None, x, t, None)
+    K.token_logprobs_backward(x, e, e, x, t, e, e, am)
+    assert am.item() == 0 and K.get_token_logprobs_scratch_size(0, 9, 4) == 0
+
+
+def test_leading_dimensions_and_registered_operators(K):
+    import llmq_amd.ops  # noqa: F401
+    x, t = make(12, 1003, 1010, torch.bfloat16)
+    want = forward(K, x, t, 1003, 3)
+    x3, t3 = x.view(3, 4, 1010), t.view(3, 4)
+    logp, ent, lse = (torch.empty((3, 4), device="cuda") for _ in range(3))
+    top, ids = torch.empty((3, 4, 3), device="cuda"), torch.empty((3, 4, 3), dtype=torch.int32, device="cuda")
+    torch.ops.llmq.token_logprobs(logp, ent, lse, top, ids, x3, t3, None, 1003)
+    for a, b in zip((logp, ent, lse, top, ids), want):
+        assert torch.equal(a.view(b.shape), b)
+    g, g3, ones, am = torch.empty_like(x), torch.empty_like(x3), torch.ones((3, 4), device="cuda"), torch.zeros(1, device="cuda")
+    K.token_logprobs_backward(g, ones.view(12), None, x, t, want[2], None, None, 1003)
+    torch.ops.llmq.token_logprobs_backward(g3, ones, None, x3, t3, lse, None, am, 1003)
+    assert torch.equal(g3.view(12, 1010), g) and am.item() == g.abs().max().item()
+
+
+def test_nothing_is_written_behind_the_tensors(K):
+    for dtype in (torch.bfloat16, torch.float32):
+        N, V, P = 5, 1001, 1003
+        x, t = make(N, V, P, dtype)
+        _, ent, lse, _, _ = forward(K, x, t, V)
+        buf = torch.full((N * P + 64,), 7.0, dtype=dtype, device="cuda")
+        ones = torch.ones(N, device="cuda")
+        K.token_logprobs_backward(buf[32:-32].view(N, P), ones, ones, x, t, lse, ent, None, V)
+        assert (buf[:32] == 7).all() and (buf[-32:] == 7).all() and torch.isfinite(buf).all()
+        outs = torch.full((6, N + 2), 7.0, device="cuda")
+        top, ids = torch.full((N + 2, 4), 7.0, device="cuda"), torch.full((N + 2, 4), 7, dtype=torch.int32, device="cuda")
+        K.token_logprobs(outs[0, 1:-1], outs[1, 1:-1], outs[2, 1:-1], top[1:-1], ids[1:-1], x, t, None, V)
+        assert (outs[:3, 0] == 7).all() and (outs[:3, -1] == 7).all() and (outs[3:] == 7).all()
+        assert (top[[0, -1]] == 7).all() and (ids[[0, -1]] == 7).all() and torch.equal(outs[2, 1:-1], lse)
+
+
+def test_refusals_on_device_tensors(K):
+    x, t = make(2, 70000, 70001, torch.bfloat16)
+    x = x[:, :70000].contiguous()
+    o = lambda *s: torch.zeros(s or (2,), device="cuda")  # noqa: E731
+    ids = torch.zeros((2, 3), dtype=torch.int32, device="cuda")
+    need = K.get_token_logprobs_scratch_size(2, 70000, 3)
+    assert need > 0
+    s = torch.empty(need, dtype=torch.uint8, device="cuda")
+    logp, ent, lse, top = o(), o(), o(), o(2, 3)
+
+    def refused(call, *a, **k):
+        with pytest.raises(ValueError):
+            call(*a, **k)
+
+    f, b = K.token_logprobs, K.token_logprobs_backward
+    refused(f, logp, ent, lse, top, ids, x.half(), t, s)
+    refused(f, logp, ent, lse, top, ids, x.double(), t, s)
+    refused(f, logp, ent, lse, top, ids, x, t.long(), s)
+    refused(f, logp, ent, lse, top, ids, x, t[:1], s)
+    refused(f, logp, ent, lse, top, None, x, t, s)
+    refused(f, logp, ent, lse, top, ids[:, :2], x, t, s)
+    refused(f, logp, ent, lse, o(2, 33), torch.zeros((2, 33), dtype=torch.int32, device="cuda"), x, t, s)
+    refused(f, logp, ent, lse, top, ids, x, t, None)
+    refused(f, logp, ent, lse, top, ids, x, t, s[:-16])
+    refused(f, logp, ent, lse, top, ids, x, t, s, 70001)
+    refused(f, logp, ent, lse, top, ids, x, t, s, 0)
+    refused(f, logp, ent, lse, top, ids, x[:, ::2], t, s)
+    refused(f, logp, ent, lse, top, ids, x[0], t, s)
+    refused(f, None, ent, lse, top, ids, x, t, s)
+    refused(f, logp.double(), ent, lse, top, ids, x, t, s)
+    flat = torch.zeros(140001, dtype=torch.bfloat16, device="cuda")
+    refused(f, logp, ent, lse, top, ids, flat[1:].view(2, 70000), t, s)
+    d = torch.empty_like(x)
+    refused(b, d[:1], logp, None, x, t, lse, None, None)
+    refused(b, d, logp, ent, x, t, lse, None, None)
+    refused(b, d.float(), logp, None, x, t, lse, None, None)
+    refused(b, d, o(3), None, x, t, lse, None, None)
+    refused(b, d, logp, None, x, t, lse, None, None, 70001)
+    refused(b, flat[1:].view(2, 70000), logp, None, x, t, lse, None, None)
+    assert all((y == 0).all() for y in (logp, ent, lse, top, ids))
