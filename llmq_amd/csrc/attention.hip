@@ -330,6 +330,10 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_forward_kernel(Att
     typedef typename W::T T;
     __shared__ __attribute__((aligned(16))) char lds[W::kLdsBytes];
     W w(a, lds);
+    if (w.t_lo <= w.t_hi) {   // before the queries, whose latency it shares
+        w.aim(w.t_lo & 1, w.t_lo);
+        w.issue_all();
+    }
     bf16x8 qf[W::kSteps];
     w.load_rows(qf, w.base, w.token);
 
@@ -339,10 +343,6 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_forward_kernel(Att
     for (int db = 0; db < W::kDims; ++db) o[db] = zero16();
     const int row_lane_ = T::row_lane(w.lane), cols_lane_ = T::cols_lane(w.lane);
 
-    if (w.t_lo <= w.t_hi) {
-        w.aim(w.t_lo & 1, w.t_lo);
-        w.issue_all();
-    }
 #pragma nounroll
     for (int t = w.t_lo; t <= w.t_hi; ++t) {
         copies_landed();
@@ -482,7 +482,10 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_q_kernel(
     typedef typename W::T T;
     __shared__ __attribute__((aligned(16))) char lds[W::kLdsBytes];
     W w(a, lds);
-
+    if (w.t_lo <= w.t_hi) {   // before the rows, whose latency it shares
+        w.aim(w.t_lo & 1, w.t_lo);
+        w.issue_all();
+    }
     bf16x8 qf[W::kSteps], gf[W::kSteps];
     w.load_rows(qf, w.base, w.token);
     const int64_t out_row = (int64_t)a.Nq * a.head_dim;
@@ -512,10 +515,6 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_q_kernel(
     f32x16 dq[W::kDims];
 #pragma unroll
     for (int db = 0; db < W::kDims; ++db) dq[db] = zero16();
-    if (w.t_lo <= w.t_hi) {
-        w.aim(w.t_lo & 1, w.t_lo);
-        w.issue_all();
-    }
 #pragma nounroll
     for (int t = w.t_lo; t <= w.t_hi; ++t) {
         copies_landed();
@@ -787,6 +786,12 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_kernel
     __shared__ __attribute__((aligned(16))) char lds[W::kLdsBytes];
     const int groups = a.B * a.Nkv, rest = blockIdx.x / groups;   // the first keys, with the most queries, first
     W w(a, lds, blockIdx.x % groups, rest / a.splits * W::kBlock, rest % a.splits, a.splits);
+    typename W::Pair next;
+    if (w.turns > 0) {
+        next = w.aimed();
+        w.aim(0);
+        w.issue_all();
+    }
     bf16x8 kf[W::kSteps];
     w.load_keys(kf);
     const int row_lane_ = T::row_lane(w.lane), cols_lane_ = T::cols_lane(w.lane);
@@ -794,12 +799,6 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_kernel
     f32x16 dk[W::kDims], dv[W::kDims];
 #pragma unroll
     for (int db = 0; db < W::kDims; ++db) dk[db] = zero16(), dv[db] = zero16();
-    typename W::Pair next;
-    if (w.turns > 0) {
-        next = w.aimed();
-        w.aim(0);
-        w.issue_all();
-    }
 #pragma nounroll
     for (int turn = 0; turn < w.turns; ++turn) {
         copies_landed();
