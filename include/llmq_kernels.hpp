@@ -604,4 +604,98 @@ inline void adamw_update(__hip_bfloat16* params, const __hip_bfloat16* grads, __
                                                    weight_decay, grad_scale, abs_max, seed, stream));
 }
 
+// ---- attention on the fused QKV tensor (llmq_fp8.h: what first_key, lse and the scratch are) ------------------------
+// bf16 tensors; first_key may be null (an empty Tensor).
+inline std::size_t get_attention_backward_scratch_size(int B, int T, int Nq, int Nkv, int head_dim) {
+    return (std::size_t)llmq_attention_backward_scratch_bytes(B, T, Nq, Nkv, head_dim);
+}
+inline void attention_forward(__hip_bfloat16* out, float* lse, const __hip_bfloat16* qkv, const std::int32_t* first_key,
+                              float* abs_max_ptr, float softmax_scale, int B, int T, int Nq, int Nkv, int head_dim,
+                              hipStream_t stream) {
+    llmq_detail::check(llmq_attention_forward_bf16(llmq_detail::u16(out), lse, llmq_detail::u16(qkv), first_key, abs_max_ptr,
+                                                   softmax_scale, B, T, Nq, Nkv, head_dim, stream));
+}
+inline void attention_forward(Tensor& out, Tensor& lse, const Tensor& qkv, const Tensor& first_key, float* abs_max_ptr,
+                              float softmax_scale, int B, int T, int Nq, int Nkv, int head_dim, hipStream_t stream) {
+    if (out.DType != ETensorDType::BF16 || lse.DType != ETensorDType::FP32 || qkv.DType != ETensorDType::BF16 ||
+        (first_key && first_key.DType != ETensorDType::INT32))
+        llmq_detail::unsupported(__func__, out, lse, qkv, first_key);
+    attention_forward(out.get<__hip_bfloat16>(), lse.get<float>(), qkv.get<__hip_bfloat16>(),
+                      first_key.get_optional<std::int32_t>(), abs_max_ptr, softmax_scale, B, T, Nq, Nkv, head_dim, stream);
+}
+inline void attention_backward(__hip_bfloat16* dqkv, const __hip_bfloat16* dout, const __hip_bfloat16* out, const float* lse,
+                               const __hip_bfloat16* qkv, const std::int32_t* first_key, std::byte* scratch,
+                               std::size_t scratch_bytes, float softmax_scale, int B, int T, int Nq, int Nkv, int head_dim,
+                               hipStream_t stream) {
+    llmq_detail::check(llmq_attention_backward_bf16(llmq_detail::u16(dqkv), llmq_detail::u16(dout), llmq_detail::u16(out), lse,
+                                                    llmq_detail::u16(qkv), first_key, scratch, scratch_bytes, softmax_scale, B,
+                                                    T, Nq, Nkv, head_dim, stream));
+}
+inline void attention_backward(Tensor& dqkv, const Tensor& dout, const Tensor& out, const Tensor& lse, const Tensor& qkv,
+                               const Tensor& first_key, Tensor& scratch, float softmax_scale, int B, int T, int Nq, int Nkv,
+                               int head_dim, hipStream_t stream) {
+    if (dqkv.DType != ETensorDType::BF16 || dout.DType != ETensorDType::BF16 || out.DType != ETensorDType::BF16 ||
+        lse.DType != ETensorDType::FP32 || qkv.DType != ETensorDType::BF16 || (first_key && first_key.DType != ETensorDType::INT32))
+        llmq_detail::unsupported(__func__, dqkv, dout, out, lse, qkv, first_key);
+    attention_backward(dqkv.get<__hip_bfloat16>(), dout.get<__hip_bfloat16>(), out.get<__hip_bfloat16>(), lse.get<float>(),
+                       qkv.get<__hip_bfloat16>(), first_key.get_optional<std::int32_t>(), scratch.Data, scratch.bytes(),
+                       softmax_scale, B, T, Nq, Nkv, head_dim, stream);
+}
+
+// ---- log probabilities of given tokens and their gradient --------------------------------------------------------------
+// N rows of V logits, P elements apart; entropy, and for k = 0 top_logp and top_ids, may be null (empty Tensors).
+inline std::size_t get_token_logprobs_scratch_size(long N, int V, int k) {
+    return (std::size_t)llmq_token_logprobs_scratch_bytes(N, V, k);
+}
+inline void token_logprobs(float* logp, float* entropy, float* lse, float* top_logp, std::int32_t* top_ids,
+                           const __hip_bfloat16* logits, const std::int32_t* targets, std::byte* scratch, std::size_t scratch_bytes,
+                           long N, int V, long P, int k, hipStream_t stream) {
+    llmq_detail::check(llmq_token_logprobs_bf16(logp, entropy, lse, top_logp, top_ids, llmq_detail::u16(logits), targets, scratch,
+                                                scratch_bytes, N, V, P, k, stream));
+}
+inline void token_logprobs(float* logp, float* entropy, float* lse, float* top_logp, std::int32_t* top_ids, const float* logits,
+                           const std::int32_t* targets, std::byte* scratch, std::size_t scratch_bytes, long N, int V, long P, int k,
+                           hipStream_t stream) {
+    llmq_detail::check(llmq_token_logprobs_f32(logp, entropy, lse, top_logp, top_ids, logits, targets, scratch, scratch_bytes, N, V,
+                                               P, k, stream));
+}
+inline void token_logprobs(Tensor& logp, Tensor& entropy, Tensor& lse, Tensor& top_logp, Tensor& top_ids, const Tensor& logits,
+                           const Tensor& targets, Tensor& scratch, long N, int V, long P, int k, hipStream_t stream) {
+    float* ent = entropy ? entropy.get<float>() : nullptr;
+    float* top = top_logp ? top_logp.get<float>() : nullptr;
+    std::int32_t* ids = top_ids ? top_ids.get<std::int32_t>() : nullptr;
+    const std::size_t bytes = scratch ? scratch.bytes() : 0;
+    if (logits.DType == ETensorDType::BF16)
+        token_logprobs(logp.get<float>(), ent, lse.get<float>(), top, ids, logits.get<__hip_bfloat16>(), targets.get<std::int32_t>(),
+                       scratch.Data, bytes, N, V, P, k, stream);
+    else if (logits.DType == ETensorDType::FP32)
+        token_logprobs(logp.get<float>(), ent, lse.get<float>(), top, ids, logits.get<float>(), targets.get<std::int32_t>(),
+                       scratch.Data, bytes, N, V, P, k, stream);
+    else llmq_detail::unsupported(__func__, logits);
+}
+inline void token_logprobs_backward(__hip_bfloat16* dlogits, const float* dlogp, const float* dentropy, const __hip_bfloat16* logits,
+                                    const std::int32_t* targets, const float* lse, const float* entropy, float* abs_max_ptr, long N,
+                                    int V, long P, hipStream_t stream) {
+    llmq_detail::check(llmq_token_logprobs_backward_bf16(llmq_detail::u16(dlogits), dlogp, dentropy, llmq_detail::u16(logits), targets,
+                                                         lse, entropy, abs_max_ptr, N, V, P, stream));
+}
+inline void token_logprobs_backward(float* dlogits, const float* dlogp, const float* dentropy, const float* logits,
+                                    const std::int32_t* targets, const float* lse, const float* entropy, float* abs_max_ptr, long N,
+                                    int V, long P, hipStream_t stream) {
+    llmq_detail::check(llmq_token_logprobs_backward_f32(dlogits, dlogp, dentropy, logits, targets, lse, entropy, abs_max_ptr, N, V, P,
+                                                        stream));
+}
+inline void token_logprobs_backward(Tensor& dlogits, const Tensor& dlogp, const Tensor& dentropy, const Tensor& logits,
+                                    const Tensor& targets, const Tensor& lse, const Tensor& entropy, float* abs_max_ptr, long N, int V,
+                                    long P, hipStream_t stream) {
+    const float *dl = dlogp.get<float>(), *de = dentropy.get_optional<float>(), *ent = entropy.get_optional<float>();
+    if (dlogits.DType == ETensorDType::BF16 && logits.DType == ETensorDType::BF16)
+        token_logprobs_backward(dlogits.get<__hip_bfloat16>(), dl, de, logits.get<__hip_bfloat16>(), targets.get<std::int32_t>(),
+                                lse.get<float>(), ent, abs_max_ptr, N, V, P, stream);
+    else if (dlogits.DType == ETensorDType::FP32 && logits.DType == ETensorDType::FP32)
+        token_logprobs_backward(dlogits.get<float>(), dl, de, logits.get<float>(), targets.get<std::int32_t>(), lse.get<float>(), ent,
+                                abs_max_ptr, N, V, P, stream);
+    else llmq_detail::unsupported(__func__, dlogits, logits);
+}
+
 #endif  // LLMQ_KERNELS_HPP
