@@ -50,7 +50,8 @@ __device__ __forceinline__ f32x16 zero16() {
     return z;
 }
 
-// Column-side operand of a wave, straight from global memory: lane -> position l % 32, chunk 2 step + l / 32.
+// Column-side operand of a wave, straight from global memory: lane -> position l % 32, chunk 2 step + l / 32.  On its way from
+// here, waited for in `arrived`.
 template <int HDP>
 __device__ __forceinline__ void load_columns(bf16x8 (&f)[HDP / 16], const uint16_t* row, int lane, int head_dim) {
 #pragma unroll
@@ -59,9 +60,11 @@ __device__ __forceinline__ void load_columns(bf16x8 (&f)[HDP / 16], const uint16
         const uint16_t* p = d < head_dim ? row + d : reinterpret_cast<const uint16_t*>(attention_zeros);
         f[s] = *reinterpret_cast<const bf16x8*>(p);
     }
-    // waited for here, not in every turn of the loop that uses them
+}
+template <int N>
+__device__ __forceinline__ void arrived(bf16x8 (&f)[N]) {   // not in every turn of the loop that uses them
 #pragma unroll
-    for (int s = 0; s < HDP / 16; ++s) asm volatile("" : "+v"(f[s]));
+    for (int s = 0; s < N; ++s) asm volatile("" : "+v"(f[s]));
 }
 
 // Stores dimensions 32 db .. of a transposed result (dimensions by positions) times `factor` as bf16 to `row`, this lane's
@@ -183,7 +186,7 @@ struct QueryBlock {
     const AttentionArgs& a;
     char* lds;
     uint32_t lds_at;            // address of the wave's share
-    int tid, lane, b, kvh, head;
+    int tid, lane, b, kvh, head, q0;
     int64_t token, stride;      // elements of a token, bytes
     const uint16_t *base, *kbase;
     Copy copy;
@@ -203,10 +206,13 @@ struct QueryBlock {
         const int ngroups = a.B * a.Nkv, nq = (a.T + kBlock - 1) / kBlock;
         const int grp = blockIdx.x % ngroups, rest = blockIdx.x / ngroups;
         b = grp / a.Nkv, kvh = grp % a.Nkv, head = kvh * a.G + rest % a.G;
-        const int q0 = (nq - 1 - rest / a.G) * kBlock + wave * 32;
+        q0 = (nq - 1 - rest / a.G) * kBlock + wave * 32;
         token = (int64_t)(a.Nq + 2 * a.Nkv) * a.head_dim, stride = token * 2;
         base = a.qkv + b * a.T * token;
         kbase = base + (int64_t)(a.Nq + kvh) * a.head_dim;
+    }
+    // What the rows look at, and the first copies.
+    __device__ __forceinline__ void begin() {
         if (a.head_dim < HDP) {   // block_range ends with a barrier
 #pragma unroll
             for (int i = 0; i < 4; ++i) T::template clear<kThreads>(lds + i * T::kBytes, tid);
@@ -217,6 +223,10 @@ struct QueryBlock {
         t_lo = lo <= hi ? lo / kKeys : 1, t_hi = lo <= hi ? hi / kKeys : 0;
         w_lo = mask.lo <= mask.hi ? mask.lo / kKeys : INT_MAX, w_hi = mask.lo <= mask.hi ? mask.hi / kKeys : -1;
         start();
+        if (t_lo <= t_hi) {
+            aim(t_lo & 1, t_lo);
+            issue_all();
+        }
     }
     // before a walk over the tiles
     __device__ __forceinline__ void start() { copy.offsets(ofs, stride, 0, INT_MAX); }
@@ -238,8 +248,9 @@ struct QueryBlock {
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) issue(i);
     }
+    __device__ __forceinline__ int row() const { return min(q0 + (lane & 31), a.T - 1); }   // rows behind the last one repeat it
     __device__ __forceinline__ void load_rows(bf16x8 (&f)[kSteps], const uint16_t* tensor, int64_t row_elements) const {
-        load_columns<HDP>(f, tensor + min(mask.q[0], a.T - 1) * row_elements + (int64_t)head * a.head_dim, lane, a.head_dim);
+        load_columns<HDP>(f, tensor + row() * row_elements + (int64_t)head * a.head_dim, lane, a.head_dim);
     }
     __device__ __forceinline__ bool whole(int t) const { return mask.whole(t * kKeys, t * kKeys + kKeys - 1); }
     __device__ __forceinline__ bool allowed(int t, int rb, int i) const { return mask.allowed(0, t * kKeys + tile_row(rb, i, lane)); }
@@ -330,12 +341,10 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_forward_kernel(Att
     typedef typename W::T T;
     __shared__ __attribute__((aligned(16))) char lds[W::kLdsBytes];
     W w(a, lds);
-    if (w.t_lo <= w.t_hi) {   // before the queries, whose latency it shares
-        w.aim(w.t_lo & 1, w.t_lo);
-        w.issue_all();
-    }
     bf16x8 qf[W::kSteps];
-    w.load_rows(qf, w.base, w.token);
+    w.load_rows(qf, w.base, w.token);   // its latency covers what follows
+    w.begin();
+    arrived(qf);
 
     f32x16 o[W::kDims], s[2];
     float m = -__builtin_huge_valf(), sum[2] = {0.f, 0.f};
@@ -482,18 +491,17 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_q_kernel(
     typedef typename W::T T;
     __shared__ __attribute__((aligned(16))) char lds[W::kLdsBytes];
     W w(a, lds);
-    if (w.t_lo <= w.t_hi) {   // before the rows, whose latency it shares
-        w.aim(w.t_lo & 1, w.t_lo);
-        w.issue_all();
-    }
     bf16x8 qf[W::kSteps], gf[W::kSteps];
-    w.load_rows(qf, w.base, w.token);
-    const int64_t out_row = (int64_t)a.Nq * a.head_dim;
-    w.load_rows(gf, a.dout + (int64_t)w.b * a.T * out_row, out_row);
     float delta, lse2;
     {
         bf16x8 of[W::kSteps];
+        const int64_t out_row = (int64_t)a.Nq * a.head_dim;
+        w.load_rows(gf, a.dout + (int64_t)w.b * a.T * out_row, out_row);
         w.load_rows(of, a.out + (int64_t)w.b * a.T * out_row, out_row);
+        w.load_rows(qf, w.base, w.token);
+        lse2 = a.lse[((int64_t)w.b * a.Nq + w.head) * a.T + w.row()] * kLog2e;
+        w.begin();
+        arrived(gf), arrived(of), arrived(qf);
         float d = 0.f;
 #pragma unroll
         for (int s = 0; s < W::kSteps; ++s)
@@ -501,7 +509,6 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_q_kernel(
             for (int j = 0; j < 8; ++j) d = __builtin_fmaf((float)gf[s][j], (float)of[s][j], d);
         delta = halves_sum(d);
         const int64_t stat = w.statistic();
-        lse2 = a.lse[w.valid() ? stat : stat - w.mask.q[0] + a.T - 1] * kLog2e;   // rows behind the last one repeat it
         if (w.lane < 32 && w.valid()) {
             a.delta[stat] = delta;
             a.lse2[stat] = lse2;
@@ -570,7 +577,7 @@ struct KeyBlock {
     const AttentionArgs& a;
     char* lds;
     uint32_t lds_at;
-    int tid, lane, wave, b, kvh, k0, k1, ng;
+    int tid, lane, wave, b, kvh, kb0, split, splits, k0, k1, ng;
     float* partial;                           // the share's partial sums, or null: the gradients
     int turns;                                // pairs of the share
     int64_t token, stride, ostride;
@@ -586,18 +593,21 @@ struct KeyBlock {
     uint32_t to, sto;                         // and destinations
     uint64_t slanes;
 
-    // Keys kb0 .. of the batch row and head `group`, share `split` of `splits`.
-    __device__ __forceinline__ KeyBlock(const AttentionArgs& args, char* lds_, int group, int kb0, int split, int splits)
+    // Keys `first` .. of the batch row and head `group`, share `share` of `shares`.
+    __device__ __forceinline__ KeyBlock(const AttentionArgs& args, char* lds_, int group, int first, int share, int shares)
         : a(args), lds(lds_), copy(threadIdx.x, args.head_dim) {
         tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
         lds_at = lds_address(lds) + wave * 1024;
-        b = group / a.Nkv, kvh = group % a.Nkv;
+        b = group / a.Nkv, kvh = group % a.Nkv, kb0 = first, split = share, splits = shares;
         partial = splits > 1 ? a.partial + (int64_t)split * a.B * a.T * a.Nkv * 2 * a.head_dim : nullptr;
-        const int kb1 = min(kb0 + kBlock, a.T) - 1;
         k0 = kb0 + wave * 32, k1 = min(k0 + 32, a.T) - 1;
         key_ = k0 + (lane & 31);
         token = (int64_t)(a.Nq + 2 * a.Nkv) * a.head_dim, stride = token * 2, ostride = (int64_t)a.Nq * a.head_dim * 2;
         base = a.qkv + b * a.T * token;
+    }
+    // The pairs that look at the keys, and the copies of the values.
+    __device__ __forceinline__ void begin() {
+        const int kb1 = min(kb0 + kBlock, a.T) - 1;
         if (a.head_dim < HDP) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) T::template clear<kThreads>(lds + i * T::kBytes, tid);
@@ -786,14 +796,16 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_kernel
     __shared__ __attribute__((aligned(16))) char lds[W::kLdsBytes];
     const int groups = a.B * a.Nkv, rest = blockIdx.x / groups;   // the first keys, with the most queries, first
     W w(a, lds, blockIdx.x % groups, rest / a.splits * W::kBlock, rest % a.splits, a.splits);
+    bf16x8 kf[W::kSteps];
+    w.load_keys(kf);   // its latency covers what follows
+    w.begin();
     typename W::Pair next;
     if (w.turns > 0) {
         next = w.aimed();
         w.aim(0);
         w.issue_all();
     }
-    bf16x8 kf[W::kSteps];
-    w.load_keys(kf);
+    arrived(kf);
     const int row_lane_ = T::row_lane(w.lane), cols_lane_ = T::cols_lane(w.lane);
 
     f32x16 dk[W::kDims], dv[W::kDims];
@@ -887,9 +899,11 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_join_kern
     }
     if (split > 0) return;
     __shared__ __attribute__((aligned(16))) char lds[W::kLdsBytes];
-    const W start(a, lds, group, kb0, 0, 1);
+    W start(a, lds, group, kb0, 0, 1);
+    start.begin();
     bf16x8 kf[W::kSteps];
     start.load_keys(kf);
+    arrived(kf);
 #pragma nounroll
     for (int db = 0; db < W::kDims; ++db) {
         f32x16 one_k = zero16(), one_v = zero16();
