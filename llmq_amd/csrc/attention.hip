@@ -249,6 +249,17 @@ struct QueryBlock {
         for (int i = 0; i < kCopies; ++i) issue(i);
     }
     __device__ __forceinline__ int row() const { return min(q0 + (lane & 31), a.T - 1); }   // rows behind the last one repeat it
+    // Tiles from t on, before `to`, that the wave only copies for the others; returns the next.  (As a branch in the walk itself it
+    // moved accumulators between registers: 8 x 1024 84 -> 87.5 us, where this way it is 82.3.)
+    __device__ __forceinline__ int pass(int t, int to) {
+#pragma nounroll
+        for (; t <= t_hi && t < to; ++t) {
+            copies_landed();
+            aim((t + 1) & 1, t + 1);
+            issue_all();
+        }
+        return t;
+    }
     __device__ __forceinline__ void load_rows(bf16x8 (&f)[kSteps], const uint16_t* tensor, int64_t row_elements) const {
         load_columns<HDP>(f, tensor + row() * row_elements + (int64_t)head * a.head_dim, lane, a.head_dim);
     }
@@ -352,8 +363,9 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_forward_kernel(Att
     for (int db = 0; db < W::kDims; ++db) o[db] = zero16();
     const int row_lane_ = T::row_lane(w.lane), cols_lane_ = T::cols_lane(w.lane);
 
+    int t = w.pass(w.t_lo, w.w_lo);
 #pragma nounroll
-    for (int t = w.t_lo; t <= w.t_hi; ++t) {
+    for (; t <= w.w_hi; ++t) {
         copies_landed();
         const char* keys = w.keys(t & 1);
         char* values = w.values(t & 1);
@@ -396,6 +408,8 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_forward_kernel(Att
 #pragma unroll
             for (int db = 0; db < W::kDims; ++db) o[db] = mfma(T::cols(values, cols_lane, db, u), pf[u], o[db]);
     }
+
+    w.pass(t, INT_MAX);
 
     const float l = halves_sum(sum[0] + sum[1]), inv = l == 0.f ? 0.f : 1.f / l;
     if (w.valid() && w.lane < 32)
@@ -522,8 +536,9 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_q_kernel(
     f32x16 dq[W::kDims];
 #pragma unroll
     for (int db = 0; db < W::kDims; ++db) dq[db] = zero16();
+    int t = w.pass(w.t_lo, w.w_lo);
 #pragma nounroll
-    for (int t = w.t_lo; t <= w.t_hi; ++t) {
+    for (; t <= w.w_hi; ++t) {
         copies_landed();
         char* keys = w.keys(t & 1);
         const char* values = w.values(t & 1);
@@ -542,6 +557,8 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_q_kernel(
                 for (int u = 0; u < 2; ++u) dq[db] = mfma(T::cols(keys, cols_lane, db, 2 * rb + u), dsf[u], dq[db]);
         }
     }
+    w.pass(t, INT_MAX);
+
     bool fine = true;
 #pragma unroll
     for (int db = 0; db < W::kDims; ++db) fine &= all_finite(dq[db]);
