@@ -405,16 +405,13 @@ def adamw_update(params, grads, m, v, learning_rate, beta1, beta2, t, eps, weigh
 def _launch_context(stream, *tensors):
     """(context, stream handle) for a call on `tensors`, which must share a device: the call runs on that device, on
     `stream` or the device's current stream, whatever the current device is."""
-    dev = None
+    dev = tensors[0].get_device()
     for t in tensors:
-        if t is None:
-            continue
-        if dev is not None and t.device != dev:
-            raise ValueError("all tensors must be on one device (got %s and %s)" % (dev, t.device))
-        dev = t.device
-    ctx = contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+        if t is not None and t.get_device() != dev:
+            raise ValueError("all tensors must be on one device (got devices %d and %d)" % (dev, t.get_device()))
+    ctx = contextlib.nullcontext() if dev == torch.cuda.current_device() else torch.cuda.device(dev)
     # the handle itself: building a Stream object for it takes 2.6 us, a quarter of a short call
-    return ctx, stream if stream else torch._C._cuda_getCurrentRawStream(dev.index)
+    return ctx, stream if stream else torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _attention_dims(qkv, per_query, Nq, Nkv, first_key, softmax_scale):

@@ -199,7 +199,10 @@ def test_values_that_are_not_finite_reach_what_they_enter_and_nothing_else(K, sh
             dout.view(B, T, Nq, HD)[0, 80, Nq - 1, 5] = value
         else:
             qkv.view(B, T, -1, HD)[0, 80, at[name], 5] = value
-        out, lse = forward(K, qkv, Nq, Nkv, first)
+        am, ref = torch.full((1,), 9e9, device="cuda"), torch.zeros(1, device="cuda")
+        out, lse = forward(K, qkv, Nq, Nkv, first, None, am)
+        K.abs_max(ref, out)
+        assert torch.equal(am, ref)
         dqkv = backward(K, qkv, dout, out, lse, Nq, Nkv, first)
         want, grad = by_rows(qkv, dout, out, Nq, Nkv, first)
         assert torch.equal(torch.isfinite(out), torch.isfinite(want)), name

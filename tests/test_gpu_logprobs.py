@@ -286,7 +286,7 @@ def test_results_repeat_and_streams_and_graphs_agree(K):
 
 def test_logits_of_more_than_four_gibibytes(K):
     """The last rows of logits that pass 2^32 bytes equal the same rows alone, bit for bit (a row is summed by one workgroup from
-    512 rows on)."""
+    256 rows on)."""
     N, V, tail = 15000, 151936, 600
     x = torch.zeros((N, V), dtype=torch.bfloat16, device="cuda")
     part, t1 = make(tail, V, V, torch.bfloat16)
