@@ -876,31 +876,41 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_kernel
     }
 }
 
-// Share `split` of the elements of keys kb0 ..: a lane takes four values of each split at a time, four such groups in flight.
-template <int KEYS, int THREADS>
+// Share `split` of the elements of keys kb0 ..: a lane takes four values of each split at a time, kFlight such groups of kSplits
+// splits on their way at once.
+template <int KEYS, int THREADS, int kFlight, int kSplits>
 __device__ __forceinline__ void join_splits(const AttentionArgs& a, int group, int kb0, int split) {
     const int per = 2 * a.head_dim / 4, n = min(KEYS, a.T - kb0) * per, step = a.splits * THREADS;
     const int b = group / a.Nkv, kvh = group % a.Nkv;
     const int64_t all = (int64_t)a.B * a.T * a.Nkv * per, token = (int64_t)(a.Nq + 2 * a.Nkv) * a.head_dim;
     const float4* first = reinterpret_cast<const float4*>(a.partial) + (((int64_t)b * a.T + kb0) * a.Nkv + kvh) * per;
     uint16_t* rows = a.dqkv + ((int64_t)b * a.T + kb0) * token + (int64_t)(a.Nq + kvh) * a.head_dim;
-    for (int i = split * THREADS + threadIdx.x; i < n; i += 4 * step) {
-        int key[4], at[4];
-        float4 x[4];
+    for (int i = split * THREADS + threadIdx.x; i < n; i += kFlight * step) {
+        int key[kFlight], at[kFlight];
+        const float4* from[kFlight];
+        float4 x[kFlight];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < kFlight; ++u) {
             const int j = min(i + u * step, n - 1);
             key[u] = j / per, at[u] = j % per;
+            from[u] = first + (int64_t)key[u] * a.Nkv * per + at[u];
             x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        for (int s = 0; s < a.splits; ++s)
+        for (int s = 0; s < a.splits; s += kSplits) {
+            float4 y[kSplits][kFlight];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const float4 y = first[s * all + (int64_t)key[u] * a.Nkv * per + at[u]];
-                x[u].x += y.x, x[u].y += y.y, x[u].z += y.z, x[u].w += y.w;
-            }
+            for (int p = 0; p < kSplits; ++p)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+                for (int u = 0; u < kFlight; ++u) y[p][u] = from[u][min(s + p, a.splits - 1) * all];
+#pragma unroll
+            for (int p = 0; p < kSplits; ++p)
+                if (s + p < a.splits) {
+#pragma unroll
+                    for (int u = 0; u < kFlight; ++u) x[u].x += y[p][u].x, x[u].y += y[p][u].y, x[u].z += y[p][u].z, x[u].w += y[p][u].w;
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < kFlight; ++u) {
             if (i + u * step >= n) break;
             const bool value = 4 * at[u] >= a.head_dim;
             const float f = value ? 1.f : a.scale;
@@ -922,7 +932,12 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_join_kern
     int again = 0;
     for (int s = 0; s < a.splits; ++s) again |= a.flags[(rest - split + s) * groups + group];
     if (!again) {
-        if (a.splits > 1) join_splits<W::kBlock, W::kThreads>(a, group, kb0, split);
+        // Where a lane has no more than one group, it asks for that group's splits at once: 1 x 40 20.3 -> 18 us, 2 x 129 27.2 -> 25.2,
+        // but 8 x 1024, with many groups a lane, 327 -> 340.
+        if (a.splits > 1) {
+            if (min(W::kBlock, a.T - kb0) * (a.head_dim / 2) <= a.splits * W::kThreads) join_splits<W::kBlock, W::kThreads, 1, 16>(a, group, kb0, split);
+            else join_splits<W::kBlock, W::kThreads, 4, 4>(a, group, kb0, split);
+        }
         return;
     }
     if (split > 0) return;
@@ -982,14 +997,13 @@ static int check_shape(const char* what, int B, int T, int Nq, int Nkv, int head
 // eight, which read the queries half as often as four: 1 x 8192 1925 -> 1640 us, documents 283 -> 214, but 8 x 1024 331 -> 340.
 static int kv_block(int head_dim) { return head_dim > 64 ? 256 : 128; }
 
-// Shares of the walk over the queries: enough workgroups for two per compute unit, each with four pairs of work at least
-// (one per unit: 1 x 8192 2180 us, 8 x 1024 370; three: 1710 and 369.  Eight pairs: 1 x 40 20.5 -> 24.4 us; two: 19.5, but
-// 2 x 129 27.6 -> 28.4).
+// Shares of the walk over the queries: enough workgroups for two per compute unit (one per unit: 1 x 8192 2180 us, 8 x 1024 370;
+// three: 1710 and 369), each with a pair at least (two: 1 x 40 17 -> 18 us, four: 20.3).
 static int kv_splits(int B, int T, int Nq, int Nkv, int keys) {
     const int64_t blocks = (int64_t)B * Nkv * ((T + keys - 1) / keys);
     const int64_t pairs = (int64_t)((T + kQueries - 1) / kQueries) * (Nq / Nkv);
     int64_t s = (2 * kUnits + blocks - 1) / blocks;
-    if (s > (pairs + 3) / 4) s = (pairs + 3) / 4;
+    if (s > pairs) s = pairs;
     return (int)(s < 1 ? 1 : s > 16 ? 16 : s);
 }
 
