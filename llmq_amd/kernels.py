@@ -30,8 +30,6 @@ Names, argument order and in-place "out first" convention are the reference's:
     get_token_logprobs_scratch_size(N, V, k)
 `stream` is a raw hipStream_t handle (0 = torch's current stream).
 """
-import contextlib
-
 import torch
 
 from . import capi
@@ -402,29 +400,35 @@ def adamw_update(params, grads, m, v, learning_rate, beta1, beta2, t, eps, weigh
                                                float(weight_decay), gs, a, int(seed) & 0xFFFFFFFF, _stream(stream)))
 
 
-def _launch_context(stream, *tensors):
-    """(context, stream handle) for a call on `tensors`, which must share a device: the call runs on that device, on
-    `stream` or the device's current stream, whatever the current device is."""
+def _launch(fn, args, stream, tensors):
+    """fn(*args, stream handle) on the device of `tensors`, which must share one: on `stream` or that device's current stream,
+    whatever the current device is."""
     dev = tensors[0].get_device()
     for t in tensors:
         if t is not None and t.get_device() != dev:
             raise ValueError("all tensors must be on one device (got devices %d and %d)" % (dev, t.get_device()))
-    ctx = contextlib.nullcontext() if dev == torch.cuda.current_device() else torch.cuda.device(dev)
-    # the handle itself: building a Stream object for it takes 2.6 us, a quarter of a short call
-    return ctx, stream if stream else torch._C._cuda_getCurrentRawStream(dev)
+    if not stream:
+        # the handle itself: building a Stream object for it takes 2.6 us, a quarter of a short call
+        stream = torch._C._cuda_getCurrentRawStream(dev)
+    if dev == torch.cuda.current_device():
+        capi.check(fn(*args, stream))
+    else:
+        with torch.cuda.device(dev):
+            capi.check(fn(*args, stream))
 
 
 def _attention_dims(qkv, per_query, Nq, Nkv, first_key, softmax_scale):
-    """(B, T, head_dim, scale) of qkv [B, T, (Nq + 2 Nkv) HD]; per_query: name -> tensor [B, T, Nq HD]."""
+    """(B, T, head_dim, scale) of qkv [B, T, (Nq + 2 Nkv) HD]; per_query: (name, tensor [B, T, Nq HD])."""
     if qkv.dim() != 3:
         raise ValueError("qkv must be [B, T, (Nq + 2 Nkv) * head_dim]")
-    if Nq <= 0 or Nkv <= 0 or Nq % Nkv or qkv.shape[2] % (Nq + 2 * Nkv):
+    B, T, C = qkv.shape
+    if Nq <= 0 or Nkv <= 0 or Nq % Nkv or C % (Nq + 2 * Nkv):
         raise ValueError("qkv must be [B, T, (Nq + 2 Nkv) * head_dim] with Nq a multiple of Nkv")
-    B, T, HD = int(qkv.shape[0]), int(qkv.shape[1]), int(qkv.shape[2]) // (Nq + 2 * Nkv)
-    for name, t in per_query.items():
-        if tuple(t.shape) != (B, T, Nq * HD):
+    HD = C // (Nq + 2 * Nkv)
+    for name, t in per_query:
+        if t.shape != (B, T, Nq * HD):
             raise ValueError("%s must be [B, T, Nq * head_dim]" % name)
-    if first_key is not None and tuple(first_key.shape) != (B, T):
+    if first_key is not None and first_key.shape != (B, T):
         raise ValueError("first_key must be [B, T]")
     return B, T, HD, float(softmax_scale) if softmax_scale is not None else max(HD, 1) ** -0.5
 
@@ -435,16 +439,15 @@ def attention_forward(out, lse, qkv, abs_max, Nq, Nkv, first_key=None, softmax_s
     max(0, first_key[b, t]) .. t (first_key: int32 [B, T] or None for 0): the document's first token for packed documents,
     t - w + 1 for a sliding window, any value above t for a row that looks at nothing (out 0, lse -inf).
     softmax_scale: 1 / sqrt(HD) unless given.  HD: a multiple of 8 up to 128."""
-    B, T, HD, scale = _attention_dims(qkv, {"out": out}, Nq, Nkv, first_key, softmax_scale)
-    if tuple(lse.shape) != (B, Nq, T):
+    B, T, HD, scale = _attention_dims(qkv, (("out", out),), Nq, Nkv, first_key, softmax_scale)
+    if lse.shape != (B, Nq, T):
         raise ValueError("lse must be [B, Nq, T]")
     bf, f32 = (torch.bfloat16,), (torch.float32,)
     o, l, x = _dev(out, "out", bf), _dev(lse, "lse", f32), _dev(qkv, "qkv", bf)
     f = _dev(first_key, "first_key", (torch.int32,), optional=True)
     a = _dev(abs_max, "abs_max", f32, optional=True)
-    ctx, st = _launch_context(stream, qkv, out, lse, first_key, abs_max)
-    with ctx:
-        capi.check(capi.lib.llmq_attention_forward_bf16(o, l, x, f, a, scale, B, T, int(Nq), int(Nkv), HD, st))
+    _launch(capi.lib.llmq_attention_forward_bf16, (o, l, x, f, a, scale, B, T, int(Nq), int(Nkv), HD), stream,
+            (qkv, out, lse, first_key, abs_max))
 
 
 def get_attention_backward_scratch_size(B, T, Nq, Nkv, HD):
@@ -456,33 +459,32 @@ def attention_backward(dqkv, dout, out, lse, qkv, scratch, Nq, Nkv, first_key=No
     """Gradient of attention_forward: dqkv (shape of qkv, every element written) from dout and the forward's out, lse, qkv,
     first_key and softmax_scale.  scratch: a device tensor of at least get_attention_backward_scratch_size(B, T, Nq, Nkv, HD)
     bytes; calls that share it must be stream ordered.  Deterministic."""
-    B, T, HD, scale = _attention_dims(qkv, {"out": out, "dout": dout}, Nq, Nkv, first_key, softmax_scale)
+    B, T, HD, scale = _attention_dims(qkv, (("out", out), ("dout", dout)), Nq, Nkv, first_key, softmax_scale)
     if dqkv.shape != qkv.shape:
         raise ValueError("dqkv must have the shape of qkv")
-    if tuple(lse.shape) != (B, Nq, T):
+    if lse.shape != (B, Nq, T):
         raise ValueError("lse must be [B, Nq, T]")
     bf, f32 = (torch.bfloat16,), (torch.float32,)
     d, g, o, x = _dev(dqkv, "dqkv", bf), _dev(dout, "dout", bf), _dev(out, "out", bf), _dev(qkv, "qkv", bf)
     l = _dev(lse, "lse", f32)
     f = _dev(first_key, "first_key", (torch.int32,), optional=True)
     s = _dev(scratch, "scratch")
-    ctx, st = _launch_context(stream, qkv, dqkv, dout, out, lse, first_key, scratch)
-    with ctx:
-        capi.check(capi.lib.llmq_attention_backward_bf16(d, g, o, l, x, f, s, scratch.numel() * scratch.element_size(), scale, B, T,
-                                                         int(Nq), int(Nkv), HD, st))
+    _launch(capi.lib.llmq_attention_backward_bf16,
+            (d, g, o, l, x, f, s, scratch.numel() * scratch.element_size(), scale, B, T, int(Nq), int(Nkv), HD), stream,
+            (qkv, dqkv, dout, out, lse, first_key, scratch))
 
 
 def _logprob_dims(logits, per_row, vocab):
-    """(rows, vocabulary, row length) of logits [..., P]; per_row: name -> tensor of one value a row (or None)."""
+    """(rows, vocabulary, row length) of logits [..., P]; per_row: (name, tensor of one value a row or None)."""
     if logits.dim() < 2:
         raise ValueError("logits must be [..., P]")
     P = int(logits.shape[-1])
     V = P if vocab is None else int(vocab)
     if not 1 <= V <= P:
         raise ValueError("vocab must lie between 1 and the row length %d (got %d)" % (P, V))
-    lead = tuple(logits.shape[:-1])
-    for name, t in per_row.items():
-        if t is not None and tuple(t.shape) != lead:
+    lead = logits.shape[:-1]
+    for name, t in per_row:
+        if t is not None and t.shape != lead:
             raise ValueError("%s must have one value for each row of logits" % name)
     return logits.numel() // P, V, P
 
@@ -497,30 +499,28 @@ def token_logprobs(logp, entropy, lse, top_logp, top_ids, logits, targets, scrat
     lse [...] fp32, and the k most likely tokens of each row in falling order, top_logp [..., k] fp32 and top_ids [..., k] int32
     (both None: not wanted; k <= 32; equal logits by token).  vocab: the columns that count (P unless given).  A target outside
     [0, vocab) is ignored (logp 0).  scratch: device tensor of get_token_logprobs_scratch_size bytes, or None if that is 0."""
-    N, V, P = _logprob_dims(logits, {"logp": logp, "entropy": entropy, "lse": lse, "targets": targets}, vocab)
+    N, V, P = _logprob_dims(logits, (("logp", logp), ("entropy", entropy), ("lse", lse), ("targets", targets)), vocab)
     if (top_logp is None) != (top_ids is None):
         raise ValueError("top_logp and top_ids go together")
     k = 0
     if top_ids is not None:
-        k = int(top_ids.shape[-1])
-        if top_ids.shape != top_logp.shape or tuple(top_ids.shape[:-1]) != tuple(logits.shape[:-1]):
+        if top_ids.dim() == 0 or top_ids.shape != top_logp.shape or top_ids.shape[:-1] != logits.shape[:-1]:
             raise ValueError("top_logp and top_ids must be [..., k]")
+        k = int(top_ids.shape[-1])
     fn, dt = _producer_entry("token_logprobs", logits)
     f32, i32 = (torch.float32,), (torch.int32,)
     p = [_dev(logp, "logp", f32), _dev(entropy, "entropy", f32, optional=True), _dev(lse, "lse", f32),
          _dev(top_logp, "top_logp", f32, optional=True), _dev(top_ids, "top_ids", i32, optional=True), _dev(logits, "logits", dt),
          _dev(targets, "targets", i32), _dev(scratch, "scratch", optional=True)]
     size = 0 if scratch is None else scratch.numel() * scratch.element_size()
-    ctx, st = _launch_context(stream, logits, logp, entropy, lse, top_logp, top_ids, targets, scratch)
-    with ctx:
-        capi.check(fn(*p, size, N, V, P, k, st))
+    _launch(fn, (*p, size, N, V, P, k), stream, (logits, logp, entropy, lse, top_logp, top_ids, targets, scratch))
 
 
 def token_logprobs_backward(dlogits, dlogp, dentropy, logits, targets, lse, entropy, abs_max, vocab=None, stream=0):
     """dlogits (shape and type of logits; may be logits itself) from dlogp [...] and dentropy [...] (or None), with the forward's
     lse and, for dentropy, entropy; abs_max (fp32 device scalar or None) receives max |dlogits|.  Columns from vocab on are
     written as zeros."""
-    N, V, P = _logprob_dims(logits, {"dlogp": dlogp, "dentropy": dentropy, "targets": targets, "lse": lse, "entropy": entropy}, vocab)
+    N, V, P = _logprob_dims(logits, (("dlogp", dlogp), ("dentropy", dentropy), ("targets", targets), ("lse", lse), ("entropy", entropy)), vocab)
     if dlogits.shape != logits.shape:
         raise ValueError("dlogits must have the shape of logits")
     if dentropy is not None and entropy is None:
@@ -530,6 +530,4 @@ def token_logprobs_backward(dlogits, dlogp, dentropy, logits, targets, lse, entr
     p = [_dev(dlogits, "dlogits", dt), _dev(dlogp, "dlogp", f32), _dev(dentropy, "dentropy", f32, optional=True),
          _dev(logits, "logits", dt), _dev(targets, "targets", (torch.int32,)), _dev(lse, "lse", f32),
          _dev(entropy, "entropy", f32, optional=True), _dev(abs_max, "abs_max", f32, optional=True)]
-    ctx, st = _launch_context(stream, logits, dlogits, dlogp, dentropy, targets, lse, entropy, abs_max)
-    with ctx:
-        capi.check(fn(*p, N, V, P, st))
+    _launch(fn, (*p, N, V, P), stream, (logits, dlogits, dlogp, dentropy, targets, lse, entropy, abs_max))
