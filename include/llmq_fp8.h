@@ -423,8 +423,9 @@ int llmq_adamw_update_f32(float* params, const float* grads, float* m, float* v,
  * A row without keys: out = 0, lse = -inf.  Scores and sums in fp32; the probabilities are rounded to bf16 for the product
  * with the values.  What lies in places the mask excludes never reaches a result, NaN and infinities included; where a value in
  * an allowed place is not finite, the outputs it enters are not finite either (NaN, also where the formula gives an infinity).
+ * A score of -inf has probability 0, and a row of nothing else counts as one without keys (its gradients are NaN).
  * abs_max_or_null: reset, then max |out|, bit-identical to llmq_abs_max_bf16(out).  head_dim: a multiple of 8 up to 128;
- * softmax_scale > 0.  out must not be qkv.
+ * softmax_scale > 0.  out and lse share no memory with each other and with qkv.
  */
 int llmq_attention_forward_bf16(uint16_t* out, float* lse, const uint16_t* qkv, const int* first_key_or_null,
                                 float* abs_max_or_null, float softmax_scale, int B, int T, int Nq, int Nkv, int head_dim,
@@ -437,7 +438,7 @@ int llmq_attention_forward_bf16(uint16_t* out, float* lse, const uint16_t* qkv, 
  * (sums of dk, dv over the query heads of the group).  p and ds are rounded to bf16 for their products, sums are fp32 in a
  * fixed order (deterministic), every element of dqkv is written.  Masked places as in the forward pass.
  * scratch: at least llmq_attention_backward_scratch_bytes(B, T, Nq, Nkv, head_dim) bytes, 16-byte aligned, overwritten by every
- * call; calls that share it must be stream ordered.  dqkv must be a tensor of its own.
+ * call; calls that share it must be stream ordered.  dqkv and the scratch share no memory with each other and the inputs.
  */
 int64_t llmq_attention_backward_scratch_bytes(int B, int T, int Nq, int Nkv, int head_dim);
 int llmq_attention_backward_bf16(uint16_t* dqkv, const uint16_t* dout, const uint16_t* out, const float* lse,
@@ -471,7 +472,7 @@ int llmq_token_logprobs_f32(float* logp, float* entropy_or_null, float* lse, flo
  * rounded once; columns V .. P-1 are written as zeros.  lse (and, with dentropy, entropy) are the forward's.  dlogp counts as 0
  * for an ignored row; a row whose two gradients are 0 is written as zeros whatever its logits hold (padding), and so is a row
  * whose lse is -inf.
- * dlogits may be logits (in place).  abs_max_or_null: reset, then max |dlogits| over all columns, bit-identical to llmq_abs_max
+ * dlogits may be logits (in place), but not otherwise overlap them.  abs_max_or_null: reset, then max |dlogits| over all columns, bit-identical to llmq_abs_max
  * of the tensor.  The loss -mean logp has dlogp = -1 / N.
  */
 int llmq_token_logprobs_backward_bf16(uint16_t* dlogits, const float* dlogp, const float* dentropy_or_null,

@@ -20,6 +20,7 @@
 // costs besides its walk: at 8 x 1024 (82 us, 0.73 PFLOP/s) 5 of its 23 us, and an eighth of the walk lies behind the diagonal.
 #include <climits>
 #include <type_traits>
+#include <utility>
 
 #include "common.hpp"
 #include "absmax_reduce.hpp"
@@ -987,10 +988,15 @@ static int check_shape(const char* what, int B, int T, int Nq, int Nkv, int head
     LLMQ_REQUIRE(head_dim >= 8 && head_dim <= 128 && head_dim % 8 == 0, "%s: head_dim must be a multiple of 8 from 8 to 128 (got %d)", what, head_dim);
     LLMQ_REQUIRE((int64_t)Nq + 2 * (int64_t)Nkv <= 65536, "%s: too many heads", what);
     LLMQ_REQUIRE(T <= (1 << 30), "%s: sequence too long", what);
-    // the grid's threads (256 for 128 queries of a head) fit 32 bits
-    LLMQ_REQUIRE((int64_t)B * T <= 0x7FFFFFFF && (int64_t)B * Nq <= INT_MAX && (int64_t)B * Nq * ((T + 127) / 128) < (1 << 24),
+    // the grids' threads (512 for 128 positions of a head at most) fit 32 bits
+    LLMQ_REQUIRE((int64_t)B * T <= 0x7FFFFFFF && (int64_t)B * Nq <= INT_MAX && (int64_t)B * Nq * ((T + 127) / 128) < (1 << 23),
                  "%s: tensor too large", what);
     return LLMQ_OK;
+}
+
+// whether two ranges of memory have nothing in common
+static bool apart(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+    return static_cast<const char*>(a) + a_bytes <= static_cast<const char*>(b) || static_cast<const char*>(b) + b_bytes <= static_cast<const char*>(a);
 }
 
 // Keys of a workgroup of the keys' kernel: as many waves as copy a tile of 32 queries with one load a thread.  Above 64 dimensions
@@ -1049,7 +1055,9 @@ extern "C" int llmq_attention_forward_bf16(uint16_t* out, float* lse, const uint
     if (some) {
         LLMQ_REQUIRE(out && lse && qkv, "%s: null tensor pointer", what);
         LLMQ_REQUIRE(aligned16(out) && aligned16(qkv), "%s: pointers must be 16-byte aligned", what);
-        LLMQ_REQUIRE(out != qkv, "%s: out must not be qkv", what);
+        const int64_t rows = (int64_t)B * T * head_dim * 2, all = rows * (Nq + 2 * Nkv), stat = (int64_t)B * T * Nq * 4;
+        LLMQ_REQUIRE(apart(out, rows * Nq, qkv, all) && apart(lse, stat, qkv, all) && apart(out, rows * Nq, lse, stat),
+                     "%s: out and lse must be memory of their own", what);
     }
     if (abs_max_or_null) {
         hipLaunchKernelGGL(reset_slot_kernel, dim3(1), dim3(1), 0, st, reinterpret_cast<unsigned*>(abs_max_or_null));
@@ -1068,7 +1076,7 @@ extern "C" int llmq_attention_forward_bf16(uint16_t* out, float* lse, const uint
 }
 
 extern "C" int64_t llmq_attention_backward_scratch_bytes(int B, int T, int Nq, int Nkv, int head_dim) {
-    if (B <= 0 || T <= 0 || Nq <= 0 || Nkv <= 0 || Nq % Nkv || head_dim <= 0) return 0;
+    if (B <= 0 || T <= 0 || check_shape("attention_backward", B, T, Nq, Nkv, head_dim)) return 0;
     return backward_plan(B, T, Nq, Nkv, head_dim).bytes;
 }
 
@@ -1082,9 +1090,13 @@ extern "C" int llmq_attention_backward_bf16(uint16_t* dqkv, const uint16_t* dout
     LLMQ_REQUIRE(dqkv && dout && out && lse && qkv && scratch, "%s: null tensor pointer", what);
     LLMQ_REQUIRE(aligned16(dqkv) && aligned16(dout) && aligned16(out) && aligned16(qkv) && aligned16(scratch),
                  "%s: pointers must be 16-byte aligned", what);
-    LLMQ_REQUIRE(dqkv != qkv && dqkv != dout && dqkv != out, "%s: dqkv must be a tensor of its own", what);
+    const int64_t rows = (int64_t)B * T * head_dim * 2, all = rows * (Nq + 2 * Nkv), stat = (int64_t)B * T * Nq * 4;
     const BackwardPlan p = backward_plan(B, T, Nq, Nkv, head_dim);
     LLMQ_REQUIRE(scratch_bytes >= (size_t)p.bytes, "%s: scratch buffer too small (%zu bytes, %lld needed)", what, scratch_bytes, (long long)p.bytes);
+    for (const auto& to : {std::pair<const void*, int64_t>{dqkv, all}, {scratch, p.bytes}})
+        LLMQ_REQUIRE(apart(to.first, to.second, qkv, all) && apart(to.first, to.second, dout, rows * Nq) && apart(to.first, to.second, out, rows * Nq) &&
+                         apart(to.first, to.second, lse, stat) && (to.first == dqkv || apart(to.first, to.second, dqkv, all)),
+                     "%s: dqkv and the scratch must be memory of their own", what);
     hipStream_t st = static_cast<hipStream_t>(stream);
     AttentionArgs a = make_args(qkv, first_key_or_null, B, T, Nq, Nkv, head_dim, softmax_scale);
     a.out = const_cast<uint16_t*>(out), a.lse = const_cast<float*>(lse), a.dout = dout, a.dqkv = dqkv;

@@ -615,6 +615,7 @@ static int token_logprobs_backward_any(E* dlogits, const float* dlogp, const flo
     if (N64 > 0) {
         LLMQ_REQUIRE(dlogits && dlogp && logits && targets && lse, "%s: null tensor pointer", what);
         LLMQ_REQUIRE(aligned16(dlogits) && aligned16(logits), "%s: pointers must be 16-byte aligned", what);
+        LLMQ_REQUIRE(dlogits == logits || dlogits + N64 * P <= logits || logits + N64 * P <= dlogits, "%s: dlogits must be logits or memory of its own", what);
     }
     if (abs_max) {
         hipLaunchKernelGGL(reset_slot_kernel, dim3(1), dim3(1), 0, stream, reinterpret_cast<unsigned*>(abs_max));

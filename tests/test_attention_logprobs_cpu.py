@@ -14,7 +14,7 @@ def capi():
 
 @pytest.fixture(scope="module")
 def p():
-    buf = (C.c_char * 4096)()
+    buf = (C.c_char * (1 << 20))()   # never read: every call below is refused or empty
     p.buf = buf
     return (C.addressof(buf) + 15) & ~15
 
@@ -22,10 +22,11 @@ def p():
 def test_attention_forward_refuses(capi, p):
     f = capi.lib.llmq_attention_forward_bf16
 
-    def rc(out=p, lse=p + 64, qkv=p + 128, first=None, am=None, scale=0.125, B=1, T=8, Nq=4, Nkv=2, HD=64):
+    def rc(out=p, lse=p + 8192, qkv=p + 16384, first=None, am=None, scale=0.125, B=1, T=8, Nq=4, Nkv=2, HD=64):
         return f(out, lse, qkv, first, am, scale, B, T, Nq, Nkv, HD, None)
 
-    bad = [dict(out=None), dict(lse=None), dict(qkv=None), dict(out=p + 2), dict(qkv=p + 8), dict(out=p + 128), dict(scale=0.0), dict(scale=-1.0),
+    bad = [dict(out=None), dict(lse=None), dict(qkv=None), dict(out=p + 2), dict(qkv=p + 8), dict(out=p + 16384), dict(out=p + 24560),
+           dict(out=p + 12320), dict(lse=p + 4080), dict(lse=p + 16380), dict(scale=0.0), dict(scale=-1.0),
            dict(scale=float("nan")), dict(scale=float("inf")), dict(B=-1), dict(T=-1), dict(Nq=0), dict(Nkv=0), dict(Nq=5), dict(Nkv=-2), dict(HD=0),
            dict(HD=4), dict(HD=12), dict(HD=136), dict(HD=-64), dict(Nq=65536, Nkv=1), dict(T=(1 << 30) + 1), dict(B=1 << 20, T=1 << 20),
            dict(B=1 << 20, Nq=32, Nkv=1)]
@@ -41,11 +42,14 @@ def test_attention_backward_refuses(capi, p):
     need = capi.lib.llmq_attention_backward_scratch_bytes(1, 8, 4, 2, 64)
     assert need > 0
 
-    def rc(d=p, dout=p + 64, out=p + 128, lse=p + 192, qkv=p + 256, first=None, s=p + 512, n=need, scale=0.125, B=1, T=8, Nq=4, Nkv=2, HD=64):
+    k = 8192   # bytes of dqkv and qkv: 8 tokens of 8 heads of 64
+
+    def rc(d=p, dout=p + k, out=p + 2 * k, lse=p + 3 * k, qkv=p + 4 * k, first=None, s=p + 5 * k, n=need, scale=0.125, B=1, T=8, Nq=4, Nkv=2, HD=64):
         return f(d, dout, out, lse, qkv, first, s, n, scale, B, T, Nq, Nkv, HD, None)
 
     bad = [dict(d=None), dict(dout=None), dict(out=None), dict(lse=None), dict(qkv=None), dict(s=None), dict(d=p + 2), dict(dout=p + 68), dict(out=p + 130),
-           dict(qkv=p + 258), dict(s=p + 520), dict(n=need - 1), dict(n=0), dict(d=p + 256), dict(d=p + 64), dict(d=p + 128), dict(scale=0.0),
+           dict(qkv=p + 258), dict(s=p + 520), dict(n=need - 1), dict(n=0), dict(d=p + 4 * k), dict(d=p + 16), dict(d=p + 2 * k - 16),
+           dict(d=p + 2 * k), dict(d=p + 3 * k - 16), dict(s=p + 4 * k), dict(s=p + 5 * k - 16), dict(s=p), dict(s=p + k - 16), dict(scale=0.0),
            dict(scale=float("nan")), dict(B=-1), dict(Nq=5), dict(HD=12), dict(HD=136)]
     for a in bad:
         assert rc(**a) == capi.LLMQ_ERR_INVALID_ARGUMENT, a
@@ -83,7 +87,7 @@ def test_token_logprobs_refuse(capi, p, ty):
     def rcb(d=p, g=p, h=None, x=p, t=p, lse=p, ent=None, am=None, N=1, V=64, P=64):
         return b(d, g, h, x, t, lse, ent, am, N, V, P, None)
 
-    bad = [dict(d=None), dict(g=None), dict(x=None), dict(t=None), dict(lse=None), dict(h=p), dict(d=p + 2), dict(x=p + 2), dict(N=-1), dict(N=1 << 24),
+    bad = [dict(d=None), dict(g=None), dict(x=None), dict(t=None), dict(lse=None), dict(h=p), dict(d=p + 2), dict(x=p + 2), dict(d=p + 16), dict(N=-1), dict(N=1 << 24),
            dict(V=0), dict(V=65), dict(P=(1 << 28) + 1), dict(N=(1 << 24) - 1, P=1 << 20)]
     for a in bad:
         assert rcb(**a) == capi.LLMQ_ERR_INVALID_ARGUMENT, a

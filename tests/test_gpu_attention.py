@@ -230,6 +230,15 @@ def test_padding_may_hold_anything(K, shape, value):
     assert ((dqkv.double() - e["grad"]).abs() <= e["bar_grad"] + 1e-30).all() and (dqkv[:, :33] == 0).all()
 
 
+def test_rows_whose_scores_are_all_minus_infinity(K):
+    qkv, _ = make(1, 3, 2, 1, 64)
+    qkv.view(3, 4, 64)[:, :2, 0] = 1.0
+    qkv.view(3, 4, 64)[:2, 2, 0] = -math.inf
+    out, lse = forward(K, qkv, 2, 1)
+    assert (out[0, :2] == 0).all() and (lse[0, :, :2] == -math.inf).all()
+    assert torch.equal(out.view(3, 2, 64)[2], qkv.view(3, 4, 64)[2, 3:].expand(2, 64)) and torch.isfinite(lse[0, :, 2]).all()
+
+
 def test_gradient_against_differences(K):
     """The loss sum(dout out) of the formulas in 64 bits, stepped along random directions; the kernel's gradient is off by its bars."""
     B, T, Nq, Nkv, HD = 1, 70, 4, 2, 64
