@@ -17,7 +17,7 @@
 //
 // The k most likely tokens need no second pass over the row.  In the first turns (about the square root of all of a lane's
 // turns) each lane keeps the largest logit of its granules of 16 bytes and the first granule that holds it.  The k-th best of
-// the lanes' (value, granule) pairs bounds the k-th best logit from below, and of these turns only the k lanes that reach it can
+// such (value, granule) pairs bounds the k-th best logit from below, and of these turns only the lanes that reach it can
 // hold one of the k.  From then on every granule with a logit above the bound is listed.  Those granules alone, of some hundreds
 // of turns a few hundred, are read again, from the caches; a full re-read of the k best lanes was 20 % of the time at k = 20.
 // Where the list overflows (logits that rise along the row) the lanes' best are taken over the whole row instead, and where that
@@ -142,7 +142,45 @@ __device__ __forceinline__ Sums join(const Sums& a, const Sums& b) {
     return c;
 }
 
+// f over the 64 lanes of a wave, the same in every lane: exchanges inside a row of 16, then of rows and of halves.  All lanes are
+// active.  (Through LDS, as shuffles go, each of the six steps took three times as long.)
+template <int CTRL>
+__device__ __forceinline__ uint32_t across(uint32_t x) { return __builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, true); }
+template <typename F>
+__device__ __forceinline__ uint64_t wave_fold(uint64_t x, F f) {
+    auto word = [](uint32_t lo, uint32_t hi) { return (uint64_t)hi << 32 | lo; };
+    const auto lo = [](uint64_t v) { return (uint32_t)v; };
+    const auto hi = [](uint64_t v) { return (uint32_t)(v >> 32); };
+    x = f(x, word(across<0xB1>(lo(x)), across<0xB1>(hi(x))));      // quad_perm 1 0 3 2
+    x = f(x, word(across<0x4E>(lo(x)), across<0x4E>(hi(x))));      // quad_perm 2 3 0 1
+    x = f(x, word(across<0x141>(lo(x)), across<0x141>(hi(x))));    // row_half_mirror
+    x = f(x, word(across<0x140>(lo(x)), across<0x140>(hi(x))));    // row_mirror
+    const auto a = __builtin_amdgcn_permlane16_swap(lo(x), lo(x), false, false), b = __builtin_amdgcn_permlane16_swap(hi(x), hi(x), false, false);
+    x = f(word(a[0], b[0]), word(a[1], b[1]));
+    const auto c = __builtin_amdgcn_permlane32_swap(lo(x), lo(x), false, false), d = __builtin_amdgcn_permlane32_swap(hi(x), hi(x), false, false);
+    return f(word(c[0], d[0]), word(c[1], d[1]));
+}
+template <typename F>
+__device__ __forceinline__ float wave_fold(float x, F f) {
+    return __uint_as_float((uint32_t)wave_fold((uint64_t)__float_as_uint(x), [&](uint64_t a, uint64_t b) {
+        return (uint64_t)__float_as_uint(f(__uint_as_float((uint32_t)a), __uint_as_float((uint32_t)b)));
+    }));
+}
+// the lanes' sums as one, against their common reference
+__device__ __forceinline__ Sums wave_join(const Sums& t) {
+    Sums c;
+    c.r = wave_fold(t.r, [](float a, float b) { return __builtin_fmaxf(a, b); });
+    const float ref = c.r == -__builtin_huge_valf() ? 0.f : c.r;
+    const float d = __builtin_fmaxf((t.r - ref) * kLog2eLp, -1e4f), f = __builtin_amdgcn_exp2f(d);
+    auto add = [](float a, float b) { return a + b; };
+    c.s = wave_fold(t.s * f, add);
+    c.w = wave_fold((t.w + d * t.s) * f, add);
+    return c;
+}
+
 __device__ __forceinline__ float lse_of(const Sums& t) { return t.s == 0.f ? -__builtin_huge_valf() : t.r + __builtin_amdgcn_logf(t.s) * kLn2Lp; }
+
+__device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
 // How many of n keys in LDS are larger than `key`.  n even, the list 16-byte aligned: two keys a read, eight reads in flight.
 __device__ __forceinline__ int count_larger(const uint64_t* keys, int n, uint64_t key) {
@@ -170,25 +208,31 @@ struct TopSearch {
     __attribute__((aligned(16))) uint64_t keys[kLpThreads];
     __attribute__((aligned(16))) uint64_t list[kCandidates + 1];
     int granules[kCandidates];
-    int chosen[kTopMax];
+    int chosen[kLpThreads];
     uint64_t floor_key;
     int count, lanes, listed;
 };
 
-// The bound below the k-th best and the lanes that reach it, from each lane's best key (0: it has none).
+// The bound below the k-th best and the lanes that reach it, from each lane's best key (0: it has none): the k-th best of the best
+// of four lanes each.  (The k-th best lane bounds a little closer, which is worth 1 % at 4096 x 151936 top 20, but finding it among
+// 256 took 2.9 us of the 15 of a single row.)
 __device__ __forceinline__ uint64_t top_bound(TopSearch& t, uint64_t mine, int k) {
+    static_assert(kLpThreads == 4 * kWave && kTopMax <= kWave, "a wave ranks the best of four lanes each");
     const int tid = threadIdx.x;
-    t.keys[tid] = mine;
+    auto word = [](uint32_t lo, uint32_t hi) { return (uint64_t)hi << 32 | lo; };
+    uint64_t four = larger(mine, word(across<0xB1>((uint32_t)mine), across<0xB1>((uint32_t)(mine >> 32))));
+    four = larger(four, word(across<0x4E>((uint32_t)four), across<0x4E>((uint32_t)(four >> 32))));
+    if (tid % 4 == 0) t.keys[tid / 4] = four;
     if (tid == 0) t.count = 0, t.lanes = 0, t.listed = 0, t.floor_key = 1;
     __syncthreads();
-    const int rank = count_larger(t.keys, kLpThreads, mine);
-    if (mine && rank < k) {
-        t.chosen[rank] = tid;
-        atomicAdd(&t.lanes, 1);
-        if (rank == k - 1) t.floor_key = mine;
+    if (tid < kWave) {
+        const uint64_t key = t.keys[tid];
+        if (key && count_larger(t.keys, kWave, key) == k - 1) t.floor_key = key;
     }
     __syncthreads();
-    return t.floor_key;
+    const uint64_t bound = t.floor_key;
+    if (mine >= bound) t.chosen[atomicAdd(&t.lanes, 1)] = tid;
+    return bound;
 }
 
 // Lists the logits of granule `at` that reach the bound.
@@ -312,13 +356,7 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
         walk(g0, g1, [](float, int) {});
     }
 
-    Sums all = t;
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-        const Sums o = {__shfl_xor(all.r, off, kWave), __shfl_xor(all.s, off, kWave), __shfl_xor(all.w, off, kWave)};
-        // the lower lane's first: both lanes of a pair get the same sum
-        all = (tid & off) ? join(o, all) : join(all, o);
-    }
+    Sums all = wave_join(t);
     if (tid % kWave == 0) wave_sums[tid / kWave] = all;
     __syncthreads();
     if (tid == 0) {
@@ -347,6 +385,7 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
             }
             __syncthreads();
             bound = top_bound(search, g0 + tid < g1 ? key_of(order_of(best), (uint32_t)best_g) : 0, a.k);
+            __syncthreads();
             end = g1;
         }
         const int turns = (end - g0 + kLpThreads - 1) / kLpThreads;
@@ -428,13 +467,8 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_join_kernel(Logprob
         if (tid < a.splits) t = sums[tid];
         const uint64_t best = a.k && tid < a.splits ? partial[tid * a.k] : 0;
         uint64_t last = a.k && tid < a.splits ? partial[tid * a.k + a.k - 1] : 0;
-#pragma unroll
-        for (int off = 1; off < kWave; off <<= 1) {
-            const Sums o = {__shfl_xor(t.r, off, kWave), __shfl_xor(t.s, off, kWave), __shfl_xor(t.w, off, kWave)};
-            t = (tid & off) ? join(o, t) : join(t, o);
-            const uint64_t other = __shfl_xor((unsigned long long)last, off, kWave);
-            last = other > last ? other : last;
-        }
+        t = wave_join(t);
+        last = wave_fold(last, larger);
         if (tid == 0) {
             const int target = a.targets[row];
             const bool given = target >= 0 && target < a.V;
