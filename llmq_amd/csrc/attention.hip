@@ -16,7 +16,7 @@
 // Bound: long sequences by the package's power.  1 x 8192 with 28 query and 4 key heads of 128: forward 465 us, 1.04 PFLOP/s of
 // allowed pairs, at 1.9 of 2.4 GHz with the matrix cores busy half of the cycles; backward 1590 us, 0.76 PFLOP/s, 1.06 with
 // the products computed twice.  (The library's product of two 8192 x 8192 bf16 matrices: 1.18.)  Deeper pipelining of the two
-// products, wave priorities and eight waves a workgroup left these times as they were.  Short ones by what a workgroup
+// products and eight waves a workgroup left these times as they were.  Short ones by what a workgroup
 // costs besides its walk: at 8 x 1024 (82 us, 0.73 PFLOP/s) 5 of its 23 us, and an eighth of the walk lies behind the diagonal.
 #include <climits>
 #include <type_traits>
@@ -321,6 +321,14 @@ __device__ __forceinline__ void mask_scores(f32x16 (&s)[2], const Block& w, int 
             if (!w.allowed(t, rb, i)) s[rb][i] = -__builtin_huge_valf();
 }
 
+// A wave in its matrix products goes before waves in their softmax, up to 64 dimensions, where the softmax is the longer part:
+// window 1 x 8192 forward 63.9 -> 61.9 us, backward (the keys' first products) 207 -> 201.5.  Above it costs: 8 x 1024 forward
+// 82.5 -> 85.8, backward 323 -> 324.5; so it does in the queries' backward pass: 201.4 -> 203.
+template <int HDP, int PRIORITY>
+__device__ __forceinline__ void matrix_priority() {
+    if constexpr (HDP == 64) __builtin_amdgcn_s_setprio(PRIORITY);
+}
+
 // ---- forward ------------------------------------------------------------------------------------------------------------
 // The careful form of a workgroup in which a value was not finite: 32 dimensions at a time, with the product that keeps masked
 // places out.  The statistics stand: the scores see no values.  (As a function of its own it cost 20 us a launch: a kernel that
@@ -382,7 +390,9 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_forward_kernel(Att
         const char* keys = w.keys(t & 1);
         char* values = w.values(t & 1);
         w.aim((t + 1) & 1, t + 1);
+        matrix_priority<HDP, 1>();
         tile_scores<HDP>(s, keys, here(row_lane_), qf, [&](int st) { w.issue(st); });
+        matrix_priority<HDP, 0>();
         if (!w.whole(t)) mask_scores(s, w, t);
         float top = -__builtin_huge_valf();
 #pragma unroll
@@ -415,10 +425,12 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_forward_kernel(Att
             pf[2 * rb + 1] = operand(s[rb], 1);
         }
         const int cols_lane = here(cols_lane_);
+        matrix_priority<HDP, 1>();
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
             for (int db = 0; db < W::kDims; ++db) o[db] = mfma(T::cols(values, cols_lane, db, u), pf[u], o[db]);
+        matrix_priority<HDP, 0>();
     }
 
     w.pass(t, INT_MAX);
@@ -855,7 +867,9 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_kernel
         }
         bf16x8 pf[2], dsf[2];
         uint32_t allowed;
+        matrix_priority<HDP, 1>();
         w.gradient(pf, dsf, allowed, buf, now.q0, whole, here(row_lane_), kf, [&](int st) { w.issue(st); });
+        matrix_priority<HDP, 0>();
         const int cols_lane = here(cols_lane_);
 #pragma unroll
         for (int db = 0; db < W::kDims; ++db)
