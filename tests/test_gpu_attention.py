@@ -3,9 +3,10 @@
 Bars, with u = 2^-8 (half a step of a bf16 rounding, relative to the value).  Forward: the scores are fp32, each probability is
 rounded to bf16 once (u of itself) and the result once more, so |err| <= u |out| + u sum_k p |v| plus fp32 terms: scores of
 head_dim products lose at most head_dim 2^-24 sum |q k| scale, which moves every probability by that factor, and the
-exponential and the sums 2^-20 together.  Backward: with the forward's rounded out, D is off by u sum_d |dout out|; p and ds are
-rounded once each, so  |err(dv)| <= u |dv| + u sum p |dout|;  |err(ds)| <= u |ds| + p (u sum_d |dout out|);  dq, dk from the sums
-of those times |k|, |q|, plus one rounding of the result.  Each bar is computed from the data below (`bars`)."""
+exponential and the sums 2^-20 together.  Backward: D comes from the forward's out, so it is off by sum_d |dout| err(out); p and ds
+are rounded once each, so  |err(dv)| <= u |dv| + u sum p |dout|;  |err(ds)| <= u |ds| + p err(D);  dq, dk from the sums of those
+times |k|, |q|, plus one rounding of the result.  Each bar is computed from the data below (`bars`), with the products of errors:
+the rounding of a value that is off by e is off by u (|x| + e)."""
 import math
 
 import pytest
@@ -79,11 +80,12 @@ def exact(qkv, dout, Nq, Nkv, first, scale=None):
     # bars.  w: relative change of a probability by the fp32 evaluation of its score, its row's lse and the exponential
     w = (HD * 2.0 ** -24 * scale * mm(q.norm(dim=-1, keepdim=True), k.norm(dim=-1, keepdim=True).transpose(2, 3)) + 2.0 ** -18)
     w = torch.where(mask, w + w.masked_fill(~mask, 0).amax(-1, keepdim=True), 0.0)
-    ep = p * (U + w)
-    bar_out = U * out.abs() * (1 + U) + mm(ep, v.abs())
-    eds = ds.abs() * (U + w) + p * (1 + U) * (U * (do * out).abs().sum(-1, keepdim=True) + HD * 2.0 ** -23 * mm(do.abs(), v.abs().transpose(2, 3)))
+    # a rounding is one of the value with its errors so far: u (|x| + e), so e becomes e (1 + u) + u |x|
+    ep = p * (w * (1 + U) + U)
+    bar_out = mm(ep, v.abs()) * (1 + U) + U * out.abs()
+    eds = ds.abs() * (w * (1 + U) + U) + p * (1 + w) * (1 + U) * ((do.abs() * bar_out).sum(-1, keepdim=True) + HD * 2.0 ** -23 * mm(do.abs(), v.abs().transpose(2, 3)))
     bars = [mm(eds, k.abs()) * scale, heads(mm(eds.transpose(2, 3), q.abs())) * scale, heads(mm(ep.transpose(2, 3), do.abs()))]
-    bars = [b + U * (1 + U) * y.abs() for b, y in zip(bars, grads)]
+    bars = [b * (1 + U) + U * y.abs() for b, y in zip(bars, grads)]
     join = lambda ys: torch.cat([y.permute(0, 2, 1, 3) for y in ys], 2).reshape(B, T, C)  # noqa: E731
     flat = lambda y: y.permute(0, 2, 1, 3).reshape(B, T, Nq * HD)  # noqa: E731
     return dict(out=flat(out), lse=lse, grad=join(grads), bar_out=flat(bar_out), bar_lse=w.amax(-1), bar_grad=join(bars))
