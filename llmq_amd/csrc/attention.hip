@@ -609,8 +609,11 @@ struct KeyBlock {
     static constexpr int kThreads = WAVES * kWave, kSteps = HDP / 16, kDims = HDP / 32, kBlock = 32 * WAVES;
     typedef Tile<HDP, kQueries> T;
     typedef Tile<HDP, kBlock> V;
-    // two buffers of a query tile and an output gradient tile, the values, two buffers of lse2, delta and first key
-    static constexpr int kValues = 4 * T::kBytes, kStats = kValues + V::kBytes, kLdsBytes = kStats + 2 * 3 * kQueries * 4;
+    // Pairs between two barriers: two where one workgroup fills the unit's LDS as it is (8 x 1024 320.5 -> 315.5 us), one where three
+    // share it (window 1 x 8192 198.5 us, with two 200.1).
+    static constexpr int kStage = HDP == 128 ? 2 : 1, kBuffers = 2 * kStage;
+    // buffers of a query tile, of an output gradient tile, the values, buffers of lse2, delta and first key
+    static constexpr int kValues = 2 * kBuffers * T::kBytes, kStats = kValues + V::kBytes, kLdsBytes = kStats + kBuffers * 3 * kQueries * 4;
     typedef TileCopy<HDP, kQueries, kThreads> Copy;
     static constexpr int kCopies = 2 * Copy::kCopies + 1;
     static_assert(kCopies <= kSteps, "a copy a step");
@@ -651,7 +654,7 @@ struct KeyBlock {
         const int kb1 = min(kb0 + kBlock, a.T) - 1;
         if (a.head_dim < HDP) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) T::template clear<kThreads>(lds + i * T::kBytes, tid);
+            for (int i = 0; i < 2 * kBuffers; ++i) T::template clear<kThreads>(lds + i * T::kBytes, tid);
             V::template clear<kThreads>(lds + kValues, tid);
             __syncthreads();
         }
@@ -699,7 +702,7 @@ struct KeyBlock {
         load_columns<HDP>(kf, base + min(key_, a.T - 1) * token + (int64_t)(a.Nq + kvh) * a.head_dim, lane, a.head_dim);
     }
     __device__ __forceinline__ char* queries(int buf) const { return lds + buf * T::kBytes; }
-    __device__ __forceinline__ char* gradients(int buf) const { return lds + (2 + buf) * T::kBytes; }
+    __device__ __forceinline__ char* gradients(int buf) const { return lds + (kBuffers + buf) * T::kBytes; }
     __device__ __forceinline__ const char* statistics(int buf, int which) const { return lds + kStats + (buf * 3 + which) * kQueries * 4; }
     // The first query of a pair and what its queries may look at.
     struct Pair {
@@ -737,7 +740,7 @@ struct KeyBlock {
     }
     __device__ __forceinline__ void issue(int i) const {
         if (i < Copy::kCopies) copy.copy(i, to, qofs, qnext);
-        else if (i < 2 * Copy::kCopies) copy.copy(i - Copy::kCopies, to + 2 * T::kBytes, gofs, gnext);
+        else if (i < 2 * Copy::kCopies) copy.copy(i - Copy::kCopies, to + kBuffers * T::kBytes, gofs, gnext);
         else if (i < kCopies) copy4(sto, sofs, snext, slanes);
     }
     __device__ __forceinline__ void issue_all() const {
@@ -840,11 +843,15 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_kernel
     bf16x8 kf[W::kSteps];
     w.load_keys(kf);   // its latency covers what follows
     w.begin();
-    typename W::Pair next;
+    typename W::Pair ahead[W::kStage];
     if (w.turns > 0) {
-        next = w.aimed();
-        w.aim(0);
-        w.issue_all();
+#pragma unroll
+        for (int i = 0; i < W::kStage; ++i) {
+            if (i > 0) w.advance(i < w.turns);
+            ahead[i] = w.aimed();
+            w.aim(i);
+            w.issue_all();
+        }
     }
     arrived(kf);
     const int row_lane_ = T::row_lane(w.lane), cols_lane_ = T::cols_lane(w.lane);
@@ -854,12 +861,14 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_kernel
     for (int db = 0; db < W::kDims; ++db) dk[db] = zero16(), dv[db] = zero16();
 #pragma nounroll
     for (int turn = 0; turn < w.turns; ++turn) {
-        copies_landed();
-        const int buf = turn & 1;
-        const typename W::Pair now = next;
-        w.advance(turn + 1 < w.turns);
-        next = w.aimed();
-        w.aim(buf ^ 1);
+        if (turn % W::kStage == 0) copies_landed();
+        const int buf = turn % W::kBuffers;
+        const typename W::Pair now = ahead[0];
+#pragma unroll
+        for (int i = 1; i < W::kStage; ++i) ahead[i - 1] = ahead[i];
+        w.advance(turn + W::kStage < w.turns);
+        ahead[W::kStage - 1] = w.aimed();
+        w.aim(buf ^ W::kStage);
         bool whole;
         if (!w.touches(now, whole)) {
             w.issue_all();
