@@ -88,6 +88,9 @@ __device__ __forceinline__ void copies_landed() {
     __syncthreads();
 }
 
+// Behind the last walk: no copy may outlive the workgroup.
+__device__ __forceinline__ void all_copies_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 // A tile of ROWS rows of HDP bf16 in LDS, row-major, the 16-byte chunks of a row XORed with a function of the row.  A fragment
 // read takes one chunk of 32 rows, 16 rows a cycle; a transposed read takes four chunks of four rows a cycle: the low bits of the
 // row move the high bits of the chunk, so that the four rows' 64 bytes and the 16 rows' 16 bytes each cover all 64 banks once.
