@@ -367,8 +367,10 @@ __device__ __forceinline__ uint32_t attention_forward_careful(W& w, const bf16x8
     return fold;
 }
 
+// Up to 64 dimensions four waves a SIMD, one register fewer than three would take: window 1 x 8192 60 -> 55.6 us, 16 x 512 20.3 ->
+// 17.4, but 8 x 1024, in one round of workgroups either way, 25.6 -> 26.6.  (The queries' backward pass spills at four.)
 template <int HDP, int WAVES>
-__global__ __launch_bounds__(WAVES * kWave, 2) void attention_forward_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(WAVES * kWave, HDP == 64 ? 4 : 2) void attention_forward_kernel(AttentionArgs a) {
     typedef QueryBlock<HDP, WAVES> W;
     typedef typename W::T T;
     __shared__ __attribute__((aligned(16))) char lds[W::kLdsBytes];
