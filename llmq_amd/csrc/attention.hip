@@ -13,11 +13,11 @@
 // one wave in a fixed order, without atomics, for two products computed twice (seven in place of five).  Rounded to bf16: the
 // probabilities and ds, as operands of the matrix instructions, and the results; scores, statistics and sums are fp32.
 //
-// Bound: long sequences by the package's power.  1 x 8192 with 28 query and 4 key heads of 128: forward 465 us, 1.04 PFLOP/s of
-// allowed pairs, at 1.9 of 2.4 GHz with the matrix cores busy half of the cycles; backward 1590 us, 0.76 PFLOP/s, 1.06 with
-// the products computed twice.  (The library's product of two 8192 x 8192 bf16 matrices: 1.18.)  Deeper pipelining of the two
-// products and eight waves a workgroup left these times as they were.  Short ones by what a workgroup
-// costs besides its walk: at 8 x 1024 (82 us, 0.73 PFLOP/s) 5 of its 23 us, and an eighth of the walk lies behind the diagonal.
+// Bound: long sequences by the package's power.  1 x 8192 with 28 query and 4 key heads of 128: forward 445 us, 1.08 PFLOP/s of
+// allowed pairs, at 1.9 of 2.4 GHz with the matrix cores busy half of the cycles; backward 1520 us, 0.79 PFLOP/s, 1.11 with
+// the products computed twice.  (The library's product of two 8192 x 8192 bf16 matrices: 1.18 to 1.25.)  Deeper pipelining of the
+// two products and eight waves a workgroup left these times as they were.  Short ones by what a workgroup costs besides its walk:
+// at 8 x 1024 (78 us, 0.77 PFLOP/s) 4 of its 21 us, and an eighth of the walk lies behind the diagonal.
 #include <climits>
 #include <type_traits>
 #include <utility>
