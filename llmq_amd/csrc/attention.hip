@@ -111,45 +111,31 @@ __device__ __forceinline__ bool all_finite(const f32x16& x) {
     return t == 0.f;
 }
 
-// What a wave's 32 NB queries may look at.
-template <int NB>
+// What a wave's 32 queries may look at.
 struct QueryMask {
-    int q[NB], first[NB];   // this lane's positions and their first keys (INT_MAX: empty, or behind the last row)
+    int q, first;           // this lane's position and its first key (INT_MAX: empty, or behind the last row)
     int lo, hi;             // smallest first key and largest position of the wave's rows that are not empty (lo > hi: none)
     int first_max, q_min;   // a tile [k0, k1] is whole for the wave if k0 >= first_max and k1 <= q_min
 
+    // the first key on its way
     __device__ __forceinline__ void load(const AttentionArgs& a, int b, int q0, int lane) {
         q_min = q0;
-        hi = q0 < a.T ? min(q0 + 32 * NB, a.T) - 1 : -1;
-        lo = q0 < a.T ? 0 : INT_MAX;
+        q = q0 + (lane & 31);
+        first = a.first_key ? a.first_key[(int64_t)b * a.T + min(q, a.T - 1)] : 0;
+    }
+    __device__ __forceinline__ void derive(const AttentionArgs& a) {
+        hi = q_min < a.T ? min(q_min + 32, a.T) - 1 : -1;
+        lo = q_min < a.T ? 0 : INT_MAX;
         first_max = 0;
-#pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            q[n] = q0 + 32 * n + (lane & 31);
-            first[n] = 0;
-        }
         if (a.first_key) {
-            int l = INT_MAX, m = 0, top = -1;
-#pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                if (q[n] < a.T) {
-                    first[n] = max(a.first_key[(int64_t)b * a.T + q[n]], 0);
-                    if (first[n] > q[n]) first[n] = INT_MAX;
-                    else top = max(top, q[n]);
-                    l = min(l, first[n]);
-                    m = max(m, first[n]);
-                } else {
-                    first[n] = INT_MAX;
-                }
-            }
-            lo = wave_min(l);
-            first_max = wave_max(m);
-            hi = wave_max(top);
+            first = q < a.T && first <= q ? max(first, 0) : INT_MAX;
+            lo = wave_min(first);
+            hi = wave_max(first <= q ? q : -1);
+            first_max = wave_max(q < a.T ? first : 0);
         }
     }
-    __device__ __forceinline__ bool touches(int k0, int k1) const { return k0 <= hi && k1 >= lo; }
     __device__ __forceinline__ bool whole(int k0, int k1) const { return k0 >= first_max && k1 <= q_min; }
-    __device__ __forceinline__ bool allowed(int n, int k) const { return k <= q[n] && k >= first[n]; }
+    __device__ __forceinline__ bool allowed(int k) const { return k <= q && k >= first; }
 };
 
 // Key of register i of row block rb of the tile that starts at k0.
@@ -205,7 +191,7 @@ struct QueryBlock {
     uint32_t ofs[Copy::kCopies];
     const char *knext, *vnext;  // of the tile that is being copied
     uint32_t to;                // and where
-    QueryMask<1> mask;
+    QueryMask mask;
     int t_lo, t_hi;             // tiles of the workgroup (t_lo > t_hi: none)
     int w_lo, w_hi;             // and of the wave
 
@@ -222,6 +208,7 @@ struct QueryBlock {
         token = (int64_t)(a.Nq + 2 * a.Nkv) * a.head_dim, stride = token * 2;
         base = a.qkv + b * a.T * token;
         kbase = base + (int64_t)(a.Nq + kvh) * a.head_dim;
+        mask.load(a, b, q0, lane);   // before the rows, which are waited for later
     }
     // What the rows look at, and the first copies.
     __device__ __forceinline__ void begin() {
@@ -229,7 +216,7 @@ struct QueryBlock {
 #pragma unroll
             for (int i = 0; i < 4; ++i) T::template clear<kThreads>(lds + i * T::kBytes, tid);
         }
-        mask.load(a, b, q0, lane);
+        mask.derive(a);
         int lo = 0, hi = min(block + kBlock, a.T) - 1;
         if (a.first_key) block_range<WAVES>(lo, hi, mask.lo, mask.hi);
         else if (a.head_dim < HDP) __syncthreads();
@@ -277,7 +264,7 @@ struct QueryBlock {
         load_columns<HDP>(f, tensor + row() * row_elements + (int64_t)head * a.head_dim, lane, a.head_dim);
     }
     __device__ __forceinline__ bool whole(int t) const { return mask.whole(t * kKeys, t * kKeys + kKeys - 1); }
-    __device__ __forceinline__ bool allowed(int t, int rb, int i) const { return mask.allowed(0, t * kKeys + tile_row(rb, i, lane)); }
+    __device__ __forceinline__ bool allowed(int t, int rb, int i) const { return mask.allowed(t * kKeys + tile_row(rb, i, lane)); }
     // ones in the places that count, as an operand
     __device__ __forceinline__ bf16x8 counted(int t, int rb, int u) const {
         f32x16 in;
@@ -285,10 +272,10 @@ struct QueryBlock {
         for (int i = 0; i < 16; ++i) in[i] = allowed(t, rb, i) ? 1.f : 0.f;
         return operand(in, u);
     }
-    __device__ __forceinline__ bool valid() const { return mask.q[0] < a.T; }
-    __device__ __forceinline__ int64_t statistic() const { return ((int64_t)b * a.Nq + head) * a.T + mask.q[0]; }
-    __device__ __forceinline__ uint16_t* out_row() const { return a.out + (((int64_t)b * a.T + mask.q[0]) * a.Nq + head) * a.head_dim; }
-    __device__ __forceinline__ uint16_t* dq_row() const { return a.dqkv + ((int64_t)b * a.T + mask.q[0]) * token + (int64_t)head * a.head_dim; }
+    __device__ __forceinline__ bool valid() const { return mask.q < a.T; }
+    __device__ __forceinline__ int64_t statistic() const { return ((int64_t)b * a.Nq + head) * a.T + mask.q; }
+    __device__ __forceinline__ uint16_t* out_row() const { return a.out + (((int64_t)b * a.T + mask.q) * a.Nq + head) * a.head_dim; }
+    __device__ __forceinline__ uint16_t* dq_row() const { return a.dqkv + ((int64_t)b * a.T + mask.q) * token + (int64_t)head * a.head_dim; }
 };
 
 constexpr int kAhead = 2;   // steps that fragments are read ahead of their matrix instructions
@@ -557,7 +544,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_q_kernel(
         }
         // what the wave's rows may look at, for the walk over the queries; one head of the row writes it
         if (a.first_key && w.head == 0 && w.valid() && w.lane == 0)
-            a.groups[(int64_t)w.b * ((a.T + 31) / 32) + w.mask.q[0] / 32] = make_int2(w.mask.lo, w.mask.first_max);
+            a.groups[(int64_t)w.b * ((a.T + 31) / 32) + w.mask.q / 32] = make_int2(w.mask.lo, w.mask.first_max);
     }
     const int row_lane_ = T::row_lane(w.lane), cols_lane_ = T::cols_lane(w.lane);
 
@@ -623,6 +610,7 @@ struct KeyBlock {
     char* lds;
     uint32_t lds_at;
     int tid, lane, wave, b, kvh, kb0, split, splits, k0, k1, ng;
+    int2 early;                               // the lane's first entry of the groups
     float* partial;                           // the share's partial sums, or null: the gradients
     int turns;                                // pairs of the share
     int64_t token, stride, ostride;
@@ -649,6 +637,9 @@ struct KeyBlock {
         key_ = k0 + (lane & 31);
         token = (int64_t)(a.Nq + 2 * a.Nkv) * a.head_dim, stride = token * 2, ostride = (int64_t)a.Nq * a.head_dim * 2;
         base = a.qkv + b * a.T * token;
+        ng = (a.T + 31) / 32;
+        early = make_int2(INT_MAX, 0);
+        if (a.first_key && kb0 / kQueries + tid < ng) early = a.groups[(int64_t)b * ng + kb0 / kQueries + tid];   // before the keys
     }
     // The pairs that look at the keys, and the copies of the values.
     __device__ __forceinline__ void begin() {
@@ -660,12 +651,11 @@ struct KeyBlock {
             __syncthreads();
         }
         // the query tiles that look at any of the workgroup's keys lie in [t_lo, t_hi]
-        ng = (a.T + 31) / 32;
         int t_lo = kb0 / kQueries, t_hi = ng - 1;
         if (a.first_key) {
             int l = INT_MAX, h = -1;
             for (int g = t_lo + tid; g < ng; g += kThreads)
-                if (a.groups[(int64_t)b * ng + g].x <= kb1) {
+                if ((g == t_lo + tid ? early : a.groups[(int64_t)b * ng + g]).x <= kb1) {
                     l = min(l, g);
                     h = max(h, g);
                 }

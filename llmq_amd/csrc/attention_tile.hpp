@@ -1,7 +1,7 @@
 // Building blocks of the attention kernels: bf16 matrix-instruction fragments, the LDS tile with its swizzle, staging from
 // global memory, and the careful product for tiles with masked places.
 //
-// Everything is computed TRANSPOSED: a wave owns 32 (or 64) positions of one side as the COLUMNS of v_mfma_f32_32x32x16_bf16
+// Everything is computed TRANSPOSED: a wave owns 32 positions of one side as the COLUMNS of v_mfma_f32_32x32x16_bf16
 // results and walks tiles of the other side as rows.  Lane l = 32 h + c of a result holds column c and the 16 rows
 // 8 (i / 4) + 4 h + i % 4.  Two things follow.  Softmax statistics belong to a column, that is to a lane and its partner
 // c + 32: no reduction over lanes but one exchange of halves.  And a result is, after rounding to bf16, the right-hand operand
