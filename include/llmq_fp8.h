@@ -454,7 +454,9 @@ int llmq_attention_backward_bf16(uint16_t* dqkv, const uint16_t* dout, const uin
  *     wanted (pointers may be NULL), k <= 32.  With V < k, or NaN among the logits, the places left over hold -1 and -inf
  *     (NaN where lse is NaN).
  * -inf logits (banned tokens) have probability 0 and add nothing; a row of nothing else has lse and logp -inf and entropy 0.  A
- * row that holds NaN or +inf has NaN for lse, logp and entropy.  All sums fp32 in a fixed order (deterministic).
+ * row that holds NaN or +inf has NaN for lse, logp and entropy.  Finite logits count as they are, whatever their size (masks of
+ * -1e10, the type's lowest value); lse and what is formed from it, logp, top_logp and the gradient's p_v, carry lse's rounding to
+ * fp32, 2^-24 |lse|.  All sums fp32 in a fixed order (deterministic).
  * scratch: at least llmq_token_logprobs_scratch_bytes(N, V, k) bytes (0 for many rows: may be NULL), 16-byte aligned,
  * overwritten by every call; calls that share it must be stream ordered.  logits 16-byte aligned, any P.
  */

@@ -12,8 +12,9 @@
 // Forward: one pass with a running reference r and sums in base 2.  With d = (x - r) log2 e,
 //     s = sum 2^d,   w = sum d 2^d,   lse = r + log2(s) ln 2,   entropy = (log2 s - w / s) ln 2.
 // A lane's reference only follows a logit that has outgrown it by 11 (a factor of 6e4), so the sums are rarely rescaled; fp32
-// sums lose nothing by a common factor.  d is one fused multiply-add, x log2 e - r log2 e; where r log2 e might overflow (a row of
-// the type's lowest value, a common mask) x - r is formed first.
+// sums lose nothing by a common factor.  x - r is formed before the product: x log2 e - r log2 e as one fused multiply-add is an
+// instruction less, but off by the rounding of r log2 e, 2^-24 of it, and 2^d is an infinity or 0 from |r| = 1e10 on, a common mask
+// value.  It was no faster either: 4096 x 151936 top 5 228.7 us, this way 229.4; 777 x 50257 fp32 31.0 and 29.8.
 //
 // The k most likely tokens need no second pass over the row.  In the first turns (about the square root of all of a lane's
 // turns) each lane keeps the largest logit of its granules of 16 bytes and the first granule that holds it.  The k-th best of
@@ -265,8 +266,7 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
     const int g0 = (int)((int64_t)x.granules * split / a.splits), g1 = (int)((int64_t)x.granules * (split + 1) / a.splits);
 
     Sums t = {-__builtin_huge_valf(), 0.f, 0.f};
-    float ref = 0.f, ref2 = 0.f, best = -__builtin_huge_valf();
-    bool wide = false;   // a reference of the wave so large that its product with log2 e may overflow (masks of the lowest value)
+    float ref = 0.f, best = -__builtin_huge_valf();
     int best_g = g0 + tid;
     auto largest = [](const float (&v)[kN]) {
         float top = v[0];
@@ -282,23 +282,13 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs 
                 t.w = (t.w + d * t.s) * f;
                 t.s *= f;
                 t.r = ref = next;
-                ref2 = ref * kLog2eLp;
             }
-            wide = __any(!(__builtin_fabsf(ref) < 1e30f));
         }
-        if (!wide) {
 #pragma unroll
-            for (int j = 0; j < kN; ++j) {
-                const float d = __builtin_fmaf(v[j], kLog2eLp, -ref2), e = __builtin_amdgcn_exp2f(d);
-                t.s += e;
-                if constexpr (ENTROPY) t.w = __builtin_fmaf(__builtin_fmaxf(d, -1e4f), e, t.w);   // 0 times -inf is nothing
-            }
-        } else {
-            for (int j = 0; j < kN; ++j) {
-                const float d = (v[j] - ref) * kLog2eLp, e = __builtin_amdgcn_exp2f(d);
-                t.s += e;
-                if constexpr (ENTROPY) t.w = __builtin_fmaf(__builtin_fmaxf(d, -1e4f), e, t.w);
-            }
+        for (int j = 0; j < kN; ++j) {
+            const float d = (v[j] - ref) * kLog2eLp, e = __builtin_amdgcn_exp2f(d);
+            t.s += e;
+            if constexpr (ENTROPY) t.w = __builtin_fmaf(__builtin_fmaxf(d, -1e4f), e, t.w);   // 0 times -inf is nothing
         }
     };
     // granules [from, to) of the workgroup, each lane's in rising order, `see`(largest logit, granule) before the sums
