@@ -423,6 +423,7 @@ int llmq_adamw_update_f32(float* params, const float* grads, float* m, float* v,
  * A row without keys: out = 0, lse = -inf.  Scores and sums in fp32; the probabilities are rounded to bf16 for the product
  * with the values.  What lies in places the mask excludes never reaches a result, NaN and infinities included; where a value in
  * an allowed place is not finite, the outputs it enters are not finite either (NaN, also where the formula gives an infinity).
+ * Finite scores of any size are right as long as q_t . k_k, and s log2 e, are in the range of fp32; beyond it they count as not finite.
  * A score of -inf has probability 0, and a row of nothing else counts as one without keys (its gradients are NaN).
  * abs_max_or_null: reset, then max |out|, bit-identical to llmq_abs_max_bf16(out).  head_dim: a multiple of 8 up to 128;
  * softmax_scale > 0.  out and lse share no memory with each other and with qkv.

@@ -13,6 +13,13 @@
 // one wave in a fixed order, without atomics, for two products computed twice (seven in place of five).  Rounded to bf16: the
 // probabilities and ds, as operands of the matrix instructions, and the results; scores, statistics and sums are fp32.
 //
+// Exponents are one fused multiply-add, s scale2 - m scale2, scale2 = scale log2 e.  The second product is rounded, which moves all of
+// a row's exponents by up to 2^-24 of it: a common factor of no account, until at scores of 1e9 it is infinite or 0.  So beyond
+// |m scale2| = 2^14 the forward pass takes (s - m) scale2.  The backward pass, whose lse is a rounded number of its own, there takes
+// (s scale - lse) log2 e, which is 0 where lse came from this score alone; up to there its exponents are off by 2^-8 at most, which
+// is what the probabilities' rounding to 16 bits is.  Both only in the careful forms behind the walks: a branch in the forward walk
+// cost 1 x 8192 461.6 -> 465.9 us, at 64 dimensions 149 -> 153.
+//
 // Bound: long sequences by the package's power.  1 x 8192 with 28 query and 4 key heads of 128: forward 445 us, 1.08 PFLOP/s of
 // allowed pairs, at 1.9 of 2.4 GHz with the matrix cores busy half of the cycles; backward 1520 us, 0.79 PFLOP/s, 1.11 with
 // the products computed twice.  (The library's product of two 8192 x 8192 bf16 matrices: 1.18 to 1.25.)  Deeper pipelining of the
@@ -36,7 +43,7 @@ struct AttentionArgs {
     unsigned* abs_max;       // forward only, or NULL
     const uint16_t* dout;
     uint16_t* dqkv;
-    float* lse2;             // backward scratch: lse in base 2, [B, Nq, T]
+    float* lse2;             // backward scratch: fused_lse, [B, Nq, T]
     float* delta;            // D, [B, Nq, T]
     int* flags;              // per workgroup of the keys' kernel: whether a value was not finite
     int2* groups;            // with first_key: per 32 queries the smallest first key of a row that has any, the largest of all
@@ -47,6 +54,21 @@ struct AttentionArgs {
 };
 
 constexpr int kKeys = 64;    // rows of a staged tile
+
+constexpr float kFusedMost = 16384.f;   // base-2 scores beyond it are subtracted before they are scaled
+
+// The base-2 lse of a row for fused exponents, NaN beyond their range: every sum that the row enters is then NaN, and the careful form,
+// which computes such sums again, takes exponent().
+__device__ __forceinline__ float fused_lse(float lse) {
+    const float lse2 = lse * kLog2e, size = __builtin_fabsf(lse2);
+    return size > kFusedMost && __builtin_fabsf(lse) < __builtin_huge_valf() ? __builtin_nanf("") : lse2;
+}
+// The exponent of a probability from its score and the row's lse, whatever their size.  (No fused multiply-add: the score is rounded
+// as the forward pass rounded the one that lse came from.)
+__device__ __forceinline__ float exponent(float s, float lse, float scale, float scale2) {
+    const float lse2 = lse * kLog2e;
+    return __builtin_fabsf(lse2) > kFusedMost ? (s * scale - lse) * kLog2e : __builtin_fmaf(s, scale2, -lse2);
+}
 
 __device__ __forceinline__ int wave_min(int x) {
 #pragma unroll
@@ -273,6 +295,7 @@ struct QueryBlock {
         return operand(in, u);
     }
     __device__ __forceinline__ bool valid() const { return mask.q < a.T; }
+    __device__ __forceinline__ int64_t row_statistic() const { return ((int64_t)b * a.Nq + head) * a.T + row(); }
     __device__ __forceinline__ int64_t statistic() const { return ((int64_t)b * a.Nq + head) * a.T + mask.q; }
     __device__ __forceinline__ uint16_t* out_row() const { return a.out + (((int64_t)b * a.T + mask.q) * a.Nq + head) * a.head_dim; }
     __device__ __forceinline__ uint16_t* dq_row() const { return a.dqkv + ((int64_t)b * a.T + mask.q) * token + (int64_t)head * a.head_dim; }
@@ -318,37 +341,72 @@ __device__ __forceinline__ void matrix_priority() {
 }
 
 // ---- forward ------------------------------------------------------------------------------------------------------------
-// The careful form of a workgroup in which a value was not finite: 32 dimensions at a time, with the product that keeps masked
-// places out.  The statistics stand: the scores see no values.  (As a function of its own it cost 20 us a launch: a kernel that
-// calls one reserves scratch memory.)
+// Whether a row's largest score lies beyond the fused exponents.
+__device__ __forceinline__ bool beyond_fused(float m, float scale2) {
+    return __builtin_fabsf(m) < __builtin_huge_valf() && __builtin_fabsf(m * scale2) > kFusedMost;
+}
+__device__ __forceinline__ float row_lse(float m, float l, float scale, float scale2) {
+    const float log2l = __builtin_amdgcn_logf(l);
+    if (m == -__builtin_huge_valf() && l == 0.f) return m;
+    return beyond_fused(m, scale2) ? m * scale + log2l * kLn2 : (m * scale2 + log2l) * kLn2;   // the first as exponent() expects it
+}
+
+// The careful form of a workgroup in which a value was not finite or a score beyond the fused exponents: 32 dimensions at a time, with
+// the product that keeps masked places out.  The rows' largest scores stand; their sums l too, unless `sums`.  (As a function of its own
+// it cost 20 us a launch: a kernel that calls one reserves scratch memory.)
+template <typename W, typename F>
+__device__ __forceinline__ void careful_walk(W& w, F each) {
+    w.start();
+#pragma nounroll
+    for (int t = w.t_lo; t <= w.t_hi; ++t) {
+        w.aim(0, t);
+        w.issue_all();
+        copies_landed();
+        if (t >= w.w_lo && t <= w.w_hi) each(t);
+        __syncthreads();
+    }
+}
 template <int HDP, typename W>
-__device__ __forceinline__ uint32_t attention_forward_careful(W& w, const bf16x8 (&qf)[W::kSteps], float ref, float inv) {
+__device__ __forceinline__ uint32_t attention_forward_careful(W& w, const bf16x8 (&qf)[W::kSteps], float m, float l, bool sums) {
     typedef typename W::T T;
+    const float scale2 = w.a.scale2, ref = m == -__builtin_huge_valf() ? 0.f : m;
+    const bool far = beyond_fused(m, scale2);
+    auto probabilities = [&](f32x16 (&s)[2], int t) {
+        tile_scores<HDP>(s, w.keys(0), T::row_lane(here(w.lane)), qf, [](int) {});
+        mask_scores(s, w, t);
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                s[rb][i] = __builtin_amdgcn_exp2f(far ? (s[rb][i] - ref) * scale2 : __builtin_fmaf(s[rb][i], scale2, -(ref * scale2)));
+    };
+    if (sums) {
+        float sum = 0.f;
+        careful_walk(w, [&](int t) {
+            f32x16 s[2];
+            probabilities(s, t);
+#pragma unroll
+            for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sum += s[rb][i];
+        });
+        l = halves_sum(sum);
+        if (w.valid() && w.lane < 32) w.a.lse[w.statistic()] = row_lse(m, l, w.a.scale, scale2);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
     uint32_t fold = 0x7F807F80u;
 #pragma nounroll
     for (int db = 0; db < W::kDims; ++db) {
         f32x16 one = zero16();
-        w.start();
-#pragma nounroll
-        for (int t = w.t_lo; t <= w.t_hi; ++t) {
-            w.aim(0, t);
-            w.issue_all();
-            copies_landed();
-            if (t >= w.w_lo && t <= w.w_hi) {
-                f32x16 s[2];
-                tile_scores<HDP>(s, w.keys(0), T::row_lane(here(w.lane)), qf, [](int) {});
-                mask_scores(s, w, t);
+        careful_walk(w, [&](int t) {
+            f32x16 s[2];
+            probabilities(s, t);
 #pragma unroll
-                for (int rb = 0; rb < 2; ++rb) {
+            for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) s[rb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][i], w.a.scale2, -ref));
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                        one = careful_product(T::cols(w.values(0), T::cols_lane(here(w.lane)), db, 2 * rb + u), operand(s[rb], u), w.counted(t, rb, u), one);
-                }
-            }
-            __syncthreads();
-        }
+                for (int u = 0; u < 2; ++u)
+                    one = careful_product(T::cols(w.values(0), T::cols_lane(here(w.lane)), db, 2 * rb + u), operand(s[rb], u), w.counted(t, rb, u), one);
+        });
         fold = store_columns(w.out_row(), one, db, inv, w.lane, w.a.head_dim, w.valid(), fold);
     }
     return fold;
@@ -426,8 +484,7 @@ __global__ __launch_bounds__(WAVES * kWave, HDP == 64 ? 4 : 2) void attention_fo
     w.pass(t, INT_MAX);
 
     const float l = halves_sum(sum[0] + sum[1]), inv = l == 0.f ? 0.f : 1.f / l;
-    if (w.valid() && w.lane < 32)
-        a.lse[w.statistic()] = m == -__builtin_huge_valf() && l == 0.f ? m : (m * a.scale2 + __builtin_amdgcn_logf(l)) * kLn2;
+    if (w.valid() && w.lane < 32) a.lse[w.statistic()] = row_lse(m, l, a.scale, a.scale2);
     bool fine = true;
 #pragma unroll
     for (int db = 0; db < W::kDims; ++db) fine &= all_finite(o[db]);
@@ -438,8 +495,10 @@ __global__ __launch_bounds__(WAVES * kWave, HDP == 64 ? 4 : 2) void attention_fo
     uint16_t* row = w.out_row();
 #pragma unroll
     for (int db = 0; db < W::kDims; ++db) fold = store_columns(row, o[db], db, inv, w.lane, a.head_dim, w.valid(), fold);
-    if (__syncthreads_or(!fine)) {
-        fold = attention_forward_careful<HDP>(w, qf, m == -__builtin_huge_valf() ? 0.f : m * a.scale2, inv);
+    const bool far = beyond_fused(m, a.scale2);
+    if (__syncthreads_or(!fine || far)) {
+        const bool sums = __syncthreads_or(far || !(__builtin_fabsf(l) < __builtin_huge_valf()));
+        fold = attention_forward_careful<HDP>(w, qf, m, l, sums);
     }
     if (a.abs_max) {
         const uint32_t x = fold & 0xFFFFu, y = fold >> 16;
@@ -451,10 +510,11 @@ __global__ __launch_bounds__(WAVES * kWave, HDP == 64 ? 4 : 2) void attention_fo
 // dq, with D and the base-2 lse left for the other kernel.  The walk of the forward kernel with a third product:
 // transposed, s = K q, dp = V dout, dq = K^T ds.
 
-// ds of 32 keys (row block rb) of a tile as operands, 0 in the places the mask excludes; between(step) after each step
-template <int HDP, typename Block, typename F>
+// ds of 32 keys (row block rb) of a tile as operands, 0 in the places the mask excludes; between(step) after each step.  lse: of base 2
+// (fused_lse), or in the careful form the row's own.
+template <int HDP, bool CAREFUL, typename Block, typename F>
 __device__ __forceinline__ void query_gradient(bf16x8 (&dsf)[2], const Block& w, const char* keys, const char* values, int row_lane, int t, int rb,
-                                               bool whole, const bf16x8 (&qf)[HDP / 16], const bf16x8 (&gf)[HDP / 16], float lse2, float delta,
+                                               bool whole, const bf16x8 (&qf)[HDP / 16], const bf16x8 (&gf)[HDP / 16], float lse, float delta,
                                                F between) {
     typedef Tile<HDP, kKeys> T;
     constexpr int kSteps = HDP / 16;
@@ -474,7 +534,7 @@ __device__ __forceinline__ void query_gradient(bf16x8 (&dsf)[2], const Block& w,
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], w.a.scale2, -lse2));
+        const float p = __builtin_amdgcn_exp2f(CAREFUL ? exponent(s[i], lse, w.a.scale, w.a.scale2) : __builtin_fmaf(s[i], w.a.scale2, -lse));
         s[i] = p * (dp[i] - delta);
     }
     if (!whole) {
@@ -486,30 +546,22 @@ __device__ __forceinline__ void query_gradient(bf16x8 (&dsf)[2], const Block& w,
 }
 
 template <int HDP, typename W>
-__device__ __forceinline__ void attention_backward_q_careful(W& w, const bf16x8 (&qf)[W::kSteps], const bf16x8 (&gf)[W::kSteps], float lse2,
-                                                             float delta) {
+__device__ __forceinline__ void attention_backward_q_careful(W& w, const bf16x8 (&qf)[W::kSteps], const bf16x8 (&gf)[W::kSteps], float delta) {
     typedef typename W::T T;
+    const float lse = w.a.lse[w.row_statistic()];
 #pragma nounroll
     for (int db = 0; db < W::kDims; ++db) {
         f32x16 one = zero16();
-        w.start();
+        careful_walk(w, [&](int t) {
 #pragma nounroll
-        for (int t = w.t_lo; t <= w.t_hi; ++t) {
-            w.aim(0, t);
-            w.issue_all();
-            copies_landed();
-            if (t >= w.w_lo && t <= w.w_hi) {
-#pragma nounroll
-                for (int rb = 0; rb < 2; ++rb) {
-                    bf16x8 dsf[2];
-                    query_gradient<HDP>(dsf, w, w.keys(0), w.values(0), T::row_lane(here(w.lane)), t, rb, false, qf, gf, lse2, delta, [](int) {});
+            for (int rb = 0; rb < 2; ++rb) {
+                bf16x8 dsf[2];
+                query_gradient<HDP, true>(dsf, w, w.keys(0), w.values(0), T::row_lane(here(w.lane)), t, rb, false, qf, gf, lse, delta, [](int) {});
 #pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                        one = careful_product(T::cols(w.keys(0), T::cols_lane(here(w.lane)), db, 2 * rb + u), dsf[u], w.counted(t, rb, u), one);
-                }
+                for (int u = 0; u < 2; ++u)
+                    one = careful_product(T::cols(w.keys(0), T::cols_lane(here(w.lane)), db, 2 * rb + u), dsf[u], w.counted(t, rb, u), one);
             }
-            __syncthreads();
-        }
+        });
         store_columns(w.dq_row(), one, db, w.a.scale, w.lane, w.a.head_dim, w.valid(), 0u);
     }
 }
@@ -528,7 +580,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_q_kernel(
         w.load_rows(gf, a.dout + (int64_t)w.b * a.T * out_row, out_row);
         w.load_rows(of, a.out + (int64_t)w.b * a.T * out_row, out_row);
         w.load_rows(qf, w.base, w.token);
-        lse2 = a.lse[((int64_t)w.b * a.Nq + w.head) * a.T + w.row()] * kLog2e;
+        lse2 = fused_lse(a.lse[w.row_statistic()]);
         w.begin();
         arrived(gf), arrived(of), arrived(qf);
         float d = 0.f;
@@ -562,7 +614,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_q_kernel(
 #pragma unroll
         for (int rb = 0; rb < 2; ++rb) {
             bf16x8 dsf[2];
-            query_gradient<HDP>(dsf, w, keys, values, here(row_lane_), t, rb, whole, qf, gf, lse2, delta, [&](int st) {
+            query_gradient<HDP, false>(dsf, w, keys, values, here(row_lane_), t, rb, whole, qf, gf, lse2, delta, [&](int st) {
                 if (rb == 0) w.issue(st);
             });
             const int cols_lane = here(cols_lane_);
@@ -581,7 +633,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_q_kernel(
     uint16_t* row = w.dq_row();
 #pragma unroll
     for (int db = 0; db < W::kDims; ++db) store_columns(row, dq[db], db, a.scale, w.lane, a.head_dim, w.valid(), 0u);
-    if (__syncthreads_or(!fine)) attention_backward_q_careful<HDP>(w, qf, gf, lse2, delta);
+    if (__syncthreads_or(!fine)) attention_backward_q_careful<HDP>(w, qf, gf, delta);
 }
 
 // ---- backward: keys and values -------------------------------------------------------------------------------------------
@@ -641,8 +693,8 @@ struct KeyBlock {
         early = make_int2(INT_MAX, 0);
         if (a.first_key && kb0 / kQueries + tid < ng) early = a.groups[(int64_t)b * ng + kb0 / kQueries + tid];   // before the keys
     }
-    // The pairs that look at the keys, and the copies of the values.
-    __device__ __forceinline__ void begin() {
+    // The pairs that look at the keys, and the copies of the values.  lse: what gradient() takes for the rows' lse.
+    __device__ __forceinline__ void begin(const float* lse) {
         const int kb1 = min(kb0 + kBlock, a.T) - 1;
         if (a.head_dim < HDP) {
 #pragma unroll
@@ -671,7 +723,7 @@ struct KeyBlock {
         const int64_t head = kvh * a.G + head_, q0 = (int64_t)tile_ * kQueries, row = ((int64_t)b * a.Nq + head) * a.T;
         qnext = reinterpret_cast<const char*>(base + head * a.head_dim) + q0 * stride;
         gnext = reinterpret_cast<const char*>(a.dout + ((int64_t)b * a.T * a.Nq + head) * a.head_dim) + q0 * ostride;
-        snext = wave == 0 ? reinterpret_cast<const char*>(a.lse2 + row + q0)
+        snext = wave == 0 ? reinterpret_cast<const char*>(lse + row + q0)
                 : wave == 1 || !a.first_key ? reinterpret_cast<const char*>(a.delta + row + q0)
                                             : reinterpret_cast<const char*>(a.first_key + (int64_t)b * a.T + q0);
         const int64_t dim = a.head_dim * 2, shead = wave == 2 && a.first_key ? 0 : (int64_t)a.T * 4;
@@ -745,8 +797,9 @@ struct KeyBlock {
         return min(p.q0 + kQueries, a.T) - 1 >= k0 && lo <= k1 && k0 < a.T;
     }
     // p and ds of the tile in `buf` as operands.  allowed: which of this lane's 16 rows may look at its key, where not `whole`.
-    // One branch around the mask alone: two forms of the step would meet with the accumulators in different registers.
-    template <typename F>
+    // One branch around the mask alone: two forms of the step would meet with the accumulators in different registers.  The rows' lse is of
+    // base 2 (fused_lse), or in the careful form their own.
+    template <bool CAREFUL, typename F>
     __device__ __forceinline__ void gradient(bf16x8 (&pf)[2], bf16x8 (&dsf)[2], uint32_t& allowed, int buf, int q0, bool whole, int row_lane,
                                              const bf16x8 (&kf)[kSteps], F between) const {
         f32x16 s = zero16(), dp = zero16();
@@ -774,7 +827,7 @@ struct KeyBlock {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int i = 4 * j + e;
-                s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, -l[e]));
+                s[i] = __builtin_amdgcn_exp2f(CAREFUL ? exponent(s[i], l[e], a.scale, a.scale2) : __builtin_fmaf(s[i], a.scale2, -l[e]));
                 dp[i] = s[i] * (dp[i] - d[e]);
             }
         }
@@ -833,7 +886,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_kernel
     W w(a, lds, blockIdx.x % groups, rest / a.splits * W::kBlock, rest % a.splits, a.splits);
     bf16x8 kf[W::kSteps];
     w.load_keys(kf);   // its latency covers what follows
-    w.begin();
+    w.begin(a.lse2);
     typename W::Pair ahead[W::kStage];
     if (w.turns > 0) {
 #pragma unroll
@@ -868,7 +921,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_kv_kernel
         bf16x8 pf[2], dsf[2];
         uint32_t allowed;
         matrix_priority<HDP, 1>();
-        w.gradient(pf, dsf, allowed, buf, now.q0, whole, here(row_lane_), kf, [&](int st) { w.issue(st); });
+        w.template gradient<false>(pf, dsf, allowed, buf, now.q0, whole, here(row_lane_), kf, [&](int st) { w.issue(st); });
         matrix_priority<HDP, 0>();
         const int cols_lane = here(cols_lane_);
 #pragma unroll
@@ -956,7 +1009,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_join_kern
     if (split > 0) return;
     __shared__ __attribute__((aligned(16))) char lds[W::kLdsBytes];
     W start(a, lds, group, kb0, 0, 1);
-    start.begin();
+    start.begin(a.lse);
     bf16x8 kf[W::kSteps];
     start.load_keys(kf);
     arrived(kf);
@@ -974,7 +1027,7 @@ __global__ __launch_bounds__(WAVES * kWave, 2) void attention_backward_join_kern
             if (w.touches(now, whole)) {
                 bf16x8 pf[2], dsf[2];
                 uint32_t allowed;
-                w.gradient(pf, dsf, allowed, 0, now.q0, false, T::row_lane(w.lane), kf, [](int) {});
+                w.template gradient<true>(pf, dsf, allowed, 0, now.q0, false, T::row_lane(w.lane), kf, [](int) {});
                 f32x16 in;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) in[i] = (allowed >> i & 1) ? 1.f : 0.f;
