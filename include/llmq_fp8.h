@@ -437,7 +437,8 @@ int llmq_attention_forward_bf16(uint16_t* out, float* lse, const uint16_t* qkv, 
  * forward's out, lse, qkv and first_key.  The probabilities are recomputed from lse; with D = sum_d dout * out,
  *     p = exp(s - lse);  ds = p (dout . v - D);  dq = scale sum_k ds k;  dk = scale sum_{h, t} ds q;  dv = sum_{h, t} p dout
  * (sums of dk, dv over the query heads of the group).  p and ds are rounded to bf16 for their products, sums are fp32 in a
- * fixed order (deterministic), every element of dqkv is written.  Masked places as in the forward pass.
+ * fixed order (deterministic), every element of dqkv is written.  Masked places and scores as in the forward pass; sums beyond the
+ * range of fp32 (dout . v, D, the gradients before scale) count as not finite.
  * scratch: at least llmq_attention_backward_scratch_bytes(B, T, Nq, Nkv, head_dim) bytes, 16-byte aligned, overwritten by every
  * call; calls that share it must be stream ordered.  dqkv and the scratch share no memory with each other and the inputs.
  */

@@ -351,9 +351,7 @@ __device__ __forceinline__ float row_lse(float m, float l, float scale, float sc
     return beyond_fused(m, scale2) ? m * scale + log2l * kLn2 : (m * scale2 + log2l) * kLn2;   // the first as exponent() expects it
 }
 
-// The careful form of a workgroup in which a value was not finite or a score beyond the fused exponents: 32 dimensions at a time, with
-// the product that keeps masked places out.  The rows' largest scores stand; their sums l too, unless `sums`.  (As a function of its own
-// it cost 20 us a launch: a kernel that calls one reserves scratch memory.)
+// The walk of the careful forms, a tile at a time.
 template <typename W, typename F>
 __device__ __forceinline__ void careful_walk(W& w, F each) {
     w.start();
@@ -366,6 +364,11 @@ __device__ __forceinline__ void careful_walk(W& w, F each) {
         __syncthreads();
     }
 }
+
+// The careful form of a workgroup in which a value was not finite or a score beyond the fused exponents: 32 dimensions at a time, with
+// the product that keeps masked places out.  The rows' largest scores stand; their sums l too, unless `sums`.  Probabilities are divided
+// by l before the product: with values near the type's largest, sums of undivided ones overflow where their mean does not.  (As a
+// function of its own it cost 20 us a launch: a kernel that calls one reserves scratch memory.)
 template <int HDP, typename W>
 __device__ __forceinline__ uint32_t attention_forward_careful(W& w, const bf16x8 (&qf)[W::kSteps], float m, float l, bool sums) {
     typedef typename W::T T;
@@ -402,12 +405,15 @@ __device__ __forceinline__ uint32_t attention_forward_careful(W& w, const bf16x8
             f32x16 s[2];
             probabilities(s, t);
 #pragma unroll
-            for (int rb = 0; rb < 2; ++rb)
+            for (int rb = 0; rb < 2; ++rb) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[rb][i] *= inv;
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
                     one = careful_product(T::cols(w.values(0), T::cols_lane(here(w.lane)), db, 2 * rb + u), operand(s[rb], u), w.counted(t, rb, u), one);
+            }
         });
-        fold = store_columns(w.out_row(), one, db, inv, w.lane, w.a.head_dim, w.valid(), fold);
+        fold = store_columns(w.out_row(), one, db, 1.f, w.lane, w.a.head_dim, w.valid(), fold);
     }
     return fold;
 }

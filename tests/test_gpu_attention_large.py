@@ -151,3 +151,22 @@ def test_scores_of_every_size_in_one_row(K):
         assert ((out[0].double().view(T, 2, HD) - want[:, None]).abs() <= 3 * U * x[0, :, 3].double().abs().amax()).all()
         assert ((lse[0].double() - el).abs() <= 2.0 ** -22 * el.abs() + 2.0 ** -20).all()
         assert torch.isfinite(backward(K, qkv, dout, out, lse, 2, 1, None, SCALE)).all()
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_values_near_the_largest_of_their_type(K, shape):
+    """A mean of values is no larger than they are: sums of probabilities that are not yet divided may not be either.  Bars of `exact`."""
+    B, T, Nq, Nkv, HD = shape
+    for first in (None, first_keys("docs", B, T)):
+        for power in (100, 120, 124):
+            qkv, dout = make(*shape, seed=19)
+            x = qkv.view(B, T, Nq + 2 * Nkv, HD)
+            x[:, :, Nq + Nkv:] *= 2.0 ** power
+            assert torch.isfinite(qkv).all()
+            e = exact(qkv, dout, Nq, Nkv, first)
+            am, ref = torch.full((1,), 0.0, device="cuda"), torch.zeros(1, device="cuda")
+            out, lse = forward(K, qkv, Nq, Nkv, first, None, am)
+            assert ((out.double() - e["out"]).abs() <= e["bar_out"]).all()
+            assert ((lse.double() - e["lse"]).abs() <= e["bar_lse"] + 2.0 ** -22 * e["lse"].abs()).all()
+            K.abs_max(ref, out)
+            assert torch.equal(am, ref)
