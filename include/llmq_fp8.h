@@ -426,7 +426,7 @@ int llmq_adamw_update_f32(float* params, const float* grads, float* m, float* v,
  * Finite scores of any size are right as long as q_t . k_k, and s log2 e, are in the range of fp32; beyond it they count as not finite.
  * A score of -inf has probability 0, and a row of nothing else counts as one without keys (its gradients are NaN).
  * abs_max_or_null: reset, then max |out|, bit-identical to llmq_abs_max_bf16(out).  head_dim: a multiple of 8 up to 128;
- * softmax_scale > 0.  out and lse share no memory with each other and with qkv.
+ * softmax_scale > 0.  out, lse and abs_max share no memory with each other and with qkv and first_key.
  */
 int llmq_attention_forward_bf16(uint16_t* out, float* lse, const uint16_t* qkv, const int* first_key_or_null,
                                 float* abs_max_or_null, float softmax_scale, int B, int T, int Nq, int Nkv, int head_dim,

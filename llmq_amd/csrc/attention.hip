@@ -1065,9 +1065,9 @@ static int check_shape(const char* what, int B, int T, int Nq, int Nkv, int head
     return LLMQ_OK;
 }
 
-// whether two ranges of memory have nothing in common
+// whether two ranges of memory have nothing in common (one of no bytes has nothing)
 static bool apart(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
-    return static_cast<const char*>(a) + a_bytes <= static_cast<const char*>(b) || static_cast<const char*>(b) + b_bytes <= static_cast<const char*>(a);
+    return a_bytes == 0 || b_bytes == 0 || static_cast<const char*>(a) + a_bytes <= static_cast<const char*>(b) || static_cast<const char*>(b) + b_bytes <= static_cast<const char*>(a);
 }
 
 // Keys of a workgroup of the keys' kernel: as many waves as copy a tile of 32 queries with one load a thread.  Above 64 dimensions
@@ -1127,8 +1127,12 @@ extern "C" int llmq_attention_forward_bf16(uint16_t* out, float* lse, const uint
         LLMQ_REQUIRE(out && lse && qkv, "%s: null tensor pointer", what);
         LLMQ_REQUIRE(aligned16(out) && aligned16(qkv), "%s: pointers must be 16-byte aligned", what);
         const int64_t rows = (int64_t)B * T * head_dim * 2, all = rows * (Nq + 2 * Nkv), stat = (int64_t)B * T * Nq * 4;
-        LLMQ_REQUIRE(apart(out, rows * Nq, qkv, all) && apart(lse, stat, qkv, all) && apart(out, rows * Nq, lse, stat),
-                     "%s: out and lse must be memory of their own", what);
+        const int64_t first = first_key_or_null ? (int64_t)B * T * 4 : 0, slot = abs_max_or_null ? 4 : 0;
+        LLMQ_REQUIRE(apart(out, rows * Nq, qkv, all) && apart(lse, stat, qkv, all) && apart(out, rows * Nq, lse, stat) &&
+                         apart(out, rows * Nq, first_key_or_null, first) && apart(lse, stat, first_key_or_null, first) &&
+                         apart(abs_max_or_null, slot, out, rows * Nq) && apart(abs_max_or_null, slot, lse, stat) &&
+                         apart(abs_max_or_null, slot, qkv, all) && apart(abs_max_or_null, slot, first_key_or_null, first),
+                     "%s: out, lse and abs_max must be memory of their own", what);
     }
     if (abs_max_or_null) {
         hipLaunchKernelGGL(reset_slot_kernel, dim3(1), dim3(1), 0, st, reinterpret_cast<unsigned*>(abs_max_or_null));
@@ -1162,11 +1166,12 @@ extern "C" int llmq_attention_backward_bf16(uint16_t* dqkv, const uint16_t* dout
     LLMQ_REQUIRE(aligned16(dqkv) && aligned16(dout) && aligned16(out) && aligned16(qkv) && aligned16(scratch),
                  "%s: pointers must be 16-byte aligned", what);
     const int64_t rows = (int64_t)B * T * head_dim * 2, all = rows * (Nq + 2 * Nkv), stat = (int64_t)B * T * Nq * 4;
+    const int64_t first = first_key_or_null ? (int64_t)B * T * 4 : 0;
     const BackwardPlan p = backward_plan(B, T, Nq, Nkv, head_dim);
     LLMQ_REQUIRE(scratch_bytes >= (size_t)p.bytes, "%s: scratch buffer too small (%zu bytes, %lld needed)", what, scratch_bytes, (long long)p.bytes);
     for (const auto& to : {std::pair<const void*, int64_t>{dqkv, all}, {scratch, p.bytes}})
         LLMQ_REQUIRE(apart(to.first, to.second, qkv, all) && apart(to.first, to.second, dout, rows * Nq) && apart(to.first, to.second, out, rows * Nq) &&
-                         apart(to.first, to.second, lse, stat) && (to.first == dqkv || apart(to.first, to.second, dqkv, all)),
+                         apart(to.first, to.second, lse, stat) && apart(to.first, to.second, first_key_or_null, first) && (to.first == dqkv || apart(to.first, to.second, dqkv, all)),
                      "%s: dqkv and the scratch must be memory of their own", what);
     hipStream_t st = static_cast<hipStream_t>(stream);
     AttentionArgs a = make_args(qkv, first_key_or_null, B, T, Nq, Nkv, head_dim, softmax_scale);
