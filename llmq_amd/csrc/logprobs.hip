@@ -659,6 +659,10 @@ static int token_logprobs_backward_any(E* dlogits, const float* dlogp, const flo
         LLMQ_REQUIRE(aligned16(dlogits) && aligned16(logits), "%s: pointers must be 16-byte aligned", what);
         LLMQ_REQUIRE(dlogits == logits || dlogits + N64 * P <= logits || logits + N64 * P <= dlogits, "%s: dlogits must be logits or memory of its own", what);
     }
+    const int64_t granules = P / Granule<E>::kN + 2;   // at most, wherever a row begins
+    const int chunks = (int)((granules + kLpThreads * kGradTurns - 1) / (kLpThreads * kGradTurns));
+    const int64_t blocks = N64 * chunks;
+    LLMQ_REQUIRE(blocks < (1 << 24), "%s: tensor too large", what);   // the threads of a grid fit 32 bits
     if (abs_max) {
         hipLaunchKernelGGL(reset_slot_kernel, dim3(1), dim3(1), 0, stream, reinterpret_cast<unsigned*>(abs_max));
         LLMQ_HIP_TRY(hipGetLastError());
@@ -667,11 +671,7 @@ static int token_logprobs_backward_any(E* dlogits, const float* dlogp, const flo
     LogprobGradArgs a = {};
     a.dlogits = dlogits, a.logits = logits, a.dlogp = dlogp, a.dentropy = dentropy, a.targets = targets, a.lse = lse, a.entropy = entropy;
     a.abs_max = reinterpret_cast<unsigned*>(abs_max);
-    a.P = P, a.V = V;
-    const int64_t granules = P / Granule<E>::kN + 2;   // at most, wherever a row begins
-    a.chunks = (int)((granules + kLpThreads * kGradTurns - 1) / (kLpThreads * kGradTurns));
-    const int64_t blocks = N64 * a.chunks;
-    LLMQ_REQUIRE(blocks < (1 << 24), "%s: tensor too large", what);   // the threads of a grid fit 32 bits
+    a.P = P, a.V = V, a.chunks = chunks;
     auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kLpThreads), 0, stream, a); };
     if (dentropy) {
         if (abs_max) launch(token_logprobs_backward_kernel<E, true, true>);

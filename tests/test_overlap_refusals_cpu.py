@@ -40,3 +40,12 @@ def test_attention_refuses_first_keys_and_abs_max_inside_other_tensors(capi, p):
     for bad in (dqkv, dqkv + k - 4, dqkv - 28, scratch, scratch + need - 4, scratch - 28):
         assert backward(bad) == capi.LLMQ_ERR_INVALID_ARGUMENT, bad
         assert b"memory of their own" in capi.lib.llmq_last_error(), bad
+
+
+def test_token_logprobs_backward_refuses_before_it_touches_abs_max(capi, p):
+    """A grid that is too large is an error of the arguments, found before abs_max is reset (which needs a device)."""
+    for ty, rows in (("bf16", p), ("f32", p)):
+        f = getattr(capi.lib, "llmq_token_logprobs_backward_" + ty)
+        rc = f(rows, p, None, rows, p, p, None, p + 4096, (1 << 24) - 1, 64, 1 << 20, None)
+        assert rc == capi.LLMQ_ERR_INVALID_ARGUMENT, rc
+        assert b"too large" in capi.lib.llmq_last_error()
