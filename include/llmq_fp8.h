@@ -460,7 +460,8 @@ int llmq_attention_backward_bf16(uint16_t* dqkv, const uint16_t* dout, const uin
  * -1e10, the type's lowest value); lse and what is formed from it, logp, top_logp and the gradient's p_v, carry lse's rounding to
  * fp32, 2^-24 |lse|.  All sums fp32 in a fixed order (deterministic).
  * scratch: at least llmq_token_logprobs_scratch_bytes(N, V, k) bytes (0 for many rows: may be NULL), 16-byte aligned,
- * overwritten by every call; calls that share it must be stream ordered.  logits 16-byte aligned, any P.
+ * overwritten by every call; calls that share it must be stream ordered.  logits 16-byte aligned, any P.  Outputs and scratch share
+ * no memory with each other, logits (padded columns too) and targets.
  */
 int64_t llmq_token_logprobs_scratch_bytes(int64_t N, int V, int k);
 int llmq_token_logprobs_bf16(float* logp, float* entropy_or_null, float* lse, float* top_logp, int* top_ids,
@@ -476,8 +477,8 @@ int llmq_token_logprobs_f32(float* logp, float* entropy_or_null, float* lse, flo
  * rounded once; columns V .. P-1 are written as zeros.  lse (and, with dentropy, entropy) are the forward's.  dlogp counts as 0
  * for an ignored row; a row whose two gradients are 0 is written as zeros whatever its logits hold (padding), and so is a row
  * whose lse is -inf.
- * dlogits may be logits (in place), but not otherwise overlap them.  abs_max_or_null: reset, then max |dlogits| over all columns, bit-identical to llmq_abs_max
- * of the tensor.  The loss -mean logp has dlogp = -1 / N.
+ * dlogits may be logits (in place); dlogits and abs_max share no other memory with each other and the inputs.  abs_max_or_null: reset,
+ * then max |dlogits| over all columns, bit-identical to llmq_abs_max of the tensor.  The loss -mean logp has dlogp = -1 / N.
  */
 int llmq_token_logprobs_backward_bf16(uint16_t* dlogits, const float* dlogp, const float* dentropy_or_null,
                                       const uint16_t* logits, const int* targets, const float* lse, const float* entropy_or_null,

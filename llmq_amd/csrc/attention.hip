@@ -26,8 +26,6 @@
 // two products and eight waves a workgroup left these times as they were.  Short ones by what a workgroup costs besides its walk:
 // at 8 x 1024 (78 us, 0.77 PFLOP/s) 4 of its 21 us, and an eighth of the walk lies behind the diagonal.
 #include <climits>
-#include <type_traits>
-#include <utility>
 
 #include "common.hpp"
 #include "absmax_reduce.hpp"
@@ -1065,11 +1063,6 @@ static int check_shape(const char* what, int B, int T, int Nq, int Nkv, int head
     return LLMQ_OK;
 }
 
-// whether two ranges of memory have nothing in common (one of no bytes has nothing)
-static bool apart(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
-    return a_bytes == 0 || b_bytes == 0 || static_cast<const char*>(a) + a_bytes <= static_cast<const char*>(b) || static_cast<const char*>(b) + b_bytes <= static_cast<const char*>(a);
-}
-
 // Keys of a workgroup of the keys' kernel: as many waves as copy a tile of 32 queries with one load a thread.  Above 64 dimensions
 // eight, which read the queries half as often as four: 1 x 8192 1925 -> 1640 us, documents 283 -> 214, but 8 x 1024 331 -> 340.
 static int kv_block(int head_dim) { return head_dim > 64 ? 256 : 128; }
@@ -1127,12 +1120,9 @@ extern "C" int llmq_attention_forward_bf16(uint16_t* out, float* lse, const uint
         LLMQ_REQUIRE(out && lse && qkv, "%s: null tensor pointer", what);
         LLMQ_REQUIRE(aligned16(out) && aligned16(qkv), "%s: pointers must be 16-byte aligned", what);
         const int64_t rows = (int64_t)B * T * head_dim * 2, all = rows * (Nq + 2 * Nkv), stat = (int64_t)B * T * Nq * 4;
-        const int64_t first = first_key_or_null ? (int64_t)B * T * 4 : 0, slot = abs_max_or_null ? 4 : 0;
-        LLMQ_REQUIRE(apart(out, rows * Nq, qkv, all) && apart(lse, stat, qkv, all) && apart(out, rows * Nq, lse, stat) &&
-                         apart(out, rows * Nq, first_key_or_null, first) && apart(lse, stat, first_key_or_null, first) &&
-                         apart(abs_max_or_null, slot, out, rows * Nq) && apart(abs_max_or_null, slot, lse, stat) &&
-                         apart(abs_max_or_null, slot, qkv, all) && apart(abs_max_or_null, slot, first_key_or_null, first),
-                     "%s: out, lse and abs_max must be memory of their own", what);
+        const Range written[] = {{out, rows * Nq}, {lse, stat}, {abs_max_or_null, abs_max_or_null ? 4 : 0}};
+        const Range read[] = {{qkv, all}, {first_key_or_null, first_key_or_null ? (int64_t)B * T * 4 : 0}};
+        LLMQ_REQUIRE(apart(written, read), "%s: out, lse and abs_max must be memory of their own", what);
     }
     if (abs_max_or_null) {
         hipLaunchKernelGGL(reset_slot_kernel, dim3(1), dim3(1), 0, st, reinterpret_cast<unsigned*>(abs_max_or_null));
@@ -1166,13 +1156,11 @@ extern "C" int llmq_attention_backward_bf16(uint16_t* dqkv, const uint16_t* dout
     LLMQ_REQUIRE(aligned16(dqkv) && aligned16(dout) && aligned16(out) && aligned16(qkv) && aligned16(scratch),
                  "%s: pointers must be 16-byte aligned", what);
     const int64_t rows = (int64_t)B * T * head_dim * 2, all = rows * (Nq + 2 * Nkv), stat = (int64_t)B * T * Nq * 4;
-    const int64_t first = first_key_or_null ? (int64_t)B * T * 4 : 0;
     const BackwardPlan p = backward_plan(B, T, Nq, Nkv, head_dim);
     LLMQ_REQUIRE(scratch_bytes >= (size_t)p.bytes, "%s: scratch buffer too small (%zu bytes, %lld needed)", what, scratch_bytes, (long long)p.bytes);
-    for (const auto& to : {std::pair<const void*, int64_t>{dqkv, all}, {scratch, p.bytes}})
-        LLMQ_REQUIRE(apart(to.first, to.second, qkv, all) && apart(to.first, to.second, dout, rows * Nq) && apart(to.first, to.second, out, rows * Nq) &&
-                         apart(to.first, to.second, lse, stat) && apart(to.first, to.second, first_key_or_null, first) && (to.first == dqkv || apart(to.first, to.second, dqkv, all)),
-                     "%s: dqkv and the scratch must be memory of their own", what);
+    const Range written[] = {{dqkv, all}, {scratch, p.bytes}};
+    const Range read[] = {{qkv, all}, {dout, rows * Nq}, {out, rows * Nq}, {lse, stat}, {first_key_or_null, first_key_or_null ? (int64_t)B * T * 4 : 0}};
+    LLMQ_REQUIRE(apart(written, read), "%s: dqkv and the scratch must be memory of their own", what);
     hipStream_t st = static_cast<hipStream_t>(stream);
     AttentionArgs a = make_args(qkv, first_key_or_null, B, T, Nq, Nkv, head_dim, softmax_scale);
     a.out = const_cast<uint16_t*>(out), a.lse = const_cast<float*>(lse), a.dout = dout, a.dqkv = dqkv;

@@ -31,6 +31,28 @@ inline int hip_fail(hipError_t e, const char* what) {
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Whether two ranges of memory have nothing in common (one of no bytes has nothing).
+inline bool apart(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a_bytes == 0 || b_bytes == 0 || x + (uint64_t)a_bytes <= y || y + (uint64_t)b_bytes <= x;
+}
+// A tensor of a call: where it is, and its bytes (0: not there).
+struct Range {
+    const void* at;
+    int64_t bytes;
+};
+// Whether each of `written` has nothing in common with the others of them and with all of `read`.
+template <int W, int R>
+inline bool apart(const Range (&written)[W], const Range (&read)[R]) {
+    for (int i = 0; i < W; ++i) {
+        for (int j = 0; j < i; ++j)
+            if (!apart(written[i].at, written[i].bytes, written[j].at, written[j].bytes)) return false;
+        for (const Range& r : read)
+            if (!apart(written[i].at, written[i].bytes, r.at, r.bytes)) return false;
+    }
+    return true;
+}
+
 // Number of compute units of the current device (cached per device id).
 int cu_count();
 // Number of accelerator dies (XCDs) the device's compute units are spread over; workgroup ids are dealt to them

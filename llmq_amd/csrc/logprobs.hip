@@ -627,6 +627,10 @@ static int token_logprobs_any(float* logp, float* entropy, float* lse, float* to
     const int64_t need = logprob_scratch(N, V, k);
     LLMQ_REQUIRE(need == 0 || (scratch && aligned16(scratch) && scratch_bytes >= (size_t)need), "%s: scratch buffer too small or not 16-byte aligned (%zu bytes, %lld needed)",
                  what, scratch_bytes, (long long)need);
+    const int64_t row = (int64_t)N * 4;
+    const Range written[] = {{logp, row}, {entropy, entropy ? row : 0}, {lse, row}, {top_logp, row * k}, {top_ids, row * k}, {scratch, need}};
+    const Range read[] = {{logits, N * P * (int64_t)sizeof(E)}, {targets, row}};
+    LLMQ_REQUIRE(apart(written, read), "%s: the outputs and the scratch must be memory of their own", what);
     LogprobArgs a = {};
     a.logits = logits, a.targets = targets, a.logp = logp, a.entropy = entropy, a.lse = lse, a.top_logp = top_logp, a.top_ids = top_ids;
     a.scratch = scratch, a.P = P, a.N = N, a.V = V, a.k = k, a.splits = logprob_splits(N, V);
@@ -654,15 +658,19 @@ static int token_logprobs_backward_any(E* dlogits, const float* dlogp, const flo
     LLMQ_REQUIRE(N64 >= 0 && N64 < (1 << 24), "%s: fewer than 2^24 rows are wanted (got %lld)", what, (long long)N64);
     LLMQ_REQUIRE(V >= 1 && V <= (1 << 28) && P >= V && P <= (1 << 28), "%s: vocabulary %d, row length %lld: 1 <= V <= P <= 2^28 is wanted", what, V, (long long)P);
     LLMQ_REQUIRE(!dentropy || entropy || N64 == 0, "%s: dentropy needs the forward's entropy", what);
-    if (N64 > 0) {
-        LLMQ_REQUIRE(dlogits && dlogp && logits && targets && lse, "%s: null tensor pointer", what);
-        LLMQ_REQUIRE(aligned16(dlogits) && aligned16(logits), "%s: pointers must be 16-byte aligned", what);
-        LLMQ_REQUIRE(dlogits == logits || dlogits + N64 * P <= logits || logits + N64 * P <= dlogits, "%s: dlogits must be logits or memory of its own", what);
-    }
     const int64_t granules = P / Granule<E>::kN + 2;   // at most, wherever a row begins
     const int chunks = (int)((granules + kLpThreads * kGradTurns - 1) / (kLpThreads * kGradTurns));
     const int64_t blocks = N64 * chunks;
     LLMQ_REQUIRE(blocks < (1 << 24), "%s: tensor too large", what);   // the threads of a grid fit 32 bits
+    if (N64 > 0) {
+        LLMQ_REQUIRE(dlogits && dlogp && logits && targets && lse, "%s: null tensor pointer", what);
+        LLMQ_REQUIRE(aligned16(dlogits) && aligned16(logits), "%s: pointers must be 16-byte aligned", what);
+        const int64_t row = N64 * 4, all = N64 * P * (int64_t)sizeof(E);
+        const Range written[] = {{dlogits, all}, {abs_max, abs_max ? 4 : 0}};
+        const Range read[] = {{logits, dlogits == logits ? 0 : all}, {dlogp, row}, {dentropy, dentropy ? row : 0}, {targets, row}, {lse, row},
+                              {entropy, dentropy ? row : 0}};
+        LLMQ_REQUIRE(apart(written, read), "%s: dlogits must be logits or memory of its own, abs_max memory of its own", what);
+    }
     if (abs_max) {
         hipLaunchKernelGGL(reset_slot_kernel, dim3(1), dim3(1), 0, stream, reinterpret_cast<unsigned*>(abs_max));
         LLMQ_HIP_TRY(hipGetLastError());

@@ -49,3 +49,48 @@ def test_token_logprobs_backward_refuses_before_it_touches_abs_max(capi, p):
         rc = f(rows, p, None, rows, p, p, None, p + 4096, (1 << 24) - 1, 64, 1 << 20, None)
         assert rc == capi.LLMQ_ERR_INVALID_ARGUMENT, rc
         assert b"too large" in capi.lib.llmq_last_error()
+
+
+@pytest.mark.parametrize("ty,es", [("bf16", 2), ("f32", 4)])
+def test_token_logprobs_refuse_shared_memory(capi, p, ty, es):
+    N, V, P, k = 2, 10000, 10016, 3
+    f, b = getattr(capi.lib, "llmq_token_logprobs_" + ty), getattr(capi.lib, "llmq_token_logprobs_backward_" + ty)
+    need = capi.lib.llmq_token_logprobs_scratch_bytes(N, V, k)
+    assert need > 0
+    size = N * P * es
+    x = p + 8192
+
+    def forward(logp=p, ent=p + 256, lse=p + 512, top=p + 768, ids=p + 1024, targets=p + 1280, scratch=p + 2048, V=V, k=k):
+        return f(logp, ent, lse, top, ids, x, targets, scratch, need, N, V, P, k, None)
+
+    for name, start, n in (("logp", p, 4 * N), ("ent", p + 256, 4 * N), ("lse", p + 512, 4 * N), ("top", p + 768, 4 * N * k),
+                           ("ids", p + 1024, 4 * N * k), ("targets", p + 1280, 4 * N), ("scratch", p + 2048, need)):
+        own = {"logp": 4 * N, "ent": 4 * N, "lse": 4 * N, "top": 4 * N * k, "ids": 4 * N * k, "targets": 4 * N, "scratch": need}
+        for other in own:
+            if other == name or (name == "targets" and other == "targets"):
+                continue
+            for at in (start, start + n - 4, start - own[other] + 4):
+                if other == "scratch":
+                    at &= ~15
+                if at < start + n and start < at + own[other]:
+                    assert forward(**{other: at}) == capi.LLMQ_ERR_INVALID_ARGUMENT, (name, other, at - p)
+                    assert b"memory of their own" in capi.lib.llmq_last_error(), (name, other)
+        if name != "targets":
+            for at in (x, (x + size - 4) & ~15 if name == "scratch" else x + size - 4):
+                assert forward(**{name: at}) == capi.LLMQ_ERR_INVALID_ARGUMENT, (name, at - x)
+                assert b"memory of their own" in capi.lib.llmq_last_error(), name
+
+    d = p + 262144
+
+    def backward(dlogits=d, dlogp=p, dent=p + 256, targets=p + 512, lse=p + 768, ent=p + 1024, am=p + 1280):
+        return b(dlogits, dlogp, dent, x, targets, lse, ent, am, N, V, P, None)
+
+    for name in ("dlogp", "dent", "targets", "lse", "ent", "am"):
+        for base in (d, x) if name == "am" else (d,):
+            for at in (base, base + size - 4) + ((base - 4 * N + 4,) if name != "am" else ()):
+                assert backward(**{name: at}) == capi.LLMQ_ERR_INVALID_ARGUMENT, (name, at - base)
+                assert b"memory of" in capi.lib.llmq_last_error() and b"own" in capi.lib.llmq_last_error(), name
+    for at in (p, p + 4, p + 256, p + 512, p + 768, p + 1028):
+        assert backward(am=at) == capi.LLMQ_ERR_INVALID_ARGUMENT, at - p
+    for at in (p, p + 4):
+        assert backward(dlogits=x, am=at) == capi.LLMQ_ERR_INVALID_ARGUMENT
