@@ -366,7 +366,7 @@ __device__ __forceinline__ void careful_walk(W& w, F each) {
 // The careful form of a workgroup in which a value was not finite or a score beyond the fused exponents: 32 dimensions at a time, with
 // the product that keeps masked places out.  The rows' largest scores stand; their sums l too, unless `sums`.  Probabilities are divided
 // by l before the product: with values near the type's largest, sums of undivided ones overflow where their mean does not.  (As a
-// function of its own it cost 20 us a launch: a kernel that calls one reserves scratch memory.)
+// function of its own, which the compiler gives a stack, it cost 20 us a launch.)
 template <int HDP, typename W>
 __device__ __forceinline__ uint32_t attention_forward_careful(W& w, const bf16x8 (&qf)[W::kSteps], float m, float l, bool sums) {
     typedef typename W::T T;
@@ -416,8 +416,9 @@ __device__ __forceinline__ uint32_t attention_forward_careful(W& w, const bf16x8
     return fold;
 }
 
-// Up to 64 dimensions four waves a SIMD, one register fewer than three would take: window 1 x 8192 60 -> 55.6 us, 16 x 512 20.3 ->
-// 17.4, but 8 x 1024, in one round of workgroups either way, 25.6 -> 26.6.  (The queries' backward pass spills at four.)
+// Up to 64 dimensions four waves a SIMD, in 128 registers for the 129 that three would take: window 1 x 8192 60.3 -> 56.4 us, 16 x 512
+// 20.3 -> 17.5, but 8 x 1024, in one round of workgroups either way, 26.4 -> 27.0, and 1 x 8192 144.9 -> 146.4.  (The queries' backward
+// pass spills vector registers at four.)
 template <int HDP, int WAVES>
 __global__ __launch_bounds__(WAVES * kWave, HDP == 64 ? 4 : 2) void attention_forward_kernel(AttentionArgs a) {
     typedef QueryBlock<HDP, WAVES> W;
@@ -497,8 +498,9 @@ __global__ __launch_bounds__(WAVES * kWave, HDP == 64 ? 4 : 2) void attention_fo
     // 79.8 -> 77.9 us); the careful form stores over it.
     all_copies_landed();
     uint16_t* row = w.out_row();
+    const int lane = here(w.lane);   // its offsets into a row are derived again: kept since the loads they spill (16 x 512 17.5 -> 17.8 us)
 #pragma unroll
-    for (int db = 0; db < W::kDims; ++db) fold = store_columns(row, o[db], db, inv, w.lane, a.head_dim, w.valid(), fold);
+    for (int db = 0; db < W::kDims; ++db) fold = store_columns(row, o[db], db, inv, lane, a.head_dim, w.valid(), fold);
     const bool far = beyond_fused(m, a.scale2);
     if (__syncthreads_or(!fine || far)) {
         const bool sums = __syncthreads_or(far || !(__builtin_fabsf(l) < __builtin_huge_valf()));
