@@ -35,36 +35,65 @@ whole 256-wide tiles, in the other three modes as well (a stored [K, M] and / or
 read in that storage, no transposed copy); other dtype combinations raise, as the reference does for what it does
 not implement.
 """
+import inspect
+
 import torch
 
 from . import kernels as _k
 
 MODE_TT, MODE_TN, MODE_NT, MODE_NN = 0, 1, 2, 3
 
+_library = torch.library.Library("llmq", "FRAGMENT")
 
-@torch.library.custom_op("llmq::abs_max", mutates_args=("scale",))
+
+def _register(name, mutates_args):
+    """Registers a function that writes `mutates_args` and returns nothing as the operator llmq::name, with the schema its annotations
+    and defaults give, and puts the operator in its place.
+
+    Not torch.library.custom_op: its count of a written tensor's versions looks every one of `mutates_args` up among the arguments,
+    but the dispatcher leaves out trailing ones that have their default value, and every call with an optional tensor left out, or
+    given as None, ended in an IndexError."""
+    def register(fn):
+        schema = torch.library.infer_schema(fn, mutates_args=mutates_args)
+        _library.define(name + schema, tags=(torch.Tag.pt2_compliant_tag,))
+        names = list(inspect.signature(fn).parameters)
+        written = [names.index(a) for a in mutates_args]
+
+        def run(*args):
+            fn(*args)
+            for i in written:
+                if i < len(args) and args[i] is not None and not args[i].is_inference():
+                    torch.autograd.graph.increment_version(args[i])
+
+        _library.impl(name, run, "CompositeExplicitAutograd")
+        torch.library.register_fake("llmq::" + name, lambda *args: None, lib=_library)
+        return getattr(torch.ops.llmq, name)
+    return register
+
+
+@_register("abs_max", ("scale",))
 def abs_max(scale: torch.Tensor, x: torch.Tensor, stream: int = 0) -> None:
     _k.abs_max(scale, x, stream)
 
 
-@torch.library.custom_op("llmq::quantize_with_abs_max", mutates_args=("out", "scale"))
+@_register("quantize_with_abs_max", ("out", "scale"))
 def quantize_with_abs_max(out: torch.Tensor, scale: torch.Tensor, x: torch.Tensor, abs_max: torch.Tensor,
                           stream: int = 0) -> None:
     _k.quantize_with_abs_max(out, scale, x, abs_max, stream)
 
 
-@torch.library.custom_op("llmq::quantize_and_transpose_with_abs_max", mutates_args=("out", "scale"))
+@_register("quantize_and_transpose_with_abs_max", ("out", "scale"))
 def quantize_and_transpose_with_abs_max(out: torch.Tensor, scale: torch.Tensor, x: torch.Tensor,
                                         abs_max: torch.Tensor, stream: int = 0) -> None:
     _k.quantize_and_transpose_with_abs_max(out, scale, x, abs_max, stream)
 
 
-@torch.library.custom_op("llmq::transpose", mutates_args=("dst",))
+@_register("transpose", ("dst",))
 def transpose(dst: torch.Tensor, src: torch.Tensor, stream: int = 0) -> None:
     _k.transpose(dst, src, stream)
 
 
-@torch.library.custom_op("llmq::matmul", mutates_args=("c", "workspace"))
+@_register("matmul", ("c", "workspace"))
 def matmul(c: torch.Tensor, a: torch.Tensor, b: torch.Tensor, bias: torch.Tensor | None,
            scale_a: torch.Tensor | None, scale_b: torch.Tensor | None, cublaslt_handle: int,
            workspace: torch.Tensor, mode: int, accumulate: bool = False, stream: int = 0) -> None:
@@ -86,62 +115,62 @@ def matmul(c: torch.Tensor, a: torch.Tensor, b: torch.Tensor, bias: torch.Tensor
               b_kmajor=mode in (MODE_TN, MODE_TT), a_kmajor=mode in (MODE_NN, MODE_TN))
 
 
-@torch.library.custom_op("llmq::backward_bias", mutates_args=("dbias", "dbias_buffer"))
+@_register("backward_bias", ("dbias", "dbias_buffer"))
 def backward_bias(dbias: torch.Tensor, dout: torch.Tensor, scale_a: torch.Tensor | None,
                   scale_b: torch.Tensor | None, dbias_buffer: torch.Tensor, stream: int = 0) -> None:
     _k.backward_bias(dbias, dout, scale_a, scale_b, dbias_buffer, stream)
 
 
-@torch.library.custom_op("llmq::swiglu_forward", mutates_args=("out", "abs_max"))
+@_register("swiglu_forward", ("out", "abs_max"))
 def swiglu_forward(out: torch.Tensor, inp: torch.Tensor, abs_max: torch.Tensor | None = None, stream: int = 0) -> None:
     _k.swiglu_forward(out, inp, abs_max, stream)
 
 
-@torch.library.custom_op("llmq::swiglu_forward_quant", mutates_args=("out", "scale"))
+@_register("swiglu_forward_quant", ("out", "scale"))
 def swiglu_forward_quant(out: torch.Tensor, scale: torch.Tensor, inp: torch.Tensor, abs_max: torch.Tensor,
                          stream: int = 0) -> None:
     _k.swiglu_forward_quant(out, scale, inp, abs_max, stream)
 
 
-@torch.library.custom_op("llmq::swiglu_backward", mutates_args=("dinp", "abs_max"))
+@_register("swiglu_backward", ("dinp", "abs_max"))
 def swiglu_backward(dinp: torch.Tensor, dout: torch.Tensor, inp: torch.Tensor, abs_max: torch.Tensor | None = None,
                     stream: int = 0) -> None:
     _k.swiglu_backward(dinp, dout, inp, abs_max, stream)
 
 
-@torch.library.custom_op("llmq::rmsnorm_forward", mutates_args=("out", "rms", "absmax"))
+@_register("rmsnorm_forward", ("out", "rms", "absmax"))
 def rmsnorm_forward(out: torch.Tensor, rms: torch.Tensor, inp: torch.Tensor, weight: torch.Tensor,
                     absmax: torch.Tensor | None = None, epsilon: float = 1e-6, stream: int = 0) -> None:
     _k.rmsnorm_forward(out, rms, inp, weight, absmax, epsilon, stream)
 
 
-@torch.library.custom_op("llmq::fused_residual_rmsnorm_forward", mutates_args=("residual", "normed", "rrms", "absmax"))
+@_register("fused_residual_rmsnorm_forward", ("residual", "normed", "rrms", "absmax"))
 def fused_residual_rmsnorm_forward(residual: torch.Tensor, normed: torch.Tensor, rrms: torch.Tensor, inp1: torch.Tensor,
                                    inp2: torch.Tensor, weight: torch.Tensor, absmax: torch.Tensor | None = None,
                                    epsilon: float = 1e-6, stream: int = 0) -> None:
     _k.fused_residual_rmsnorm_forward(residual, normed, rrms, inp1, inp2, weight, absmax, epsilon, stream)
 
 
-@torch.library.custom_op("llmq::rmsnorm_backward", mutates_args=("dinp", "dweight", "scratch", "absmax"))
+@_register("rmsnorm_backward", ("dinp", "dweight", "scratch", "absmax"))
 def rmsnorm_backward(dinp: torch.Tensor, dweight: torch.Tensor, scratch: torch.Tensor, dresidual: torch.Tensor,
                      dout: torch.Tensor, inp: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor,
                      absmax: torch.Tensor | None = None, stream: int = 0) -> None:
     _k.rmsnorm_backward(dinp, dweight, scratch, dresidual, dout, inp, weight, rstd, absmax, stream)
 
 
-@torch.library.custom_op("llmq::rope_forward", mutates_args=("out", "absmax"))
+@_register("rope_forward", ("out", "absmax"))
 def rope_forward(out: torch.Tensor, inp: torch.Tensor, freqs_cis: torch.Tensor, absmax: torch.Tensor | None = None,
                  Nq: int = 0, Nkv: int = 0, stream: int = 0) -> None:
     _k.rope_forward(out, inp, freqs_cis, absmax, Nq, Nkv, stream)
 
 
-@torch.library.custom_op("llmq::rope_backward", mutates_args=("dinp", "absmax"))
+@_register("rope_backward", ("dinp", "absmax"))
 def rope_backward(dinp: torch.Tensor, dout: torch.Tensor, freqs_cis: torch.Tensor, absmax: torch.Tensor | None = None,
                   Nq: int = 0, Nkv: int = 0, stream: int = 0) -> None:
     _k.rope_backward(dinp, dout, freqs_cis, absmax, Nq, Nkv, stream)
 
 
-@torch.library.custom_op("llmq::adamw_update", mutates_args=("params", "m", "v", "m_scales", "abs_max"))
+@_register("adamw_update", ("params", "m", "v", "m_scales", "abs_max"))
 def adamw_update(params: torch.Tensor, grads: torch.Tensor, m: torch.Tensor, v: torch.Tensor, learning_rate: float,
                  beta1: float, beta2: float, t: int, eps: float, weight_decay: float, grad_scale: torch.Tensor,
                  m_scales: torch.Tensor | None = None, abs_max: torch.Tensor | None = None, seed: int = 0,
@@ -150,13 +179,13 @@ def adamw_update(params: torch.Tensor, grads: torch.Tensor, m: torch.Tensor, v: 
                     seed, stream)
 
 
-@torch.library.custom_op("llmq::attention_forward", mutates_args=("out", "lse", "absmax"))
+@_register("attention_forward", ("out", "lse", "absmax"))
 def attention_forward(out: torch.Tensor, lse: torch.Tensor, inp: torch.Tensor, absmax: torch.Tensor | None = None, Nq: int = 0,
                       Nkv: int = 0, first_key: torch.Tensor | None = None, softmax_scale: float = 0.0, stream: int = 0) -> None:
     _k.attention_forward(out, lse, inp, absmax, Nq, Nkv, first_key, softmax_scale or None, stream)
 
 
-@torch.library.custom_op("llmq::attention_backward", mutates_args=("dinp", "scratch"))
+@_register("attention_backward", ("dinp", "scratch"))
 def attention_backward(dinp: torch.Tensor, dout: torch.Tensor, out: torch.Tensor, lse: torch.Tensor, inp: torch.Tensor,
                        scratch: torch.Tensor, Nq: int, Nkv: int, first_key: torch.Tensor | None = None,
                        softmax_scale: float = 0.0, stream: int = 0) -> None:
@@ -167,14 +196,14 @@ def get_attention_backward_scratch_size(B: int, T: int, Nq: int, Nkv: int, HD: i
     return _k.get_attention_backward_scratch_size(B, T, Nq, Nkv, HD)
 
 
-@torch.library.custom_op("llmq::token_logprobs", mutates_args=("logp", "entropy", "lse", "top_logp", "top_ids", "scratch"))
+@_register("token_logprobs", ("logp", "entropy", "lse", "top_logp", "top_ids", "scratch"))
 def token_logprobs(logp: torch.Tensor, entropy: torch.Tensor | None, lse: torch.Tensor, top_logp: torch.Tensor | None,
                    top_ids: torch.Tensor | None, logits: torch.Tensor, targets: torch.Tensor, scratch: torch.Tensor | None,
                    vocab: int = 0, stream: int = 0) -> None:
     _k.token_logprobs(logp, entropy, lse, top_logp, top_ids, logits, targets, scratch, vocab or None, stream)
 
 
-@torch.library.custom_op("llmq::token_logprobs_backward", mutates_args=("dlogits", "absmax"))
+@_register("token_logprobs_backward", ("dlogits", "absmax"))
 def token_logprobs_backward(dlogits: torch.Tensor, dlogp: torch.Tensor, dentropy: torch.Tensor | None, logits: torch.Tensor,
                             targets: torch.Tensor, lse: torch.Tensor, entropy: torch.Tensor | None,
                             absmax: torch.Tensor | None = None, vocab: int = 0, stream: int = 0) -> None:
