@@ -20,11 +20,12 @@
 // is what the probabilities' rounding to 16 bits is.  Both only in the careful forms behind the walks: a branch in the forward walk
 // cost 1 x 8192 461.6 -> 465.9 us, at 64 dimensions 149 -> 153.
 //
-// Bound: long sequences by the package's power.  1 x 8192 with 28 query and 4 key heads of 128: forward 445 us, 1.08 PFLOP/s of
-// allowed pairs, at 1.9 of 2.4 GHz with the matrix cores busy half of the cycles; backward 1520 us, 0.79 PFLOP/s, 1.11 with
-// the products computed twice.  (The library's product of two 8192 x 8192 bf16 matrices: 1.18 to 1.25.)  Deeper pipelining of the
-// two products and eight waves a workgroup left these times as they were.  Short ones by what a workgroup costs besides its walk:
-// at 8 x 1024 (78 us, 0.77 PFLOP/s) 4 of its 21 us, and an eighth of the walk lies behind the diagonal.
+// Bound: long sequences by the package's power.  1 x 8192 with 28 query and 4 key heads of 128, from box to box: forward 443 to 466 us,
+// 1.03 to 1.09 PFLOP/s of allowed pairs, at 1.9 of 2.4 GHz with the matrix cores busy 55 % of the cycles; backward 1525 to 1590 us, 0.76 to
+// 0.79 PFLOP/s, 1.06 to 1.10 with the products computed twice.  (The library's product of two 8192 x 8192 bf16 matrices: 1.18 to 1.25.)
+// Deeper pipelining of the two products and eight waves a workgroup left these times as they were.  Short ones by what a workgroup
+// costs besides its walk: forward 8 x 1024 (77 to 88 us, 0.68 to 0.78 PFLOP/s) 4 of its 21 us, and an eighth of the walk lies behind
+// the diagonal; of the keys' walk a sixth, and its waves wait 47 % of their cycles (matrix cores busy 33 %, LDS 25 %).
 #include <climits>
 
 #include "common.hpp"
